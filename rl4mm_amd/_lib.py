@@ -121,6 +121,55 @@ def build_bounds_library(force: bool = False) -> Path:
     return BOUNDS_LIB_PATH
 
 
+POLICY_LIB_PATH = CSRC / "liblobpolicy.so"
+POLICY_SOURCES = [CSRC / "policy_ops.hip", CSRC.parent.parent / "include" / "lobpolicy.h"]
+# -packed-fp32-ops: no v_pk_{add,mul,fma}_f32, some of whose forms are not reliable on this hardware
+POLICY_FLAGS = ["-O3", "--offload-arch=gfx950", "-fPIC", "-shared", "-std=c++17", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-Wno-unknown-warning-option"]
+_policy_binding = None
+
+
+def _policy_stale() -> bool:
+    return not POLICY_LIB_PATH.exists() or any(s.exists() and s.stat().st_mtime > POLICY_LIB_PATH.stat().st_mtime for s in POLICY_SOURCES)
+
+
+def build_policy_library(force: bool = False) -> Path:
+    """hipcc -> liblobpolicy.so (include/lobpolicy.h), in-tree like the simulator's library and replaced atomically under the same lock."""
+    if not force and not _policy_stale():
+        return POLICY_LIB_PATH
+    import fcntl
+    import tempfile
+
+    hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
+    if not os.path.exists(hipcc):
+        raise RuntimeError("hipcc was not found: cannot build the HIP library")
+    with open(CSRC / ".build.lock", "w") as lock:
+        fcntl.flock(lock, fcntl.LOCK_EX)
+        try:
+            if force or _policy_stale():
+                fd, tmp = tempfile.mkstemp(suffix=".so", dir=str(CSRC))
+                os.close(fd)
+                try:
+                    subprocess.check_call([hipcc, *POLICY_FLAGS, "-o", tmp, str(POLICY_SOURCES[0])], cwd=str(CSRC))
+                    os.replace(tmp, POLICY_LIB_PATH)
+                finally:
+                    if os.path.exists(tmp):
+                        os.unlink(tmp)
+        finally:
+            fcntl.flock(lock, fcntl.LOCK_UN)
+    return POLICY_LIB_PATH
+
+
+def policy_binding():
+    """The policy operators' library (rl4mm_amd/policy_ops.py); raises if it can neither be loaded nor built."""
+    global _policy_binding
+    if _policy_binding is None:
+        from . import _policy_capi
+
+        _one_hip_runtime()
+        _policy_binding = _policy_capi.Binding(build_policy_library())
+    return _policy_binding
+
+
 def bounds_binding() -> _capi.Binding:
     _one_hip_runtime()
     return _capi.Binding(build_bounds_library(), prefix="lobsim_")

@@ -1,0 +1,860 @@
+// policy_ops.hip - the HIP kernels (gfx950) behind include/lobpolicy.h and their C-ABI host side.
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <cstdarg>
+#include <cstdint>
+#include <cstdio>
+
+#include "../../include/lobpolicy.h"
+
+namespace {
+
+// ---------------------------------------------------------------------------------------------------------------------------
+// host: errors
+
+thread_local char g_error[256] = "";
+
+int fail(int code, const char* format, ...) {
+    va_list args;
+    va_start(args, format);
+    vsnprintf(g_error, sizeof g_error, format, args);
+    va_end(args);
+    return code;
+}
+
+int launched() {
+    hipError_t e = hipGetLastError();
+    return e == hipSuccess ? LOBPOLICY_OK : fail(LOBPOLICY_ERR_HIP, "launch: %s", hipGetErrorString(e));
+}
+
+#define REQUIRE(condition, ...) \
+    do { \
+        if (!(condition)) return fail(LOBPOLICY_ERR_ARG, __VA_ARGS__); \
+    } while (0)
+
+constexpr int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// ---------------------------------------------------------------------------------------------------------------------------
+// device: small tools
+
+typedef __bf16 bf16;
+
+template <class T, int W>
+struct alignas(sizeof(T) * W < 16 ? sizeof(T) * W : 16) Pack {
+    T v[W];
+};
+
+template <class T, int W>
+__device__ __forceinline__ void load_pack(const T* p, float* out) {
+    const Pack<T, W> x = *reinterpret_cast<const Pack<T, W>*>(p);
+#pragma unroll
+    for (int i = 0; i < W; ++i) out[i] = (float)x.v[i];
+}
+
+template <class T, int W>
+__device__ __forceinline__ void store_pack(T* p, const float* in) {
+    Pack<T, W> x;
+#pragma unroll
+    for (int i = 0; i < W; ++i) x.v[i] = (T)in[i];
+    *reinterpret_cast<Pack<T, W>*>(p) = x;
+}
+
+__device__ __forceinline__ float wave_sum(float x) {
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d);
+    return x;
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------
+// decay attention over segments
+//
+// One recurrence serves the forward pass and all three gradients: with "queries" a, "keys" b and "values" c,
+//     S = [cut] ? 0 : e^g S;   S += in_scale b_t c_t^T;   out_t = out_scale a_t^T S
+//   out  a = q,  b = k,  c = v   forwards,  S: the state
+//   dq   a = do, b = v,  c = k   forwards,  S: the state, transposed
+//   dk   a = v,  b = do, c = q   backwards, S: the state's gradient, transposed
+//   dv   a = k,  b = q,  c = do  backwards, S: the state's gradient
+// Forwards a token with a reset cuts what came before it.  Backwards the gradient passes from token t + 1 to token t with e^g, unless
+// t + 1 has a reset; what enters behind the last token (the gradient of the final state) enters without a decay, and what leaves
+// in front of token 0 (the gradient of the initial state) leaves with one.
+
+struct Rows {  // one operand: [steps][envs][heads][width], the last dimension contiguous
+    const void* data;
+    int64_t st, sn, sh;
+};
+
+struct Scan {
+    Rows a, b, c, out;
+    const float* log_decay;
+    const uint8_t* reset;
+    int64_t reset_st, reset_sn;
+    const int32_t* lengths;
+    const float* state_in;  // [envs][heads] matrices of da x dc, by the strides below
+    float* state_out;
+    int64_t in_row, in_col, out_row, out_col;
+    int64_t steps, envs;
+    int heads, da, dc;
+    float in_scale, out_scale;
+};
+
+__device__ __forceinline__ int64_t length_of(const Scan& s, int64_t n) {
+    if (!s.lengths) return s.steps;
+    const int64_t l = s.lengths[n];
+    return l < 0 ? 0 : (l > s.steps ? s.steps : l);
+}
+
+// The recurrence as it stands, a token at a time: one workgroup per environment and head, a column of the state per thread.
+template <class T, int DA, bool REVERSE>
+__global__ __launch_bounds__(128) void scan_tokens(Scan s) {
+    __shared__ float row_a[DA], row_b[DA];
+    const int64_t unit = blockIdx.x, n = unit / s.heads;
+    const int h = (int)(unit % s.heads), j = threadIdx.x;
+    const float decay = expf(s.log_decay[h]);
+    const int64_t length = length_of(s, n);
+    const T* a = (const T*)s.a.data + n * s.a.sn + h * s.a.sh;
+    const T* b = (const T*)s.b.data + n * s.b.sn + h * s.b.sh;
+    const T* c = (const T*)s.c.data + n * s.c.sn + h * s.c.sh;
+    T* out = (T*)s.out.data + n * s.out.sn + h * s.out.sh;
+    const uint8_t* reset = s.reset ? s.reset + n * s.reset_sn : nullptr;
+    const bool mine = j < s.dc;
+    float state[DA];
+#pragma unroll
+    for (int i = 0; i < DA; ++i) state[i] = s.state_in && mine && i < s.da ? s.state_in[unit * s.da * s.dc + i * s.in_row + j * s.in_col] : 0.f;
+    for (int64_t k = 0; k < length; ++k) {
+        const int64_t t = REVERSE ? length - 1 - k : k;
+        __syncthreads();
+        for (int i = j; i < DA; i += 128) {
+            row_a[i] = i < s.da ? (float)a[t * s.a.st + i] : 0.f;
+            row_b[i] = i < s.da ? (float)b[t * s.b.st + i] * s.in_scale : 0.f;
+        }
+        __syncthreads();
+        const float value = mine ? (float)c[t * s.c.st + j] : 0.f;
+        const bool cut = reset && (REVERSE ? k > 0 && reset[(t + 1) * s.reset_st] : reset[t * s.reset_st]);
+        const float carry = REVERSE && k == 0 ? 1.f : decay;
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < DA; ++i) {
+            state[i] = (cut ? 0.f : state[i] * carry) + row_b[i] * value;
+            if (i < s.da) sum += row_a[i] * state[i];
+        }
+        if (mine) out[t * s.out.st + j] = (T)(sum * s.out_scale);
+    }
+    if (mine) {
+        for (int64_t t = length; t < s.steps; ++t) out[t * s.out.st + j] = (T)0.f;
+        if (s.state_out) {
+            const bool leave = REVERSE && length > 0, cut = leave && reset && reset[0];
+#pragma unroll
+            for (int i = 0; i < DA; ++i)
+                if (i < s.da) s.state_out[unit * s.da * s.dc + i * s.out_row + j * s.out_col] = cut ? 0.f : (leave ? state[i] * decay : state[i]);
+        }
+    }
+}
+
+template <class T, int DA>
+int scan_launch(const Scan& s, bool reverse, hipStream_t stream) {
+    const dim3 grid((unsigned)(s.envs * s.heads));
+    if (reverse)
+        scan_tokens<T, DA, true><<<grid, 128, 0, stream>>>(s);
+    else
+        scan_tokens<T, DA, false><<<grid, 128, 0, stream>>>(s);
+    return launched();
+}
+
+template <class T>
+int scan_typed(const Scan& s, bool reverse, hipStream_t stream) {
+    if (s.da <= 32) return scan_launch<T, 32>(s, reverse, stream);
+    if (s.da <= 64) return scan_launch<T, 64>(s, reverse, stream);
+    return scan_launch<T, 128>(s, reverse, stream);
+}
+
+int scan(const lobpolicy_attention* a, const Scan& s, bool reverse, void* stream) {
+    return a->dtype == LOBPOLICY_BF16 ? scan_typed<bf16>(s, reverse, (hipStream_t)stream) : scan_typed<float>(s, reverse, (hipStream_t)stream);
+}
+
+int check_attention(const lobpolicy_attention* a) {
+    REQUIRE(a, "no description");
+    REQUIRE(a->dtype == LOBPOLICY_F32 || a->dtype == LOBPOLICY_BF16, "dtype %d", a->dtype);
+    REQUIRE(a->heads >= 1 && a->heads <= 65536, "heads = %d", a->heads);
+    REQUIRE(a->dk >= 1 && a->dk <= LOBPOLICY_MAX_HEAD && a->dv >= 1 && a->dv <= LOBPOLICY_MAX_HEAD, "dk = %d, dv = %d: 1 to %d", a->dk, a->dv, LOBPOLICY_MAX_HEAD);
+    REQUIRE(a->steps >= 1 && a->envs >= 1, "steps and envs are 1 or more");
+    REQUIRE(a->steps < (1ll << 31), "steps: at most 2^31 - 1");
+    REQUIRE(a->envs <= (1ll << 22) / a->heads, "envs x heads: at most 2^22");
+    REQUIRE(a->log_decay, "no log_decay");
+    return LOBPOLICY_OK;
+}
+
+Rows rows_of(const lobpolicy_operand& o) { return {o.data, o.stride_t, o.stride_n, o.stride_h}; }
+
+Scan scan_of(const lobpolicy_attention* a) {
+    Scan s = {};
+    s.log_decay = a->log_decay;
+    s.reset = a->reset;
+    s.reset_st = a->reset_stride_t;
+    s.reset_sn = a->reset_stride_n;
+    s.lengths = a->lengths;
+    s.steps = a->steps;
+    s.envs = a->envs;
+    s.heads = a->heads;
+    s.in_scale = s.out_scale = 1.f;
+    return s;
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------
+// decay attention, one token of every environment
+//
+// Reads and writes the state once: 8 dk dv bytes per environment and head, next to which the operands are nothing.  One workgroup per
+// environment and head; a thread holds VW neighbouring columns of every RG-th row, so that a wave moves whole rows.
+
+struct Step {
+    const void *q, *k, *v;
+    void* out;
+    int64_t q_sn, q_sh, k_sn, k_sh, v_sn, v_sh, out_sn, out_sh;
+    const float* log_decay;
+    const uint8_t *reset, *skip;
+    int64_t reset_sn;
+    float* state;
+    int heads, dk, dv;
+    float scale;
+};
+
+template <class T, int VW, int LPR>
+__global__ __launch_bounds__(256) void step_kernel(Step s) {
+    constexpr int RG = 256 / LPR;
+    __shared__ float part[RG][LPR * VW];
+    const int64_t unit = blockIdx.x, n = unit / s.heads;
+    const int h = (int)(unit % s.heads), col = (threadIdx.x % LPR) * VW, group = threadIdx.x / LPR;
+    const bool mine = col < s.dv;
+    T* out = (T*)s.out + n * s.out_sn + h * s.out_sh;
+    if (s.skip && s.skip[n]) {
+        if (mine && group == 0)
+            for (int i = 0; i < VW; ++i) out[col + i] = (T)0.f;
+        return;
+    }
+    const T* q = (const T*)s.q + n * s.q_sn + h * s.q_sh;
+    const T* k = (const T*)s.k + n * s.k_sn + h * s.k_sh;
+    const T* v = (const T*)s.v + n * s.v_sn + h * s.v_sh;
+    float* state = s.state + unit * s.dk * s.dv + col;
+    const bool fresh = s.reset && s.reset[n * s.reset_sn];
+    const float decay = expf(s.log_decay[h]);
+    float value[VW], sum[VW];
+#pragma unroll
+    for (int i = 0; i < VW; ++i) value[i] = mine ? (float)v[col + i] : 0.f, sum[i] = 0.f;
+    if (mine) {
+#pragma unroll 4
+        for (int row = group; row < s.dk; row += RG) {
+            float x[VW];
+            const float key = (float)k[row], query = (float)q[row];
+            if (fresh) {
+#pragma unroll
+                for (int i = 0; i < VW; ++i) x[i] = 0.f;
+            } else
+                load_pack<float, VW>(state + row * s.dv, x);
+#pragma unroll
+            for (int i = 0; i < VW; ++i) {
+                x[i] = x[i] * decay + key * value[i];
+                sum[i] += query * x[i];
+            }
+            store_pack<float, VW>(state + row * s.dv, x);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < VW; ++i) part[group][(threadIdx.x % LPR) * VW + i] = sum[i];
+    __syncthreads();
+    for (int c = threadIdx.x; c < s.dv; c += 256) {
+        float total = 0.f;
+        for (int g = 0; g < RG; ++g) total += part[g][c];
+        out[c] = (T)(total * s.scale);
+    }
+}
+
+template <class T>
+int step_typed(const Step& s, int64_t units, hipStream_t stream) {
+    const dim3 grid((unsigned)units);
+    const bool wide = s.dv % 4 == 0 && (uintptr_t)s.state % 16 == 0;
+    if (wide && s.dv <= 32)
+        step_kernel<T, 4, 8><<<grid, 256, 0, stream>>>(s);
+    else if (wide && s.dv <= 64)
+        step_kernel<T, 4, 16><<<grid, 256, 0, stream>>>(s);
+    else if (wide)
+        step_kernel<T, 4, 32><<<grid, 256, 0, stream>>>(s);
+    else
+        step_kernel<T, 1, 128><<<grid, 256, 0, stream>>>(s);
+    return launched();
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------
+// the block's end
+//
+// Bound by memory: every operand is read once and every result written once.  A row lives in the registers of one wave (width up to 1024)
+// or of one workgroup, VW neighbouring elements per thread and step, E elements per thread in all; the sums are 32-bit.
+
+struct Block {
+    const void *x, *block, *gate, *grad_y, *grad_z;
+    int64_t x_sr, block_sr, gate_sr, grad_y_sr, grad_z_sr;
+    const float *post, *res, *pre;
+    void *y, *z, *grad_x, *grad_block, *grad_gate;
+    float* partial;  // [2][gridDim.x][width]
+    int64_t rows;
+    int width;
+    float eps;
+};
+
+template <int TPR>
+__device__ __forceinline__ void row_sums(float* v, int count, float* shared) {
+    for (int i = 0; i < count; ++i) v[i] = wave_sum(v[i]);
+    if (TPR > 64) {
+        __syncthreads();
+        if (threadIdx.x % 64 == 0)
+            for (int i = 0; i < count; ++i) shared[(threadIdx.x / 64) * 2 + i] = v[i];
+        __syncthreads();
+        for (int i = 0; i < count; ++i) v[i] = shared[i] + shared[2 + i] + shared[4 + i] + shared[6 + i];
+    }
+}
+
+template <class T, int VW, int E, int TPR>
+__device__ __forceinline__ void load_row(const T* row, int width, int lane, float* out) {
+#pragma unroll
+    for (int s = 0; s < E / VW; ++s) {
+        const int col = (s * TPR + lane) * VW;
+        if (row && col < width)
+            load_pack<T, VW>(row + col, out + s * VW);
+        else
+#pragma unroll
+            for (int i = 0; i < VW; ++i) out[s * VW + i] = 0.f;
+    }
+}
+
+template <class T, int VW, int E, int TPR>
+__device__ __forceinline__ void store_row(T* row, int width, int lane, const float* in) {
+#pragma unroll
+    for (int s = 0; s < E / VW; ++s) {
+        const int col = (s * TPR + lane) * VW;
+        if (col < width) store_pack<T, VW>(row + col, in + s * VW);
+    }
+}
+
+__device__ __forceinline__ float sigmoid(float u) { return 1.f / (1.f + expf(-u)); }
+
+template <class X, class B, int VW, int E, int TPR>
+__global__ __launch_bounds__(256) void block_forward_kernel(Block p) {
+    __shared__ float shared[8];
+    const int lane = threadIdx.x % TPR;
+    for (int64_t row = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR; row < p.rows; row += (int64_t)gridDim.x * (256 / TPR)) {
+        float x[E], b[E], g[E], w[E];
+        load_row<X, VW, E, TPR>((const X*)p.x + row * p.x_sr, p.width, lane, x);
+        load_row<B, VW, E, TPR>((const B*)p.block + row * p.block_sr, p.width, lane, b);
+        load_row<B, VW, E, TPR>(p.gate ? (const B*)p.gate + row * p.gate_sr : nullptr, p.width, lane, g);
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) sum += b[i] * b[i];
+        row_sums<TPR>(&sum, 1, shared);
+        const float rb = 1.f / sqrtf(sum / p.width + p.eps);
+#pragma unroll
+        for (int i = 0; i < E; ++i) b[i] *= rb * (p.gate ? sigmoid(g[i]) : 1.f);
+        load_row<float, VW, E, TPR>(p.post, p.width, lane, w);
+        load_row<float, VW, E, TPR>(p.res, p.width, lane, g);
+        sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            x[i] += g[i] * (w[i] * b[i]);
+            sum += x[i] * x[i];
+        }
+        store_row<X, VW, E, TPR>((X*)p.y + row * p.width, p.width, lane, x);
+        row_sums<TPR>(&sum, 1, shared);
+        const float ry = 1.f / sqrtf(sum / p.width + p.eps);
+        load_row<float, VW, E, TPR>(p.pre, p.width, lane, w);
+#pragma unroll
+        for (int i = 0; i < E; ++i) x[i] = x[i] * ry * w[i];
+        store_row<B, VW, E, TPR>((B*)p.z + row * p.width, p.width, lane, x);
+    }
+}
+
+// With bn = b / rms(b), yn = y / rms(y), sg = sigmoid(gate), f = the gradient of y, what came through z with it:
+//     f   = dy + (dz pre - yn mean(dz pre yn)) / rms(y)
+//     dx  = f;   dgate = f res bn post sg (1 - sg);   db = (e - bn mean(e bn)) / rms(b),  e = f res sg post
+//     dpre = sum dz yn;   m = sum f sg bn:  dpost = res m,  dres = post m
+// y is worked out again from x, b and the gate, which costs no memory.  A workgroup keeps its share of the two column sums in registers
+// over all its rows and writes it once; column_sums adds the workgroups' shares in their order.
+template <class X, class B, int VW, int E, int TPR>
+__global__ __launch_bounds__(256) void block_backward_kernel(Block p) {
+    constexpr int RPB = 256 / TPR;
+    __shared__ float shared[8];
+    __shared__ float fold[TPR == 64 ? 4 * 64 * E : 1];
+    const int lane = threadIdx.x % TPR;
+    float sum_m[E], sum_p[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) sum_m[i] = sum_p[i] = 0.f;
+    for (int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR; row < p.rows; row += (int64_t)gridDim.x * RPB) {
+        float x[E], b[E], g[E], dy[E], dz[E], w[E], sums[2];
+        load_row<X, VW, E, TPR>((const X*)p.x + row * p.x_sr, p.width, lane, x);
+        load_row<B, VW, E, TPR>((const B*)p.block + row * p.block_sr, p.width, lane, b);
+        load_row<B, VW, E, TPR>(p.gate ? (const B*)p.gate + row * p.gate_sr : nullptr, p.width, lane, g);
+        load_row<X, VW, E, TPR>(p.grad_y ? (const X*)p.grad_y + row * p.grad_y_sr : nullptr, p.width, lane, dy);
+        load_row<B, VW, E, TPR>(p.grad_z ? (const B*)p.grad_z + row * p.grad_z_sr : nullptr, p.width, lane, dz);
+        sums[0] = 0.f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) sums[0] += b[i] * b[i];
+        row_sums<TPR>(sums, 1, shared);
+        const float rb = 1.f / sqrtf(sums[0] / p.width + p.eps);
+        load_row<float, VW, E, TPR>(p.post, p.width, lane, w);
+        float r[E];
+        load_row<float, VW, E, TPR>(p.res, p.width, lane, r);
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            b[i] *= rb;
+            g[i] = p.gate ? sigmoid(g[i]) : 1.f;
+            w[i] *= r[i];
+            x[i] += w[i] * (g[i] * b[i]);
+        }
+        load_row<float, VW, E, TPR>(p.pre, p.width, lane, r);
+        sums[0] = sums[1] = 0.f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            sums[0] += x[i] * x[i];
+            sums[1] += x[i] * (dz[i] * r[i]);
+        }
+        row_sums<TPR>(sums, 2, shared);
+        const float ry = 1.f / sqrtf(sums[0] / p.width + p.eps), mean = sums[1] * ry / p.width;
+        sums[0] = 0.f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const float yn = x[i] * ry;
+            sum_p[i] += dz[i] * yn;
+            dy[i] += ry * (dz[i] * r[i] - yn * mean);
+            sum_m[i] += dy[i] * (g[i] * b[i]);
+            r[i] = dy[i] * w[i];  // f res post
+            sums[0] += r[i] * g[i] * b[i];
+        }
+        store_row<X, VW, E, TPR>((X*)p.grad_x + row * p.width, p.width, lane, dy);
+        row_sums<TPR>(sums, 1, shared);
+        const float back = sums[0] / p.width;
+        if (p.gate) {
+#pragma unroll
+            for (int i = 0; i < E; ++i) x[i] = r[i] * b[i] * (g[i] * (1.f - g[i]));
+            store_row<B, VW, E, TPR>((B*)p.grad_gate + row * p.width, p.width, lane, x);
+        }
+#pragma unroll
+        for (int i = 0; i < E; ++i) x[i] = rb * (r[i] * g[i] - b[i] * back);
+        store_row<B, VW, E, TPR>((B*)p.grad_block + row * p.width, p.width, lane, x);
+    }
+    float* to = p.partial + (int64_t)blockIdx.x * p.width;
+    const int64_t second = (int64_t)gridDim.x * p.width;
+    if (TPR > 64) {
+        store_row<float, VW, E, TPR>(to, p.width, lane, sum_m);
+        store_row<float, VW, E, TPR>(to + second, p.width, lane, sum_p);
+    } else {
+        const int wave = threadIdx.x / 64;
+        for (int which = 0; which < 2; ++which) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < E; ++i) fold[(wave * E + i) * 64 + lane] = which ? sum_p[i] : sum_m[i];
+            __syncthreads();
+            for (int e = threadIdx.x; e < E * 64; e += 256) {
+                const int i = e / 64, col = ((i / VW) * 64 + e % 64) * VW + i % VW;
+                if (col < p.width) to[which * second + col] = fold[e] + fold[E * 64 + e] + fold[2 * E * 64 + e] + fold[3 * E * 64 + e];
+            }
+        }
+    }
+}
+
+// grid (columns / 32, 2): 32 columns, 32 threads to each; blockIdx.y 0: post and res, 1: pre
+__global__ __launch_bounds__(1024) void column_sums(const float* partial, int parts, int width, const float* post, const float* res, float* grad_post, float* grad_res, float* grad_pre) {
+    __shared__ float fold[32][33];
+    const int c = threadIdx.x % 32, r = threadIdx.x / 32, col = blockIdx.x * 32 + c;
+    const float* from = partial + (int64_t)blockIdx.y * parts * width;
+    float sum = 0.f;
+    if (col < width)
+        for (int i = r; i < parts; i += 32) sum += from[(int64_t)i * width + col];
+    fold[r][c] = sum;
+    __syncthreads();
+    if (r == 0 && col < width) {
+        sum = 0.f;
+        for (int i = 0; i < 32; ++i) sum += fold[i][c];
+        if (blockIdx.y)
+            grad_pre[col] = sum;
+        else {
+            grad_post[col] = res[col] * sum;
+            grad_res[col] = post[col] * sum;
+        }
+    }
+}
+
+constexpr int64_t BLOCK_PARTS = 512;
+
+int block_rows(int64_t width) { return width <= 1024 ? 4 : 1; }  // rows a workgroup holds at once
+int64_t block_parts(const lobpolicy_block* b) {
+    const int64_t groups = ceil_div(b->rows, block_rows(b->width));
+    return groups < BLOCK_PARTS ? groups : BLOCK_PARTS;
+}
+
+template <class X, class B, int VW, int E, int TPR>
+int block_launch(const Block& p, bool backward, int64_t parts, hipStream_t stream) {
+    const int64_t groups = ceil_div(p.rows, 256 / TPR);
+    if (backward)
+        block_backward_kernel<X, B, VW, E, TPR><<<dim3((unsigned)parts), 256, 0, stream>>>(p);
+    else
+        block_forward_kernel<X, B, VW, E, TPR><<<dim3((unsigned)(groups < (1 << 20) ? groups : (1 << 20))), 256, 0, stream>>>(p);
+    return launched();
+}
+
+template <class X, class B, int VW>
+int block_wide(const Block& p, bool backward, int64_t parts, hipStream_t stream) {
+    constexpr int LEAST = VW < 4 ? 4 : VW;
+    if (p.width <= 64 * LEAST) return block_launch<X, B, VW, LEAST, 64>(p, backward, parts, stream);
+    if (p.width <= 1024) return block_launch<X, B, VW, 16, 64>(p, backward, parts, stream);
+    if (p.width <= 2048) return block_launch<X, B, VW, 8, 256>(p, backward, parts, stream);
+    return block_launch<X, B, VW, 32, 256>(p, backward, parts, stream);
+}
+
+bool aligned(const void* p, int64_t bytes) { return (uintptr_t)p % bytes == 0; }
+
+template <class X, class B>
+int block_typed(const Block& p, bool backward, int64_t parts, hipStream_t stream) {
+    auto fits = [&](int w) {
+        const int64_t xs = w * sizeof(X) < 16 ? w * sizeof(X) : 16, bs = w * sizeof(B) < 16 ? w * sizeof(B) : 16, fs = w * 4 < 16 ? w * 4 : 16;
+        bool ok = p.width % w == 0 && p.x_sr % w == 0 && p.block_sr % w == 0 && p.gate_sr % w == 0 && p.grad_y_sr % w == 0 && p.grad_z_sr % w == 0;
+        ok = ok && aligned(p.x, xs) && aligned(p.y, xs) && aligned(p.grad_y, xs) && aligned(p.grad_x, xs);
+        ok = ok && aligned(p.block, bs) && aligned(p.gate, bs) && aligned(p.z, bs) && aligned(p.grad_z, bs) && aligned(p.grad_block, bs) && aligned(p.grad_gate, bs);
+        return ok && aligned(p.post, fs) && aligned(p.res, fs) && aligned(p.pre, fs) && aligned(p.partial, fs);
+    };
+    if (p.width > 256 && fits(8)) return block_wide<X, B, 8>(p, backward, parts, stream);
+    if (fits(4)) return block_wide<X, B, 4>(p, backward, parts, stream);
+    return block_wide<X, B, 1>(p, backward, parts, stream);
+}
+
+int block_any(const lobpolicy_block* b, const Block& p, bool backward, int64_t parts, void* stream) {
+    hipStream_t s = (hipStream_t)stream;
+    if (b->stream_dtype == LOBPOLICY_F32) return b->dtype == LOBPOLICY_F32 ? block_typed<float, float>(p, backward, parts, s) : block_typed<float, bf16>(p, backward, parts, s);
+    return b->dtype == LOBPOLICY_F32 ? block_typed<bf16, float>(p, backward, parts, s) : block_typed<bf16, bf16>(p, backward, parts, s);
+}
+
+int check_block(const lobpolicy_block* b) {
+    REQUIRE(b, "no description");
+    for (int d : {b->stream_dtype, b->dtype}) REQUIRE(d == LOBPOLICY_F32 || d == LOBPOLICY_BF16, "dtype %d", d);
+    REQUIRE(b->rows >= 1 && b->rows <= (1ll << 40), "rows = %lld: 1 to 2^40", (long long)b->rows);
+    REQUIRE(b->width >= 1 && b->width <= LOBPOLICY_MAX_WIDTH, "width = %lld: 1 to %d", (long long)b->width, LOBPOLICY_MAX_WIDTH);
+    REQUIRE(b->x && b->block && b->post && b->res && b->pre, "an operand is missing");
+    return LOBPOLICY_OK;
+}
+
+Block block_of(const lobpolicy_block* b) {
+    Block p = {};
+    p.x = b->x, p.block = b->block, p.gate = b->gate;
+    p.x_sr = b->x_stride, p.block_sr = b->block_stride, p.gate_sr = b->gate ? b->gate_stride : 0;
+    p.post = b->post, p.res = b->res, p.pre = b->pre;
+    p.rows = b->rows, p.width = (int)b->width, p.eps = b->eps;
+    return p;
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------
+// the global norm, and clipping
+//
+// Two passes, each bound by memory: the squares are summed in 64 bits (which neither overflows nor loses what many small gradients add),
+// one number per workgroup, in a fixed order; the second pass begins by adding those numbers up, in every workgroup alike, and scales.
+// The tensors' table travels as a kernel argument: nothing is copied to the device, and a captured graph holds it.
+
+constexpr int CLIP_TENSORS = 128;        // per launch: 3 KB of arguments
+constexpr int64_t CLIP_CHUNK = 8192;     // elements
+constexpr int64_t CLIP_PARTS = 1024;     // workgroups per launch, at most
+
+struct ClipTable {
+    void* data[CLIP_TENSORS];
+    int64_t count[CLIP_TENSORS];
+    uint32_t first[CLIP_TENSORS + 1];  // chunk at which each begins
+    uint8_t dtype[CLIP_TENSORS];
+    int n;
+};
+
+__device__ __forceinline__ int find_tensor(const ClipTable& t, uint32_t chunk) {
+    int lo = 0, hi = t.n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (t.first[mid] <= chunk)
+            lo = mid;
+        else
+            hi = mid - 1;
+    }
+    return lo;
+}
+
+template <bool MAX>
+__device__ __forceinline__ double join(double a, double b) {
+    if (!MAX) return a + b;
+    return a != a || a > b ? a : b;  // (not a number stays: b is taken where a > b is false, and b != b where a is one)
+}
+
+template <bool MAX>
+__device__ __forceinline__ double joined(double x, double* shared) {  // over the workgroup, in a fixed order
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) x = join<MAX>(x, __shfl_xor(x, d));
+    __syncthreads();
+    if (threadIdx.x % 64 == 0) shared[threadIdx.x / 64] = x;
+    __syncthreads();
+    return join<MAX>(join<MAX>(shared[0], shared[1]), join<MAX>(shared[2], shared[3]));
+}
+
+// f(pointer to W elements, W) over the chunk's elements: single ones up to the first 16-byte boundary of the tensor and behind the last
+template <class T, class One, class Many>
+__device__ __forceinline__ void over_chunk(T* data, int64_t count, uint32_t chunk, One one, Many many) {
+    constexpr int W = 16 / sizeof(T);
+    int64_t head = (16 - (int64_t)((uintptr_t)data % 16)) % 16 / (int64_t)sizeof(T);
+    head = head < count ? head : count;
+    const int64_t begin = head + (int64_t)chunk * CLIP_CHUNK;
+    int64_t end = begin + CLIP_CHUNK;
+    end = end < count ? end : count;
+    if (chunk == 0 && threadIdx.x < head) one(data + threadIdx.x);
+    const int64_t whole = begin + (end - begin) / W * W;
+#pragma unroll 4
+    for (int64_t i = begin + threadIdx.x * W; i < whole; i += 256 * W) many(data + i);
+    if (whole + threadIdx.x < end) one(data + whole + threadIdx.x);
+}
+
+template <bool MAX>
+__global__ __launch_bounds__(256) void norm_kernel(ClipTable t, double* partial) {
+    __shared__ double shared[4];
+    double sum = 0.0;
+    auto take = [&](float x) { sum = MAX ? join<true>(sum, (double)fabsf(x)) : fma((double)x, (double)x, sum); };
+    for (uint32_t chunk = blockIdx.x; chunk < t.first[t.n]; chunk += gridDim.x) {
+        const int i = find_tensor(t, chunk);
+        auto go = [&](auto* data) {
+            using T = std::remove_pointer_t<decltype(data)>;
+            over_chunk(data, t.count[i], chunk - t.first[i], [&](T* p) { take((float)*p); },
+                       [&](T* p) {
+                           float x[16 / sizeof(T)];
+                           load_pack<T, 16 / sizeof(T)>(p, x);
+#pragma unroll
+                           for (int e = 0; e < 16 / (int)sizeof(T); ++e) take(x[e]);
+                       });
+        };
+        if (t.dtype[i] == LOBPOLICY_BF16)
+            go((bf16*)t.data[i]);
+        else
+            go((float*)t.data[i]);
+    }
+    sum = joined<MAX>(sum, shared);
+    if (threadIdx.x == 0) partial[blockIdx.x] = sum;
+}
+
+template <bool MAX>
+__global__ __launch_bounds__(256) void clip_kernel(ClipTable t, const double* partial, int parts, double max_norm, float* norm_out) {
+    __shared__ double shared[4];
+    double sum = 0.0;
+    for (int i = threadIdx.x; i < parts; i += 256) sum = join<MAX>(sum, partial[i]);
+    sum = joined<MAX>(sum, shared);
+    const double norm = MAX ? sum : sqrt(sum);
+    if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
+    const double ratio = max_norm / (norm + 1e-6);
+    const float by = ratio > 1.0 ? 1.f : (float)ratio;  // (not a number stays one)
+    if (by == 1.f) return;  // times one: the elements stay as they are
+    for (uint32_t chunk = blockIdx.x; chunk < t.first[t.n]; chunk += gridDim.x) {
+        const int i = find_tensor(t, chunk);
+        auto go = [&](auto* data) {
+            using T = std::remove_pointer_t<decltype(data)>;
+            over_chunk(data, t.count[i], chunk - t.first[i], [&](T* p) { *p = (T)((float)*p * by); },
+                       [&](T* p) {
+                           float x[16 / sizeof(T)];
+                           load_pack<T, 16 / sizeof(T)>(p, x);
+#pragma unroll
+                           for (int e = 0; e < 16 / (int)sizeof(T); ++e) x[e] *= by;
+                           store_pack<T, 16 / sizeof(T)>(p, x);
+                       });
+        };
+        if (t.dtype[i] == LOBPOLICY_BF16)
+            go((bf16*)t.data[i]);
+        else
+            go((float*)t.data[i]);
+    }
+}
+
+__global__ void zero_norm(float* norm) { *norm = 0.f; }
+
+struct ClipPlan {  // the next up to CLIP_TENSORS tensors that are not empty, from index i on
+    ClipTable table;
+    int64_t next;
+    int64_t parts;
+};
+
+ClipPlan clip_plan(void* const* tensors, const int64_t* counts, const int32_t* dtypes, int64_t n, int64_t i) {
+    ClipPlan p;
+    p.table.n = 0;
+    uint64_t chunks = 0;
+    for (; i < n && p.table.n < CLIP_TENSORS; ++i) {
+        if (counts[i] == 0) continue;
+        // (by the count alone: the elements in front of the first 16-byte boundary can only make it fewer chunks, and an empty chunk does nothing)
+        const uint64_t more = (uint64_t)ceil_div(counts[i], CLIP_CHUNK);
+        if (chunks + more > 0x7fffffffull && p.table.n) break;
+        const int k = p.table.n++;
+        p.table.data[k] = tensors ? tensors[i] : nullptr;
+        p.table.count[k] = counts[i];
+        p.table.dtype[k] = (uint8_t)dtypes[i];
+        p.table.first[k] = (uint32_t)chunks;
+        chunks += more;
+        p.table.first[k + 1] = (uint32_t)chunks;
+    }
+    p.next = i;
+    p.parts = (int64_t)(chunks < (uint64_t)CLIP_PARTS ? chunks : (uint64_t)CLIP_PARTS);
+    return p;
+}
+
+int check_clip(const int64_t* counts, const int32_t* dtypes, int64_t n) {
+    REQUIRE(n >= 0 && n <= 1000000, "n = %lld tensors", (long long)n);
+    REQUIRE(n == 0 || (counts && dtypes), "no counts or dtypes");
+    for (int64_t i = 0; i < n; ++i) {
+        REQUIRE(counts[i] >= 0 && counts[i] <= (1ll << 43), "tensor %lld has %lld elements", (long long)i, (long long)counts[i]);
+        REQUIRE(dtypes[i] == LOBPOLICY_F32 || dtypes[i] == LOBPOLICY_BF16, "tensor %lld: dtype %d", (long long)i, dtypes[i]);
+    }
+    return LOBPOLICY_OK;
+}
+
+int64_t clip_parts(const int64_t* counts, const int32_t* dtypes, int64_t n) {
+    int64_t parts = 0;
+    for (int64_t i = 0; i < n;) {
+        const ClipPlan p = clip_plan(nullptr, counts, dtypes, n, i);
+        parts += p.parts;
+        i = p.next;
+    }
+    return parts;
+}
+
+}  // namespace
+
+// ---------------------------------------------------------------------------------------------------------------------------
+// the C-ABI
+
+extern "C" {
+
+int lobpolicy_abi_version(void) { return LOBPOLICY_ABI_VERSION; }
+const char* lobpolicy_last_error(void) { return g_error; }
+
+int64_t lobpolicy_attention_workspace(const lobpolicy_attention* a, int32_t backward) {
+    (void)backward;
+    if (int e = check_attention(a)) return e;
+    return 0;
+}
+
+int lobpolicy_attention_forward(const lobpolicy_attention* a, void* stream) {
+    if (int e = check_attention(a)) return e;
+    REQUIRE(a->q.data && a->k.data && a->v.data && a->out.data, "an operand is missing");
+    Scan s = scan_of(a);
+    s.a = rows_of(a->q), s.b = rows_of(a->k), s.c = rows_of(a->v), s.out = rows_of(a->out);
+    s.da = a->dk, s.dc = a->dv;
+    s.out_scale = a->scale;
+    s.state_in = a->state_in, s.in_row = a->dv, s.in_col = 1;
+    s.state_out = a->state_out, s.out_row = a->dv, s.out_col = 1;
+    return scan(a, s, false, stream);
+}
+
+int lobpolicy_attention_backward(const lobpolicy_attention* a, void* stream) {
+    if (int e = check_attention(a)) return e;
+    REQUIRE(a->q.data && a->k.data && a->v.data && a->out.data, "an operand is missing");
+    REQUIRE(a->grad_q.data && a->grad_k.data && a->grad_v.data, "a gradient is missing");
+    Scan s = scan_of(a);
+    s.a = rows_of(a->out), s.b = rows_of(a->v), s.c = rows_of(a->k), s.out = rows_of(a->grad_q);
+    s.da = a->dv, s.dc = a->dk;
+    s.out_scale = a->scale;
+    s.state_in = a->state_in, s.in_row = 1, s.in_col = a->dv;
+    if (int e = scan(a, s, false, stream)) return e;
+    s.a = rows_of(a->v), s.b = rows_of(a->out), s.c = rows_of(a->q), s.out = rows_of(a->grad_k);
+    s.out_scale = 1.f, s.in_scale = a->scale;
+    s.state_in = a->grad_state_out;
+    if (int e = scan(a, s, true, stream)) return e;
+    s.a = rows_of(a->k), s.b = rows_of(a->q), s.c = rows_of(a->out), s.out = rows_of(a->grad_v);
+    s.da = a->dk, s.dc = a->dv;
+    s.in_row = s.out_row = a->dv, s.in_col = s.out_col = 1;
+    s.state_out = a->grad_state_in;
+    return scan(a, s, true, stream);
+}
+
+int lobpolicy_attention_step(const lobpolicy_attention* a, void* stream) {
+    if (int e = check_attention(a)) return e;
+    REQUIRE(a->steps == 1, "a step takes one token of every environment: steps = %lld", (long long)a->steps);
+    REQUIRE(a->q.data && a->k.data && a->v.data && a->out.data && a->state_out, "an operand is missing");
+    Step s = {};
+    s.q = a->q.data, s.k = a->k.data, s.v = a->v.data, s.out = a->out.data;
+    s.q_sn = a->q.stride_n, s.q_sh = a->q.stride_h, s.k_sn = a->k.stride_n, s.k_sh = a->k.stride_h;
+    s.v_sn = a->v.stride_n, s.v_sh = a->v.stride_h, s.out_sn = a->out.stride_n, s.out_sh = a->out.stride_h;
+    s.log_decay = a->log_decay, s.reset = a->reset, s.reset_sn = a->reset_stride_n, s.skip = a->skip;
+    s.state = a->state_out, s.heads = a->heads, s.dk = a->dk, s.dv = a->dv, s.scale = a->scale;
+    const int64_t units = a->envs * a->heads;
+    return a->dtype == LOBPOLICY_BF16 ? step_typed<bf16>(s, units, (hipStream_t)stream) : step_typed<float>(s, units, (hipStream_t)stream);
+}
+
+int64_t lobpolicy_block_workspace(const lobpolicy_block* b) {
+    if (int e = check_block(b)) return e;
+    return 2 * block_parts(b) * b->width * (int64_t)sizeof(float);
+}
+
+int lobpolicy_block_forward(const lobpolicy_block* b, void* stream) {
+    if (int e = check_block(b)) return e;
+    REQUIRE(b->y && b->z, "a result is missing");
+    Block p = block_of(b);
+    p.y = b->y, p.z = b->z;
+    return block_any(b, p, false, 0, stream);
+}
+
+int lobpolicy_block_backward(const lobpolicy_block* b, void* stream) {
+    if (int e = check_block(b)) return e;
+    REQUIRE(b->grad_x && b->grad_block && (b->grad_gate || !b->gate) && b->grad_post && b->grad_res && b->grad_pre, "a gradient is missing");
+    REQUIRE(b->workspace && b->workspace_bytes >= lobpolicy_block_workspace(b), "the workspace has %lld bytes", (long long)b->workspace_bytes);
+    Block p = block_of(b);
+    p.grad_y = b->grad_y, p.grad_z = b->grad_z, p.grad_y_sr = b->grad_y ? b->grad_y_stride : 0, p.grad_z_sr = b->grad_z ? b->grad_z_stride : 0;
+    p.grad_x = b->grad_x, p.grad_block = b->grad_block, p.grad_gate = b->grad_gate;
+    p.partial = (float*)b->workspace;
+    const int64_t parts = block_parts(b);
+    if (int e = block_any(b, p, true, parts, stream)) return e;
+    column_sums<<<dim3((unsigned)ceil_div(b->width, 32), 2), 1024, 0, (hipStream_t)stream>>>(p.partial, (int)parts, p.width, b->post, b->res, b->grad_post, b->grad_res, b->grad_pre);
+    return launched();
+}
+
+int64_t lobpolicy_clip_workspace(const int64_t* counts, const int32_t* dtypes, int64_t n) {
+    if (int e = check_clip(counts, dtypes, n)) return e;
+    return clip_parts(counts, dtypes, n) * (int64_t)sizeof(double);
+}
+
+int lobpolicy_clip(void* const* tensors, const int64_t* counts, const int32_t* dtypes, int64_t n, int32_t kind, double max_norm, float* norm, void* workspace,
+                   int64_t workspace_bytes, void* stream) {
+    if (int e = check_clip(counts, dtypes, n)) return e;
+    REQUIRE(kind == 0 || kind == 2, "kind = %d: 0 (largest) or 2 (squares)", kind);
+    REQUIRE(max_norm >= 0.0, "max_norm = %g", max_norm);
+    REQUIRE(norm && (n == 0 || tensors), "an operand is missing");
+    for (int64_t i = 0; i < n; ++i)
+        REQUIRE(counts[i] == 0 || (tensors[i] && aligned(tensors[i], dtypes[i] == LOBPOLICY_BF16 ? 2 : 4)), "tensor %lld: no data, or not aligned to its type", (long long)i);
+    hipStream_t s = (hipStream_t)stream;
+    const int64_t parts = clip_parts(counts, dtypes, n);
+    if (parts == 0) {
+        zero_norm<<<1, 1, 0, s>>>(norm);
+        return launched();
+    }
+    REQUIRE(parts <= 0x7fffffff && workspace && aligned(workspace, 8) && workspace_bytes >= parts * (int64_t)sizeof(double), "the workspace has %lld bytes", (long long)workspace_bytes);
+    double* partial = (double*)workspace;
+    int64_t at = 0;
+    for (int64_t i = 0; i < n;) {
+        const ClipPlan p = clip_plan(tensors, counts, dtypes, n, i);
+        if (p.parts) {
+            if (kind == 0)
+                norm_kernel<true><<<dim3((unsigned)p.parts), 256, 0, s>>>(p.table, partial + at);
+            else
+                norm_kernel<false><<<dim3((unsigned)p.parts), 256, 0, s>>>(p.table, partial + at);
+            if (int e = launched()) return e;
+        }
+        at += p.parts;
+        i = p.next;
+    }
+    float* first = norm;  // the first launch writes it
+    for (int64_t i = 0; i < n;) {
+        const ClipPlan p = clip_plan(tensors, counts, dtypes, n, i);
+        if (p.parts) {
+            if (kind == 0)
+                clip_kernel<true><<<dim3((unsigned)p.parts), 256, 0, s>>>(p.table, partial, (int)parts, max_norm, first);
+            else
+                clip_kernel<false><<<dim3((unsigned)p.parts), 256, 0, s>>>(p.table, partial, (int)parts, max_norm, first);
+            if (int e = launched()) return e;
+            first = nullptr;
+        }
+        i = p.next;
+    }
+    return LOBPOLICY_OK;
+}
+
+}  // extern "C"

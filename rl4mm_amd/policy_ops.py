@@ -1,0 +1,360 @@
+"""Operators for a policy that remembers order flow, as hand-written HIP kernels (include/lobpolicy.h): torch tensors in and out, launched
+asynchronously on torch's current stream of the tensors' device, like the tensor path of rl4mm_amd/env.py they run next to.
+
+  decay_attention_step   one observation of every environment: the state of each, [heads][dk][dv], is updated in place
+  decay_attention        the same over recorded segments [T, N], differentiable
+  gated_residual_norm    a block's end: norm, gate, residual scale, and the norm before the next block; differentiable
+  clip_grad_norm         the global gradient norm, and clipping by it
+
+float32 and bfloat16; states, norms and sums are float32 or wider.  There is no CPU path: CPU tensors raise, as does a missing
+library.  Every call can be captured into a graph (nothing waits for the device, nothing is allocated but results and workspaces, through
+torch's allocator).  A call that cannot be right raises ValueError or TypeError before anything is launched."""
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+import torch
+
+from . import _lib
+from . import _policy_capi as capi
+
+_DTYPES = {torch.float32: capi.F32, torch.bfloat16: capi.BF16}
+_NONE = capi.Operand(None, 0, 0, 0)
+
+
+class _on:
+    """The raw current stream of `device`, with that device current inside the block."""
+
+    __slots__ = ("index", "before")
+
+    def __init__(self, device):
+        self.index = device.index
+
+    def __enter__(self):
+        self.before = torch.cuda.current_device()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+        return torch.cuda.current_stream(self.index).cuda_stream
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            torch.cuda.set_device(self.before)
+
+
+def _need(ok, message, kind=ValueError):
+    if not ok:
+        raise kind(message)
+
+
+def _tensor(t, name, dtypes, device=None, shape=None):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} is a torch tensor, got {type(t).__name__}")
+    if not t.is_cuda or t.layout != torch.strided:
+        raise ValueError(f"{name} is a strided tensor on the GPU (there is no CPU path): got {t.layout} on {t.device}")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name} is {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the other operands on {device}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} has the shape {tuple(shape)}, got {tuple(t.shape)}")
+
+
+def _lined(t):
+    """`t`, its last dimension contiguous."""
+    return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def _operand(t):  # [T, N, H, D] or [N, H, D]
+    return capi.Operand(t.data_ptr(), *t.stride()[:3]) if t.dim() == 4 else capi.Operand(t.data_ptr(), 0, *t.stride()[:2])
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _changed(tensors):
+    """Tells autograd that these were written in place (tensors made in inference mode keep no count of it)."""
+    for t in tensors:
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
+def _flags(t, name, shape, device):
+    if t is None:
+        return None
+    _tensor(t, name, (torch.bool, torch.uint8), device, shape)
+    return t
+
+
+def _heads(q, k, v, log_decay, state, scale, dims):
+    """Checks what the two forms have in common -> (log_decay, scale)."""
+    _tensor(q, "q", _DTYPES)
+    _need(q.dim() == len(dims), f"q is [{', '.join(dims)}], got {tuple(q.shape)}")
+    _tensor(k, "k", (q.dtype,), q.device, q.shape)
+    _tensor(v, "v", (q.dtype,), q.device)
+    _need(v.shape[:-1] == q.shape[:-1], f"v is [{', '.join(dims[:-1])}, dv] beside q {tuple(q.shape)}, got {tuple(v.shape)}")
+    heads, dk, dv = q.shape[-2], q.shape[-1], v.shape[-1]
+    _need(heads >= 1 and 1 <= dk <= capi.MAX_HEAD and 1 <= dv <= capi.MAX_HEAD, f"{heads} heads of dk = {dk} and dv = {dv}: one head or more, dk and dv 1 to {capi.MAX_HEAD}")
+    _tensor(log_decay, "log_decay", (torch.float32,), q.device, (heads,))
+    _need(not log_decay.requires_grad, "log_decay takes no gradient: the decays are constants of the policy")
+    if state is not None:
+        _tensor(state, "the state", (torch.float32,), q.device, (q.shape[-3], heads, dk, dv))
+    scale = dk**-0.5 if scale is None else float(scale)
+    _need(math.isfinite(scale), f"scale = {scale}")
+    return log_decay.contiguous(), scale
+
+
+def _describe(q, k, v, log_decay, reset, lengths, scale):
+    a = capi.Attention()
+    a.dtype, a.heads, a.dk, a.dv, a.envs, a.steps = _DTYPES[q.dtype], q.shape[-2], q.shape[-1], v.shape[-1], q.shape[-3], q.shape[0] if q.dim() == 4 else 1
+    a.q, a.k, a.v = _operand(q), _operand(k), _operand(v)
+    a.log_decay, a.scale = log_decay.data_ptr(), scale
+    if reset is not None:
+        a.reset = reset.data_ptr()
+        a.reset_stride_t, a.reset_stride_n = reset.stride() if reset.dim() == 2 else (0, reset.stride(0))
+    a.lengths = _ptr(lengths)
+    return a
+
+
+def _workspace(a, backward, lib, device):
+    """The description's workspace -> the tensor that holds it (to be kept until the launch is made)."""
+    need = lib.check(lib.fn["attention_workspace"](C.byref(a), backward), "attention_workspace")
+    held = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    a.workspace, a.workspace_bytes = _ptr(held), need
+    return held
+
+
+def _attention_forward(q, k, v, log_decay, state, reset, lengths, scale):
+    out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+    last = torch.empty((q.shape[1], q.shape[2], q.shape[3], v.shape[3]), dtype=torch.float32, device=q.device)
+    lib = _lib.policy_binding()
+    a = _describe(q, k, v, log_decay, reset, lengths, scale)
+    a.out, a.state_in, a.state_out = _operand(out), _ptr(state), last.data_ptr()
+    with _on(q.device) as stream:
+        held = _workspace(a, 0, lib, q.device)  # noqa: F841
+        lib.check(lib.fn["attention_forward"](C.byref(a), stream), "attention_forward")
+    return out, last
+
+
+class _DecayAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, state, reset, lengths, scale):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(q, k, v, log_decay, state, reset, lengths)
+        ctx.scale = scale
+        return _attention_forward(q, k, v, log_decay, state, reset, lengths, scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, dlast):
+        q, k, v, log_decay, state, reset, lengths = ctx.saved_tensors
+        if dout is None and dlast is None:
+            return (None,) * 8
+        dout = torch.zeros(v.shape, dtype=v.dtype, device=v.device) if dout is None else _lined(dout)
+        dlast = None if dlast is None else dlast.contiguous()
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        dstate = torch.empty(state.shape, dtype=torch.float32, device=q.device) if ctx.needs_input_grad[4] else None
+        lib = _lib.policy_binding()
+        a = _describe(q, k, v, log_decay, reset, lengths, ctx.scale)
+        a.out, a.state_in, a.grad_state_out = _operand(dout), _ptr(state), _ptr(dlast)
+        a.grad_q, a.grad_k, a.grad_v, a.grad_state_in = _operand(dq), _operand(dk), _operand(dv), _ptr(dstate)
+        with _on(q.device) as stream:
+            held = _workspace(a, 1, lib, q.device)  # noqa: F841
+            lib.check(lib.fn["attention_backward"](C.byref(a), stream), "attention_backward")
+        need = ctx.needs_input_grad
+        return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, dstate, None, None, None
+
+
+def decay_attention(q, k, v, log_decay, *, initial_state=None, reset=None, lengths=None, scale=None):
+    """Linear attention with a decay for each head over recorded segments -> (out [T, N, H, dv], state [N, H, dk, dv] after the last token).
+
+    Of every environment n and head h, with a state S [dk, dv] that begins as ``initial_state`` (zeros without one):
+
+        S = 0 where reset[t, n];   S = exp(log_decay[h]) S + k_t v_t^T;   out_t = scale q_t^T S
+
+    q, k [T, N, H, dk], v [T, N, H, dv], float32 or bfloat16, time-major like the framework's traces; any strides, so they may be views of one
+    projection's output.  log_decay [H] float32, a constant (no gradient).  reset [T, N] bool or uint8: token t is the first of a new episode, and
+    nothing before it reaches it - not even a value that is not a number.  lengths [N] int32: environment n has that many tokens (clamped to 0 .. T);
+    what lies behind them is not read, its rows of ``out`` and of the gradients are 0, and the state is the one after its last token.  scale: dk ** -0.5
+    by default.  Gradients reach q, k, v and initial_state."""
+    log_decay, scale = _heads(q, k, v, log_decay, initial_state, scale, ("T", "N", "H", "dk"))
+    reset = _flags(reset, "reset", q.shape[:2], q.device)
+    if lengths is not None:
+        _tensor(lengths, "lengths", (torch.int32,), q.device, (q.shape[1],))
+        lengths = lengths.contiguous()
+    if q.shape[0] == 0 or q.shape[1] == 0:
+        state = torch.zeros((*q.shape[1:], v.shape[3]), dtype=torch.float32, device=q.device)
+        return v.clone(), state if initial_state is None else initial_state.clone()
+    state = None if initial_state is None else initial_state.contiguous()
+    args = (_lined(q), _lined(k), _lined(v), log_decay, state, reset, lengths, scale)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (state is not None and state.requires_grad)):
+        return _DecayAttention.apply(*args)
+    return _attention_forward(*args)
+
+
+def decay_attention_step(q, k, v, log_decay, state, *, reset=None, skip=None, scale=None):
+    """One token of every environment -> out [N, H, dv]; ``state`` [N, H, dk, dv] float32, contiguous, is updated IN PLACE.
+
+    The step of ``decay_attention`` (q, k [N, H, dk], v [N, H, dv]): reset [N] - this observation begins an episode; skip [N] - the environment is
+    done and sits out (the ``done`` flags of ``vector_step_tensors``): its state stays as it is, its row of out is 0.  No gradient: raises when one
+    is asked for."""
+    log_decay, scale = _heads(q, k, v, log_decay, state, scale, ("N", "H", "dk"))
+    _need(state is not None, "state is the [N, H, dk, dv] tensor that the step updates", TypeError)
+    _need(state.is_contiguous(), "the state is updated in place: it has to be contiguous")
+    _need(not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad)),
+          "decay_attention_step has no gradient: call it under torch.no_grad(), or decay_attention for the gradients")  # fmt: skip
+    reset, skip = _flags(reset, "reset", q.shape[:1], q.device), _flags(skip, "skip", q.shape[:1], q.device)
+    out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+    if q.shape[0] == 0:
+        return out
+    q, k, v = _lined(q), _lined(k), _lined(v)
+    skip = None if skip is None else skip.contiguous()
+    lib = _lib.policy_binding()
+    a = _describe(q, k, v, log_decay, reset, None, scale)
+    a.out, a.state_out, a.skip = _operand(out), state.data_ptr(), _ptr(skip)
+    with _on(q.device) as stream:
+        lib.check(lib.fn["attention_step"](C.byref(a), stream), "attention_step")
+    _changed([state])
+    return out
+
+
+# ---- the block's end ----------------------------------------------------------------------------------------------------------
+
+
+def _rows(t, width):
+    """[..., width] -> [rows, width] with contiguous rows; a copy only where the strides leave no other way."""
+    t = _lined(t)
+    return t if t.dim() == 2 else t.reshape(-1, width)
+
+
+def _describe_block(x, block, gate, post, res, pre, eps):
+    b = capi.Block()
+    b.stream_dtype, b.dtype, b.rows, b.width = _DTYPES[x.dtype], _DTYPES[block.dtype], *x.shape
+    b.x, b.block, b.gate, b.x_stride, b.block_stride = x.data_ptr(), block.data_ptr(), _ptr(gate), x.stride(0), block.stride(0)
+    b.gate_stride = 0 if gate is None else gate.stride(0)
+    b.post, b.res, b.pre, b.eps = post.data_ptr(), res.data_ptr(), pre.data_ptr(), eps
+    return b
+
+
+def _block_forward(x, block, gate, post, res, pre, eps):
+    y, z = torch.empty(x.shape, dtype=x.dtype, device=x.device), torch.empty(x.shape, dtype=block.dtype, device=x.device)
+    lib = _lib.policy_binding()
+    b = _describe_block(x, block, gate, post, res, pre, eps)
+    b.y, b.z = y.data_ptr(), z.data_ptr()
+    with _on(x.device) as stream:
+        lib.check(lib.fn["block_forward"](C.byref(b), stream), "block_forward")
+    return y, z
+
+
+class _GatedResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, block, gate, post, res, pre, eps):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x, block, gate, post, res, pre)
+        ctx.eps = eps
+        return _block_forward(x, block, gate, post, res, pre, eps)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dz):
+        x, block, gate, post, res, pre = ctx.saved_tensors
+        if dy is None and dz is None:
+            return (None,) * 7
+        dy, dz = (None if d is None else _lined(d) for d in (dy, dz))
+        dx, dblock = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (x, block))
+        dgate = None if gate is None else torch.empty_like(dblock)
+        dpost, dres, dpre = torch.empty((3, x.shape[1]), dtype=torch.float32, device=x.device)
+        lib = _lib.policy_binding()
+        b = _describe_block(x, block, gate, post, res, pre, ctx.eps)
+        b.grad_y, b.grad_z = _ptr(dy), _ptr(dz)
+        b.grad_y_stride, b.grad_z_stride = 0 if dy is None else dy.stride(0), 0 if dz is None else dz.stride(0)
+        b.grad_x, b.grad_block, b.grad_gate = dx.data_ptr(), dblock.data_ptr(), _ptr(dgate)
+        b.grad_post, b.grad_res, b.grad_pre = dpost.data_ptr(), dres.data_ptr(), dpre.data_ptr()
+        with _on(x.device) as stream:
+            need = lib.check(lib.fn["block_workspace"](C.byref(b)), "block_workspace")
+            held = torch.empty(need, dtype=torch.uint8, device=x.device)
+            b.workspace, b.workspace_bytes = held.data_ptr(), need
+            lib.check(lib.fn["block_backward"](C.byref(b), stream), "block_backward")
+        return tuple(g if wanted else None for g, wanted in zip((dx, dblock, dgate, dpost, dres, dpre), ctx.needs_input_grad)) + (None,)
+
+
+def gated_residual_norm(x, block, gate, post_weight, residual_scale, pre_weight, eps=1e-6):
+    """A block's end and the next one's beginning -> (y, z), both shaped like x [..., width]:
+
+        y = x + residual_scale * sigmoid(gate) * post_weight * block / rms(block);   z = pre_weight * y / rms(y);   rms(a) = sqrt(mean(a ** 2) + eps)
+
+    x: the residual stream, float32 or bfloat16, y its type.  block: what the block put out; gate: its gate's logits (None: no gate); z has their type,
+    float32 or bfloat16, and is taken from y before that is rounded.  The three weights: float32 [width].  width: 1 to 8192; rows of any stride.
+    Differentiable in all six; the weights' gradients are summed in a fixed order."""
+    _tensor(x, "x", _DTYPES)
+    _need(x.dim() >= 1, "x is [..., width], got a single number")
+    width = x.shape[-1]
+    _need(1 <= width <= capi.MAX_WIDTH, f"width = {width}: 1 to {capi.MAX_WIDTH}")
+    _tensor(block, "block", _DTYPES, x.device, x.shape)
+    if gate is not None:
+        _tensor(gate, "gate", (block.dtype,), x.device, x.shape)
+    weights = (post_weight, residual_scale, pre_weight)
+    for t, name in zip(weights, ("post_weight", "residual_scale", "pre_weight")):
+        _tensor(t, name, (torch.float32,), x.device, (width,))
+    eps = float(eps)
+    _need(math.isfinite(eps) and eps > 0.0, f"eps = {eps}")
+    shape, wanted = x.shape, torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, block, gate, *weights))
+    rows = [_rows(t, width) if t is not None else None for t in (x, block, gate)]
+    if x.numel() == 0:  # (nothing to compute, and the gradients are zeros: torch's own operations say so)
+        y = rows[0] + 0.0 * sum(w.sum() for w in weights)
+        z = rows[1] + 0.0 * (rows[2] if gate is not None else rows[1])
+        return y.to(x.dtype).reshape(shape), z.to(block.dtype).reshape(shape)
+    args = (*rows, *(t.contiguous() for t in weights), eps)
+    y, z = _GatedResidualNorm.apply(*args) if wanted else _block_forward(*args)
+    return (y, z) if len(shape) == 2 else (y.view(shape), z.view(shape))
+
+
+# ---- the global gradient norm -------------------------------------------------------------------------------------------------
+
+
+def _dense(t):
+    """Whether t's elements fill its span of memory once each, in whatever order."""
+    if t.is_contiguous():
+        return True
+    expect = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
+        if stride != expect:
+            return False
+        expect *= size
+    return True
+
+
+def clip_grad_norm(grads, max_norm, norm_type=2.0):
+    """Scales ``grads`` IN PLACE by min(1, max_norm / (norm + 1e-6)) -> norm, one float32 on their device (nothing waits for it).
+
+    grads: a tensor, or an iterable of tensors (None among them is passed over: a parameter without a gradient); float32 and bfloat16, mixed as you like, on
+    one GPU, each dense in some order of its dimensions, no two of them overlapping.  norm_type 2.0: the root of the sum of all squares, summed in 64 bits
+    in a fixed order; float("inf"): the largest magnitude.  A gradient that is not a number makes the norm one, and with it every gradient; an infinite
+    norm makes the finite ones 0.  No gradients: the norm is a CPU zero, as there is no device to put it on."""
+    grads = [grads] if isinstance(grads, torch.Tensor) else [g for g in grads if g is not None]
+    max_norm, norm_type = float(max_norm), float(norm_type)
+    _need(max_norm >= 0.0, f"max_norm = {max_norm}: 0 or more")
+    _need(norm_type in (2.0, math.inf), f"norm_type = {norm_type}: 2 or inf")
+    if not grads:
+        return torch.zeros(())
+    device, spans = getattr(grads[0], "device", None), []
+    for i, g in enumerate(grads):
+        _tensor(g, f"gradient {i}", _DTYPES, device)
+        _need(not g.requires_grad, f"gradient {i} requires a gradient itself: it is scaled outside autograd (detach it)")
+        _need(_dense(g), f"gradient {i} is not dense in memory (shape {tuple(g.shape)}, strides {g.stride()}): it could not be scaled in place")
+        if g.numel():
+            spans.append((g.data_ptr(), g.numel() * g.element_size(), i))
+    spans.sort()
+    for (p, size, i), (q, _, j) in zip(spans, spans[1:]):
+        _need(p + size <= q, f"gradients {min(i, j)} and {max(i, j)} share memory: each element is counted and scaled once")
+    n = len(grads)
+    tensors = (C.c_void_p * n)(*[g.data_ptr() for g in grads])
+    counts, dtypes = (C.c_int64 * n)(*[g.numel() for g in grads]), (C.c_int32 * n)(*[_DTYPES[g.dtype] for g in grads])
+    lib = _lib.policy_binding()
+    with _on(device) as stream:
+        need = lib.check(lib.fn["clip_workspace"](counts, dtypes, n), "clip_workspace")
+        norm, held = torch.empty((), dtype=torch.float32, device=device), torch.empty(max(need, 8), dtype=torch.uint8, device=device)
+        lib.check(lib.fn["clip"](tensors, counts, dtypes, n, 2 if norm_type == 2.0 else 0, max_norm, norm.data_ptr(), held.data_ptr(), need, stream), "clip")
+    _changed(grads)
+    return norm

@@ -16,6 +16,9 @@
 #ifdef __cplusplus
 extern "C" {
 #endif
+#if defined(__GNUC__)
+#pragma GCC visibility push(default)
+#endif
 
 #define LOBPOLICY_ABI_VERSION 1
 #define LOBPOLICY_MAX_HEAD 128   /* largest dk, dv */
@@ -94,6 +97,9 @@ int64_t lobpolicy_clip_workspace(const int64_t* counts, const int32_t* dtypes, i
 int lobpolicy_clip(void* const* tensors, const int64_t* counts, const int32_t* dtypes, int64_t n, int32_t kind, double max_norm, float* norm,
                    void* workspace, int64_t workspace_bytes, void* stream);
 
+#if defined(__GNUC__)
+#pragma GCC visibility pop
+#endif
 #ifdef __cplusplus
 }
 #endif

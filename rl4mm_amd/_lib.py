@@ -122,9 +122,9 @@ def build_bounds_library(force: bool = False) -> Path:
 
 
 POLICY_LIB_PATH = CSRC / "liblobpolicy.so"
-POLICY_SOURCES = [CSRC / "policy_ops.hip", CSRC.parent.parent / "include" / "lobpolicy.h"]
+POLICY_SOURCES = [CSRC / "policy_ops.hip", CSRC / "policy_scan.hip", CSRC / "policy_common.h", CSRC.parent.parent / "include" / "lobpolicy.h"]
 # -packed-fp32-ops: no v_pk_{add,mul,fma}_f32, some of whose forms are not reliable on this hardware
-POLICY_FLAGS = ["-O3", "--offload-arch=gfx950", "-fPIC", "-shared", "-std=c++17", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-Wno-unknown-warning-option"]
+POLICY_FLAGS = ["-O3", "--offload-arch=gfx950", "-fPIC", "-fvisibility=hidden", "-std=c++17", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 _policy_binding = None
 
 
@@ -132,16 +132,37 @@ def _policy_stale() -> bool:
     return not POLICY_LIB_PATH.exists() or any(s.exists() and s.stat().st_mtime > POLICY_LIB_PATH.stat().st_mtime for s in POLICY_SOURCES)
 
 
+def compile_policy_library(out: Path, extra_flags=(), csrc: Path = CSRC, jobs: int = None) -> None:
+    """hipcc: policy_ops.hip and policy_scan.hip, the latter once for each type and width of a state's rows -> objects (in parallel) -> one
+    shared library at `out`."""
+    import tempfile
+    from concurrent.futures import ThreadPoolExecutor
+
+    hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
+    if not os.path.exists(hipcc):
+        raise RuntimeError("hipcc was not found: cannot build the HIP library")
+    csrc = Path(csrc).resolve()
+    units = [("policy_scan.hip", [f"-DLOBPOLICY_TYPE={t}", f"-DLOBPOLICY_ROWS={rows}"]) for rows in (128, 64, 32) for t in ("float", "__bf16")] + [("policy_ops.hip", [])]
+    with tempfile.TemporaryDirectory(prefix="lobpolicy_build_") as td:
+
+        def one(k):
+            name, defines = units[k]
+            obj = str(Path(td) / f"part{k}.o")
+            subprocess.check_call([hipcc, *POLICY_FLAGS, *extra_flags, *defines, "-c", "-o", obj, str(csrc / name)], cwd=str(csrc))
+            return obj
+
+        with ThreadPoolExecutor(max_workers=jobs or min(len(units), os.cpu_count() or 1)) as ex:
+            objs = list(ex.map(one, range(len(units))))
+        subprocess.check_call([hipcc, "--offload-arch=gfx950", "-fPIC", "-shared", "-o", str(out), *objs])
+
+
 def build_policy_library(force: bool = False) -> Path:
-    """hipcc -> liblobpolicy.so (include/lobpolicy.h), in-tree like the simulator's library and replaced atomically under the same lock."""
+    """liblobpolicy.so (include/lobpolicy.h), in-tree like the simulator's library and replaced atomically under the same lock."""
     if not force and not _policy_stale():
         return POLICY_LIB_PATH
     import fcntl
     import tempfile
 
-    hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
-    if not os.path.exists(hipcc):
-        raise RuntimeError("hipcc was not found: cannot build the HIP library")
     with open(CSRC / ".build.lock", "w") as lock:
         fcntl.flock(lock, fcntl.LOCK_EX)
         try:
@@ -149,7 +170,7 @@ def build_policy_library(force: bool = False) -> Path:
                 fd, tmp = tempfile.mkstemp(suffix=".so", dir=str(CSRC))
                 os.close(fd)
                 try:
-                    subprocess.check_call([hipcc, *POLICY_FLAGS, "-o", tmp, str(POLICY_SOURCES[0])], cwd=str(CSRC))
+                    compile_policy_library(Path(tmp))
                     os.replace(tmp, POLICY_LIB_PATH)
                 finally:
                     if os.path.exists(tmp):

@@ -1,0 +1,105 @@
+// policy_common.h - what the translation units of liblobpolicy.so share: errors, packed loads, the description of a segment's walk.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "../../include/lobpolicy.h"
+
+namespace lobpolicy {
+
+// ---------------------------------------------------------------------------------------------------------------------------
+// host: errors
+
+int fail(int code, const char* format, ...);  // notes the calling thread's message; returns code
+
+inline int launched() {
+    hipError_t e = hipGetLastError();
+    return e == hipSuccess ? LOBPOLICY_OK : fail(LOBPOLICY_ERR_HIP, "launch: %s", hipGetErrorString(e));
+}
+
+#define REQUIRE(condition, ...) \
+    do { \
+        if (!(condition)) return fail(LOBPOLICY_ERR_ARG, __VA_ARGS__); \
+    } while (0)
+
+inline bool aligned(const void* p, int64_t bytes) { return (uintptr_t)p % bytes == 0; }
+constexpr int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// ---------------------------------------------------------------------------------------------------------------------------
+// device: small tools
+
+typedef __bf16 bf16;
+
+template <class T, int W>
+struct alignas(sizeof(T) * W < 16 ? sizeof(T) * W : 16) Pack {
+    T v[W];
+};
+
+template <class T, int W>
+__device__ __forceinline__ void load_pack(const T* p, float* out) {
+    const Pack<T, W> x = *reinterpret_cast<const Pack<T, W>*>(p);
+#pragma unroll
+    for (int i = 0; i < W; ++i) out[i] = (float)x.v[i];
+}
+
+template <class T, int W>
+__device__ __forceinline__ void store_pack(T* p, const float* in) {
+    Pack<T, W> x;
+#pragma unroll
+    for (int i = 0; i < W; ++i) x.v[i] = (T)in[i];
+    *reinterpret_cast<Pack<T, W>*>(p) = x;
+}
+
+__device__ __forceinline__ float wave_sum(float x) {
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d);
+    return x;
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------
+// decay attention over segments
+//
+// One recurrence serves the forward pass and all three gradients: with "queries" a, "keys" b and "values" c,
+//     S = [cut] ? 0 : e^g S;   S += in_scale b_t c_t^T;   out_t = out_scale a_t^T S
+//   out  a = q,  b = k,  c = v   forwards,  S: the state
+//   dq   a = do, b = v,  c = k   forwards,  S: the state, transposed
+//   dk   a = v,  b = do, c = q   backwards, S: the state's gradient, transposed
+//   dv   a = k,  b = q,  c = do  backwards, S: the state's gradient
+// Forwards a token with a reset cuts what came before it.  Backwards the gradient passes from token t + 1 to token t with e^g, unless
+// t + 1 has a reset; what enters behind the last token (the gradient of the final state) enters without a decay, and what leaves
+// in front of token 0 (the gradient of the initial state) leaves with one.
+
+struct Rows {  // one operand: [steps][envs][heads][width], the last dimension contiguous
+    const void* data;
+    int64_t st, sn, sh;
+};
+
+struct Scan {
+    Rows a, b, c, out;
+    const float* log_decay;
+    const uint8_t* reset;
+    int64_t reset_st, reset_sn;
+    const int32_t* lengths;
+    const float* state_in;  // [envs][heads] matrices of da x dc, by the strides below
+    float* state_out;
+    int64_t in_row, in_col, out_row, out_col;
+    int64_t steps, envs;
+    int heads, da, dc;
+    float in_scale, out_scale;
+    int64_t part_steps;  // the steps are split into `parts` of this many, each a workgroup's; state_in and state_out are then [unit][part]
+    int parts;
+    uint8_t* cut_out;  // [unit][part]: whether a reset lies in the part (where out.data is NULL: the walk for the states alone)
+};
+
+__device__ __forceinline__ int64_t length_of(const Scan& s, int64_t n) {
+    if (!s.lengths) return s.steps;
+    const int64_t l = s.lengths[n];
+    return l < 0 ? 0 : (l > s.steps ? s.steps : l);
+}
+
+// one kernel family per type and rows of the state (DA = 32, 64 or 128 holds s.da)
+template <class T, int DA>
+int scan_rows(const Scan& s, bool reverse, hipStream_t stream);
+
+}  // namespace lobpolicy

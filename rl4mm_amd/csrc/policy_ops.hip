@@ -1,17 +1,12 @@
-// policy_ops.hip - the HIP kernels (gfx950) behind include/lobpolicy.h and their C-ABI host side.
-#include <hip/hip_runtime.h>
+// policy_ops.hip - the C-ABI host side of include/lobpolicy.h and the kernels (gfx950) but for those over segments (policy_scan.hip).
+#include "policy_common.h"
 
 #include <cmath>
 #include <cstdarg>
-#include <cstdint>
 #include <cstdio>
+#include <type_traits>
 
-#include "../../include/lobpolicy.h"
-
-namespace {
-
-// ---------------------------------------------------------------------------------------------------------------------------
-// host: errors
+namespace lobpolicy {
 
 thread_local char g_error[256] = "";
 
@@ -23,153 +18,77 @@ int fail(int code, const char* format, ...) {
     return code;
 }
 
-int launched() {
-    hipError_t e = hipGetLastError();
-    return e == hipSuccess ? LOBPOLICY_OK : fail(LOBPOLICY_ERR_HIP, "launch: %s", hipGetErrorString(e));
+template <class T>
+int scan_typed(const Scan& s, bool reverse, hipStream_t stream) {
+    if (s.da <= 32) return scan_rows<T, 32>(s, reverse, stream);
+    if (s.da <= 64) return scan_rows<T, 64>(s, reverse, stream);
+    return scan_rows<T, 128>(s, reverse, stream);
 }
 
-#define REQUIRE(condition, ...) \
-    do { \
-        if (!(condition)) return fail(LOBPOLICY_ERR_ARG, __VA_ARGS__); \
-    } while (0)
-
-constexpr int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
-// ---------------------------------------------------------------------------------------------------------------------------
-// device: small tools
-
-typedef __bf16 bf16;
-
-template <class T, int W>
-struct alignas(sizeof(T) * W < 16 ? sizeof(T) * W : 16) Pack {
-    T v[W];
-};
-
-template <class T, int W>
-__device__ __forceinline__ void load_pack(const T* p, float* out) {
-    const Pack<T, W> x = *reinterpret_cast<const Pack<T, W>*>(p);
-#pragma unroll
-    for (int i = 0; i < W; ++i) out[i] = (float)x.v[i];
-}
-
-template <class T, int W>
-__device__ __forceinline__ void store_pack(T* p, const float* in) {
-    Pack<T, W> x;
-#pragma unroll
-    for (int i = 0; i < W; ++i) x.v[i] = (T)in[i];
-    *reinterpret_cast<Pack<T, W>*>(p) = x;
-}
-
-__device__ __forceinline__ float wave_sum(float x) {
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d);
-    return x;
-}
-
-// ---------------------------------------------------------------------------------------------------------------------------
-// decay attention over segments
-//
-// One recurrence serves the forward pass and all three gradients: with "queries" a, "keys" b and "values" c,
-//     S = [cut] ? 0 : e^g S;   S += in_scale b_t c_t^T;   out_t = out_scale a_t^T S
-//   out  a = q,  b = k,  c = v   forwards,  S: the state
-//   dq   a = do, b = v,  c = k   forwards,  S: the state, transposed
-//   dk   a = v,  b = do, c = q   backwards, S: the state's gradient, transposed
-//   dv   a = k,  b = q,  c = do  backwards, S: the state's gradient
-// Forwards a token with a reset cuts what came before it.  Backwards the gradient passes from token t + 1 to token t with e^g, unless
-// t + 1 has a reset; what enters behind the last token (the gradient of the final state) enters without a decay, and what leaves
-// in front of token 0 (the gradient of the initial state) leaves with one.
-
-struct Rows {  // one operand: [steps][envs][heads][width], the last dimension contiguous
-    const void* data;
-    int64_t st, sn, sh;
-};
-
-struct Scan {
-    Rows a, b, c, out;
-    const float* log_decay;
-    const uint8_t* reset;
-    int64_t reset_st, reset_sn;
-    const int32_t* lengths;
-    const float* state_in;  // [envs][heads] matrices of da x dc, by the strides below
-    float* state_out;
-    int64_t in_row, in_col, out_row, out_col;
-    int64_t steps, envs;
-    int heads, da, dc;
-    float in_scale, out_scale;
-};
-
-__device__ __forceinline__ int64_t length_of(const Scan& s, int64_t n) {
-    if (!s.lengths) return s.steps;
-    const int64_t l = s.lengths[n];
-    return l < 0 ? 0 : (l > s.steps ? s.steps : l);
-}
-
-// The recurrence as it stands, a token at a time: one workgroup per environment and head, a column of the state per thread.
-template <class T, int DA, bool REVERSE>
-__global__ __launch_bounds__(128) void scan_tokens(Scan s) {
-    __shared__ float row_a[DA], row_b[DA];
-    const int64_t unit = blockIdx.x, n = unit / s.heads;
-    const int h = (int)(unit % s.heads), j = threadIdx.x;
-    const float decay = expf(s.log_decay[h]);
-    const int64_t length = length_of(s, n);
-    const T* a = (const T*)s.a.data + n * s.a.sn + h * s.a.sh;
-    const T* b = (const T*)s.b.data + n * s.b.sn + h * s.b.sh;
-    const T* c = (const T*)s.c.data + n * s.c.sn + h * s.c.sh;
-    T* out = (T*)s.out.data + n * s.out.sn + h * s.out.sh;
-    const uint8_t* reset = s.reset ? s.reset + n * s.reset_sn : nullptr;
-    const bool mine = j < s.dc;
-    float state[DA];
-#pragma unroll
-    for (int i = 0; i < DA; ++i) state[i] = s.state_in && mine && i < s.da ? s.state_in[unit * s.da * s.dc + i * s.in_row + j * s.in_col] : 0.f;
-    for (int64_t k = 0; k < length; ++k) {
-        const int64_t t = REVERSE ? length - 1 - k : k;
-        __syncthreads();
-        for (int i = j; i < DA; i += 128) {
-            row_a[i] = i < s.da ? (float)a[t * s.a.st + i] : 0.f;
-            row_b[i] = i < s.da ? (float)b[t * s.b.st + i] * s.in_scale : 0.f;
-        }
-        __syncthreads();
-        const float value = mine ? (float)c[t * s.c.st + j] : 0.f;
-        const bool cut = reset && (REVERSE ? k > 0 && reset[(t + 1) * s.reset_st] : reset[t * s.reset_st]);
-        const float carry = REVERSE && k == 0 ? 1.f : decay;
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < DA; ++i) {
-            state[i] = (cut ? 0.f : state[i] * carry) + row_b[i] * value;
-            if (i < s.da) sum += row_a[i] * state[i];
-        }
-        if (mine) out[t * s.out.st + j] = (T)(sum * s.out_scale);
+// Few environments and heads, many steps: the steps are split into parts.  A first walk finds what each part adds to the state, join_parts
+// turns that into the state in front of each part, a second walk starts from it.
+struct Parts {
+    int64_t steps;
+    int count;
+    Parts(const lobpolicy_attention* a) {
+        const int64_t units = a->envs * a->heads;
+        int64_t n = a->steps < 512 || units >= 512 ? 1 : ceil_div(1024, units);
+        n = n < ceil_div(a->steps, 256) ? n : ceil_div(a->steps, 256);
+        steps = ceil_div(ceil_div(a->steps, n), 64) * 64;
+        count = (int)ceil_div(a->steps, steps);
     }
-    if (mine) {
-        for (int64_t t = length; t < s.steps; ++t) out[t * s.out.st + j] = (T)0.f;
-        if (s.state_out) {
-            const bool leave = REVERSE && length > 0, cut = leave && reset && reset[0];
-#pragma unroll
-            for (int i = 0; i < DA; ++i)
-                if (i < s.da) s.state_out[unit * s.da * s.dc + i * s.out_row + j * s.out_col] = cut ? 0.f : (leave ? state[i] * decay : state[i]);
-        }
+    int64_t matrices(const lobpolicy_attention* a) const { return a->envs * a->heads * count; }
+    int64_t bytes(const lobpolicy_attention* a) const { return count == 1 ? 0 : matrices(a) * (a->dk * a->dv * (int64_t)sizeof(float) + 1); }
+};
+
+// grid (elements / 256, units): `states` [unit][part] from what each part adds to what is in front of it; the state behind the last to state_out
+template <bool REVERSE>
+__global__ __launch_bounds__(256) void join_parts(Scan s, float* states, const uint8_t* cut) {
+    const int64_t unit = blockIdx.y, matrix = (int64_t)s.da * s.dc, e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (e >= matrix) return;
+    const int64_t n = unit / s.heads, length = length_of(s, n), row = e / s.dc, col = e % s.dc;
+    const float log_decay = s.log_decay[unit % s.heads];
+    float state = s.state_in ? s.state_in[unit * matrix + row * s.in_row + col * s.in_col] : 0.f;
+    float* at = states + unit * s.parts * matrix + e;
+#pragma unroll 4
+    for (int part = 0; part < s.parts; ++part) {
+        const int64_t left = length - part * s.part_steps, places = left < 0 ? 0 : left < s.part_steps ? left : s.part_steps;
+        const int64_t decays = places - (REVERSE && part == 0 && places ? 1 : 0);  // (backwards nothing decays in front of the first place)
+        const float added = at[part * matrix];
+        at[part * matrix] = state;
+        state = (cut[unit * s.parts + part] ? 0.f : decays ? state * expf(log_decay * (float)decays) : state) + added;
+    }
+    if (s.state_out) {
+        if (REVERSE && length > 0) state = s.reset && s.reset[n * s.reset_sn] ? 0.f : state * expf(log_decay);
+        s.state_out[unit * matrix + row * s.out_row + col * s.out_col] = state;
     }
 }
 
-template <class T, int DA>
-int scan_launch(const Scan& s, bool reverse, hipStream_t stream) {
-    const dim3 grid((unsigned)(s.envs * s.heads));
+int walk(const lobpolicy_attention* a, const Scan& s, bool reverse, hipStream_t stream) {
+    return a->dtype == LOBPOLICY_BF16 ? scan_typed<bf16>(s, reverse, stream) : scan_typed<float>(s, reverse, stream);
+}
+
+// the states in front of each part, to the workspace (which holds them by rows, whatever s.in_row says); s.state_out
+int part_states(const lobpolicy_attention* a, Scan s, bool reverse, hipStream_t stream) {
+    const Parts parts(a);
+    float* states = (float*)a->workspace;
+    uint8_t* cut = (uint8_t*)(states + parts.matrices(a) * a->dk * a->dv);
+    Scan first = s;
+    first.a = first.b, first.out = {};
+    first.state_in = nullptr, first.state_out = states, first.out_row = s.dc, first.out_col = 1, first.cut_out = cut;
+    if (int e = walk(a, first, reverse, stream)) return e;
+    const dim3 grid((unsigned)ceil_div((int64_t)s.da * s.dc, 256), (unsigned)(a->envs * a->heads));
     if (reverse)
-        scan_tokens<T, DA, true><<<grid, 128, 0, stream>>>(s);
+        join_parts<true><<<grid, 256, 0, stream>>>(s, states, cut);
     else
-        scan_tokens<T, DA, false><<<grid, 128, 0, stream>>>(s);
+        join_parts<false><<<grid, 256, 0, stream>>>(s, states, cut);
     return launched();
 }
 
-template <class T>
-int scan_typed(const Scan& s, bool reverse, hipStream_t stream) {
-    if (s.da <= 32) return scan_launch<T, 32>(s, reverse, stream);
-    if (s.da <= 64) return scan_launch<T, 64>(s, reverse, stream);
-    return scan_launch<T, 128>(s, reverse, stream);
-}
-
-int scan(const lobpolicy_attention* a, const Scan& s, bool reverse, void* stream) {
-    return a->dtype == LOBPOLICY_BF16 ? scan_typed<bf16>(s, reverse, (hipStream_t)stream) : scan_typed<float>(s, reverse, (hipStream_t)stream);
+int check_workspace(const lobpolicy_attention* a) {
+    const int64_t need = Parts(a).bytes(a);
+    REQUIRE(need == 0 || (a->workspace && aligned(a->workspace, 16) && a->workspace_bytes >= need), "the workspace has %lld bytes, %lld are needed", (long long)a->workspace_bytes, (long long)need);
+    return LOBPOLICY_OK;
 }
 
 int check_attention(const lobpolicy_attention* a) {
@@ -197,6 +116,8 @@ Scan scan_of(const lobpolicy_attention* a) {
     s.envs = a->envs;
     s.heads = a->heads;
     s.in_scale = s.out_scale = 1.f;
+    const Parts parts(a);
+    s.parts = parts.count, s.part_steps = parts.steps;
     return s;
 }
 
@@ -507,8 +428,6 @@ int block_wide(const Block& p, bool backward, int64_t parts, hipStream_t stream)
     return block_launch<X, B, VW, 32, 256>(p, backward, parts, stream);
 }
 
-bool aligned(const void* p, int64_t bytes) { return (uintptr_t)p % bytes == 0; }
-
 template <class X, class B>
 int block_typed(const Block& p, bool backward, int64_t parts, hipStream_t stream) {
     auto fits = [&](int w) {
@@ -717,7 +636,9 @@ int64_t clip_parts(const int64_t* counts, const int32_t* dtypes, int64_t n) {
     return parts;
 }
 
-}  // namespace
+}  // namespace lobpolicy
+
+using namespace lobpolicy;
 
 // ---------------------------------------------------------------------------------------------------------------------------
 // the C-ABI
@@ -730,40 +651,60 @@ const char* lobpolicy_last_error(void) { return g_error; }
 int64_t lobpolicy_attention_workspace(const lobpolicy_attention* a, int32_t backward) {
     (void)backward;
     if (int e = check_attention(a)) return e;
-    return 0;
+    return Parts(a).bytes(a);
 }
 
 int lobpolicy_attention_forward(const lobpolicy_attention* a, void* stream) {
     if (int e = check_attention(a)) return e;
     REQUIRE(a->q.data && a->k.data && a->v.data && a->out.data, "an operand is missing");
+    if (int e = check_workspace(a)) return e;
     Scan s = scan_of(a);
     s.a = rows_of(a->q), s.b = rows_of(a->k), s.c = rows_of(a->v), s.out = rows_of(a->out);
     s.da = a->dk, s.dc = a->dv;
     s.out_scale = a->scale;
-    s.state_in = a->state_in, s.in_row = a->dv, s.in_col = 1;
-    s.state_out = a->state_out, s.out_row = a->dv, s.out_col = 1;
-    return scan(a, s, false, stream);
+    s.state_in = a->state_in, s.state_out = a->state_out;
+    s.in_row = s.out_row = a->dv, s.in_col = s.out_col = 1;
+    if (s.parts > 1) {
+        if (int e = part_states(a, s, false, (hipStream_t)stream)) return e;
+        s.state_in = (const float*)a->workspace, s.state_out = nullptr;
+    }
+    return walk(a, s, false, (hipStream_t)stream);
 }
 
 int lobpolicy_attention_backward(const lobpolicy_attention* a, void* stream) {
     if (int e = check_attention(a)) return e;
     REQUIRE(a->q.data && a->k.data && a->v.data && a->out.data, "an operand is missing");
     REQUIRE(a->grad_q.data && a->grad_k.data && a->grad_v.data, "a gradient is missing");
+    if (int e = check_workspace(a)) return e;
+    hipStream_t st = (hipStream_t)stream;
+    const Rows q = rows_of(a->q), k = rows_of(a->k), v = rows_of(a->v), d = rows_of(a->out);
+    const float* states = (const float*)a->workspace;
+    // forwards: the state, for dq
     Scan s = scan_of(a);
-    s.a = rows_of(a->out), s.b = rows_of(a->v), s.c = rows_of(a->k), s.out = rows_of(a->grad_q);
-    s.da = a->dv, s.dc = a->dk;
+    s.state_in = a->state_in;
+    if (s.parts > 1) {
+        s.b = k, s.c = v, s.da = a->dk, s.dc = a->dv, s.in_row = a->dv, s.in_col = 1;
+        if (int e = part_states(a, s, false, st)) return e;
+        s.state_in = states;
+    }
+    s.a = d, s.b = v, s.c = k, s.out = rows_of(a->grad_q);
+    s.da = a->dv, s.dc = a->dk, s.in_row = 1, s.in_col = a->dv;
     s.out_scale = a->scale;
-    s.state_in = a->state_in, s.in_row = 1, s.in_col = a->dv;
-    if (int e = scan(a, s, false, stream)) return e;
-    s.a = rows_of(a->v), s.b = rows_of(a->out), s.c = rows_of(a->q), s.out = rows_of(a->grad_k);
+    if (int e = walk(a, s, false, st)) return e;
+    // backwards: its gradient, for dv and dk
     s.out_scale = 1.f, s.in_scale = a->scale;
-    s.state_in = a->grad_state_out;
-    if (int e = scan(a, s, true, stream)) return e;
-    s.a = rows_of(a->k), s.b = rows_of(a->q), s.c = rows_of(a->out), s.out = rows_of(a->grad_v);
-    s.da = a->dk, s.dc = a->dv;
-    s.in_row = s.out_row = a->dv, s.in_col = s.out_col = 1;
-    s.state_out = a->grad_state_in;
-    return scan(a, s, true, stream);
+    s.state_in = a->grad_state_out, s.state_out = a->grad_state_in;
+    s.a = k, s.b = q, s.c = d, s.out = rows_of(a->grad_v);
+    s.da = a->dk, s.dc = a->dv, s.in_row = s.out_row = a->dv, s.in_col = s.out_col = 1;
+    if (s.parts > 1) {
+        if (int e = part_states(a, s, true, st)) return e;
+        s.state_in = states, s.state_out = nullptr;
+    }
+    if (int e = walk(a, s, true, st)) return e;
+    s.state_out = nullptr;
+    s.a = v, s.b = d, s.c = q, s.out = rows_of(a->grad_k);
+    s.da = a->dv, s.dc = a->dk, s.in_row = 1, s.in_col = a->dv;
+    return walk(a, s, true, st);
 }
 
 int lobpolicy_attention_step(const lobpolicy_attention* a, void* stream) {

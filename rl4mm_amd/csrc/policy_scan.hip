@@ -1,0 +1,442 @@
+// policy_scan.hip - decay attention over segments: the kernels of one type and one width of a state's rows, chosen by -DLOBPOLICY_TYPE and
+// -DLOBPOLICY_ROWS (the library holds the six of float and __bf16 with 32, 64 and 128).
+#include "policy_common.h"
+
+namespace lobpolicy {
+
+// ---- chunks of tokens on the matrix units ------------------------------------------------------------------------------------
+//
+// CH tokens at a time, with the state S at their beginning (p: place in the chunk, e^g = l):
+//     out_i = out_scale ( l^(i+1) a_i S + sum_{j <= i} l^(i-j) in_scale (a_i . b_j) c_j ),    S <- l^CH S + sum_j l^(CH-1-j) in_scale b_j c_j^T
+// where a reset between j and i takes the term away.  Four products of tiles, on 16x16 matrix instructions; one workgroup walks the
+// chunks of one environment and head (or of a part of its steps), its waves share the state by columns:
+//   - scores, transposed (rows j, columns i), weighted, rounded to T and put to LDS, each tile by one wave
+//   - out, transposed (rows c, columns i), each wave its own columns of the state: S as it lies in the accumulators is the left operand
+//     of a_i S (an accumulator holds rows 4 (lane / 16) .. + 3 of column lane % 16, which read the other way round is the operand's
+//     layout), so the state never leaves the registers
+//   - the state's update
+// The tiles a, b, c lie in LDS as they lie in memory; what needs them by columns reads them transposed (bf16: the transposing LDS load,
+// f32: single words).  Rows are padded by 16 bytes, which spreads 16 rows over all banks.  The next chunk's tiles are on their way from
+// memory while one is computed.
+//
+// Exponents are never negative (all products are of j <= i), so no decay overflows.  What is masked is selected away, not multiplied by
+// 0; a chunk that holds an infinity or a NaN anywhere is computed token by token instead, from the same LDS tiles, because a matrix
+// product would spread it to tokens that do not see it.
+//
+// bf16: the scores and the state's copy that multiplies a are rounded to bf16 once (half a step, 2^-8, of single terms, like the output's own
+// rounding); the state itself is kept in 32 bits, its update's weighted c split into three bf16 that together hold 24 bits.
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+template <class T>
+struct Tile;
+
+template <>
+struct Tile<float> {  // a fragment: 16 of the summed index, places 4 (lane / 16) + r in its word r
+    typedef f32x4 Frag;
+    static constexpr int K = 16, PAD = 4;
+    static __device__ __forceinline__ f32x4 product(Frag a, Frag b, f32x4 c) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r], b[r], c, 0, 0, 0);
+        return c;
+    }
+    static __device__ __forceinline__ Frag rows(const float* tile, int stride, int row, int k) {  // tile[row + lane % 16][k ..]
+        const int l = threadIdx.x % 16, g = threadIdx.x % 64 / 16;
+        return *reinterpret_cast<const f32x4*>(tile + (row + l) * stride + k + 4 * g);
+    }
+    static __device__ __forceinline__ Frag rows_as_state(const float* tile, int stride, int row, int k) { return rows(tile, stride, row, k); }
+    static __device__ __forceinline__ Frag columns(const float* tile, int stride, int k, int column) {  // tile[k ..][column + lane % 16]
+        const int l = threadIdx.x % 16, g = threadIdx.x % 64 / 16;
+        Frag f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) f[r] = tile[(k + 4 * g + r) * stride + column + l];
+        return f;
+    }
+    static __device__ __forceinline__ int place(int e) { return 4 * (threadIdx.x % 64 / 16) + e; }  // of a fragment's element e in `columns`
+    static __device__ __forceinline__ Frag of_state(const f32x4* s) { return s[0]; }
+    static constexpr int SPLITS = 1;
+    // c's columns times w, as SPLITS fragments whose sum is the product
+    static __device__ __forceinline__ void weighted(Frag c, const float* w, Frag* f) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) f[0][r] = c[r] * w[r];
+    }
+};
+
+template <>
+struct Tile<bf16> {  // a fragment: 32 of the summed index, places 8 (lane / 16) + e
+    typedef bf16x8 Frag;
+    static constexpr int K = 32, PAD = 8;
+    static __device__ __forceinline__ f32x4 product(Frag a, Frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ Frag rows(const bf16* tile, int stride, int row, int k) {
+        const int l = threadIdx.x % 16, g = threadIdx.x % 64 / 16;
+        return *reinterpret_cast<const bf16x8*>(tile + (row + l) * stride + k + 8 * g);
+    }
+    // the order in which two accumulators one above the other hold the summed index: 4 (lane / 16) + r, then 16 more
+    static __device__ __forceinline__ Frag rows_as_state(const bf16* tile, int stride, int row, int k) {
+        const int l = threadIdx.x % 16, g = threadIdx.x % 64 / 16;
+        const bf16x4 lo = *reinterpret_cast<const bf16x4*>(tile + (row + l) * stride + k + 4 * g), hi = *reinterpret_cast<const bf16x4*>(tile + (row + l) * stride + k + 16 + 4 * g);
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+    // 16 lanes that address 4 rows of 16 elements, 4 elements each, get a column each
+    static __device__ __forceinline__ Frag columns(const bf16* tile, int stride, int k, int column) {
+        const int l = threadIdx.x % 16, g = threadIdx.x % 64 / 16;
+        typedef __attribute__((address_space(3))) s16x4 lds;
+        const bf16* at = tile + (k + 8 * g + l / 4) * stride + column + l % 4 * 4;
+        const bf16x4 lo = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds*)(at)));
+        const bf16x4 hi = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds*)(at + 4 * stride)));
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+    static __device__ __forceinline__ int place(int e) { return 8 * (threadIdx.x % 64 / 16) + e; }
+    static __device__ __forceinline__ Frag of_state(const f32x4* s) {
+        Frag f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) f[r] = (bf16)s[0][r], f[4 + r] = (bf16)s[1][r];
+        return f;
+    }
+    static constexpr int SPLITS = 3;
+    static __device__ __forceinline__ void weighted(Frag c, const float* w, Frag* f) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            float x = (float)c[e] * w[e];
+#pragma unroll
+            for (int i = 0; i < 3; ++i) f[i][e] = (bf16)x, x -= (float)f[i][e];
+        }
+    }
+};
+
+template <class T, int CH, int DA, int DC>
+struct Shape {
+    static constexpr int WAVES = DC == 32 ? 2 : 4, THREADS = 64 * WAVES;
+    static constexpr int COLS = DC / 16 / WAVES;  // tiles of 16 of the state's columns per wave
+    static constexpr int PAD = Tile<T>::PAD, SA = DA + PAD, SC = DC + PAD, SP = CH + PAD, VW = 16 / (int)sizeof(T);
+};
+
+// whether one of the 16 bytes' numbers has all exponent bits set
+template <class T>
+__device__ __forceinline__ uint32_t not_finite(uint4 x) {
+    constexpr uint32_t mask = sizeof(T) == 2 ? 0x7f807f80u : 0x7f800000u, one = sizeof(T) == 2 ? 0x00800080u : 0x00800000u;
+    return ((x.x & mask) + one) | ((x.y & mask) + one) | ((x.z & mask) + one) | ((x.w & mask) + one);
+}
+template <class T>
+constexpr uint32_t NOT_FINITE = sizeof(T) == 2 ? 0x80008000u : 0x80000000u;
+
+// A tile's share of a thread, on its way: places first .. first + CH - 1 in the order of the walk, 16 bytes at a time.  The walk goes
+// over the tokens 0 .. length - 1 or backwards; places from `end` on are 0.
+template <class T, int CH, int D, int THREADS, bool VEC, bool REVERSE>
+struct Moving {
+    static constexpr int VW = 16 / (int)sizeof(T), PACKS = CH * D / VW, N = PACKS / THREADS;
+    static_assert(PACKS % THREADS == 0, "");
+    uint4 x[N];
+
+    __device__ __forceinline__ void load(const T* base, int64_t st, int64_t first, int64_t end, int64_t length, int width) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int pack = n * THREADS + threadIdx.x, row = pack / (D / VW), col = pack % (D / VW) * VW;
+            const int64_t p = first + row;
+            x[n] = make_uint4(0, 0, 0, 0);
+            if (p < end && col < width) {
+                const T* from = base + (REVERSE ? length - 1 - p : p) * st + col;
+                if (VEC)
+                    x[n] = *reinterpret_cast<const uint4*>(from);
+                else {
+                    Pack<T, VW> one;
+#pragma unroll
+                    for (int e = 0; e < VW; ++e) one.v[e] = col + e < width ? from[e] : (T)0.f;
+                    x[n] = __builtin_bit_cast(uint4, one);
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ uint32_t store(T* tile, int stride) const {
+        uint32_t bad = 0;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int pack = n * THREADS + threadIdx.x, row = pack / (D / VW), col = pack % (D / VW) * VW;
+            *reinterpret_cast<uint4*>(tile + row * stride + col) = x[n];
+            bad |= not_finite<T>(x[n]);
+        }
+        return bad;
+    }
+};
+
+// OUT: the walk's outputs; without it the state behind each part alone, from a state of 0 in front of it
+template <class T, int CH, int DA, int DC, bool REVERSE, bool OUT, bool VEC>
+__global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS)) void scan_chunks(Scan s) {
+    typedef Shape<T, CH, DA, DC> S;
+    typedef Tile<T> M;
+    typedef typename M::Frag Frag;
+    constexpr int NT = CH / 16, KA = DA / M::K, KC = CH / M::K, DT = DA / 16, PER = M::K / 16;
+    __shared__ __align__(16) T tile_a[OUT ? CH * S::SA : 8];
+    __shared__ __align__(16) T tile_b[CH * S::SA];
+    __shared__ __align__(16) T tile_c[CH * S::SC];
+    __shared__ __align__(16) T tile_p[OUT ? CH * S::SP : 8];
+    __shared__ float power[CH + 1];
+    __shared__ uint32_t spoiled[2];
+
+    // neighbouring workgroups run on different dies, each with a cache of its own: every die gets a run of neighbouring units
+    const int64_t blocks = gridDim.x, die = blockIdx.x % 8, each = blocks / 8, more = blocks % 8;
+    const int64_t index = die * each + (die < more ? die : more) + blockIdx.x / 8;
+    const int64_t units = s.envs * s.heads, unit = index % units, part = index / units, n = unit / s.heads;
+    const int h = (int)(unit % s.heads);
+    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, l = lane % 16, g = lane / 16, column = wave * S::COLS * 16;
+
+    const int64_t length = length_of(s, n), begin = part * s.part_steps;
+    const int64_t end = begin + s.part_steps < length ? begin + s.part_steps : length;
+    const T* a = (const T*)s.a.data + n * s.a.sn + h * s.a.sh;
+    const T* b = (const T*)s.b.data + n * s.b.sn + h * s.b.sh;
+    const T* c = (const T*)s.c.data + n * s.c.sn + h * s.c.sh;
+    T* out = OUT ? (T*)s.out.data + n * s.out.sn + h * s.out.sh : nullptr;
+    const uint8_t* reset = s.reset ? s.reset + n * s.reset_sn : nullptr;
+    // of the chunk from place `first` on: whether nothing in front of place first + lane reaches it
+    auto load_flag = [&](int64_t first) -> uint32_t {
+        const int64_t p = first + lane;
+        return reset && lane < CH && p < end && (!REVERSE || p > 0) ? reset[(REVERSE ? length - p : p) * s.reset_st] : 0;
+    };
+
+    const float log_decay = s.log_decay[h];
+    auto decay_of = [&](int k) { return k == 0 ? 1.f : expf(log_decay * (float)k); };  // (k = 0: not 0 * infinity)
+    for (int k = threadIdx.x; k <= CH; k += S::THREADS) power[k] = decay_of(k);
+    if (threadIdx.x < 2) spoiled[threadIdx.x] = 0;
+    float w_diagonal[4], w_below[4];  // of a score tile on the diagonal, and of the one below it
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int gap = l - 4 * g - r;
+        w_diagonal[r] = gap >= 0 ? decay_of(gap) * s.in_scale : 0.f;
+        w_below[r] = decay_of(16 + gap) * s.in_scale;
+    }
+
+    const int64_t matrix = (int64_t)s.da * s.dc, which = s.parts == 1 ? unit : unit * s.parts + part;
+    f32x4 state[S::COLS][DT];  // rows 16 t + 4 g + r, column `column` + 16 ct + l
+#pragma unroll
+    for (int ct = 0; ct < S::COLS; ++ct)
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int i = 16 * t + 4 * g + r, j = column + 16 * ct + l;
+                state[ct][t][r] = s.state_in && i < s.da && j < s.dc ? s.state_in[which * matrix + i * s.in_row + j * s.in_col] : 0.f;
+            }
+
+    Moving<T, CH, DA, S::THREADS, VEC, REVERSE> move_a, move_b;
+    Moving<T, CH, DC, S::THREADS, VEC, REVERSE> move_c;
+    uint32_t flag = 0;
+    if (begin < end) {
+        if (OUT) move_a.load(a, s.a.st, begin, end, length, s.da);
+        move_b.load(b, s.b.st, begin, end, length, s.da);
+        move_c.load(c, s.c.st, begin, end, length, s.dc);
+        flag = load_flag(begin);
+    }
+    int parity = 0;
+    uint64_t any_cut = 0;
+    for (int64_t first = begin; first < end; first += CH, parity ^= 1) {
+        const int places = end - first < CH ? (int)(end - first) : CH;
+        uint32_t bad = OUT ? move_a.store(tile_a, S::SA) : 0;
+        bad |= move_b.store(tile_b, S::SA);
+        bad |= move_c.store(tile_c, S::SC);
+        if (bad & NOT_FINITE<T>) spoiled[parity] = 1;
+        const uint64_t cuts = __ballot(flag != 0);
+        any_cut |= cuts;
+        __syncthreads();
+        const bool by_token = spoiled[parity] != 0;
+        if (threadIdx.x == 0) spoiled[parity ^ 1] = 0;
+        if (first + CH < end) {
+            if (OUT) move_a.load(a, s.a.st, first + CH, end, length, s.da);
+            move_b.load(b, s.b.st, first + CH, end, length, s.da);
+            move_c.load(c, s.c.st, first + CH, end, length, s.dc);
+            flag = load_flag(first + CH);
+        }
+        const int enters = REVERSE && first == 0 ? 0 : 1;  // decays between what comes into the chunk and its first place
+        auto token = [&](int p) { return (REVERSE ? length - 1 - (first + p) : first + p) * s.out.st; };
+
+        if (by_token) {
+            for (int p = 0; p < places; ++p) {
+                const bool cut = cuts >> p & 1;
+                const float carry = power[p == 0 ? enters : 1];
+#pragma unroll
+                for (int ct = 0; ct < S::COLS; ++ct) {
+                    const int j = column + 16 * ct + l;
+                    const float value = (float)tile_c[p * S::SC + j] * s.in_scale;
+                    float sum = 0.f;
+#pragma unroll
+                    for (int t = 0; t < DT; ++t)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const int i = 16 * t + 4 * g + r;
+                            if (i < s.da) {
+                                state[ct][t][r] = (cut ? 0.f : state[ct][t][r] * carry) + (float)tile_b[p * S::SA + i] * value;
+                                if (OUT) sum += (float)tile_a[p * S::SA + i] * state[ct][t][r];
+                            }
+                        }
+                    if (OUT) {
+                        sum += __shfl_xor(sum, 16);
+                        sum += __shfl_xor(sum, 32);
+                        if (g == 0 && j < s.dc) out[token(p) + j] = (T)(sum * s.out_scale);
+                    }
+                }
+            }
+            __syncthreads();
+            continue;
+        }
+
+        const int tiles = (places + 15) / 16;
+        if (OUT) {
+            // scores: tile (it, jt) holds rows j = 16 jt + .., columns i = 16 it + ..
+            for (int k = wave; k < tiles * (tiles + 1) / 2; k += S::WAVES) {
+                const int it = k >= 6 ? 3 : k >= 3 ? 2 : k >= 1 ? 1 : 0, jt = k - it * (it + 1) / 2, i = 16 * it + l;
+                f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int kk = 0; kk < KA; ++kk) x = M::product(M::rows(tile_b, S::SA, 16 * jt, kk * M::K), M::rows(tile_a, S::SA, 16 * it, kk * M::K), x);
+                const uint64_t before = cuts & (~0ull >> (63 - i));
+                const int from = before ? 63 - __builtin_clzll(before) : 0;  // the first place that i sees
+                const float far = it - jt > 1 ? power[16 * (it - jt - 1)] : 1.f;
+                Pack<T, 4> p;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int j = 16 * jt + 4 * g + r;
+                    const float w = it == jt ? w_diagonal[r] : w_below[r] * far;
+                    p.v[r] = (T)(j <= i && j >= from ? x[r] * w : 0.f);
+                }
+                *reinterpret_cast<Pack<T, 4>*>(tile_p + i * S::SP + 16 * jt + 4 * g) = p;
+                if (PER == 2 && it == jt && it % 2 == 0) {  // the tile above the diagonal that shares a fragment with it
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) p.v[r] = (T)0.f;
+                    *reinterpret_cast<Pack<T, 4>*>(tile_p + i * S::SP + 16 * jt + 16 + 4 * g) = p;
+                }
+            }
+            __syncthreads();
+            Frag left[S::COLS][KA];
+#pragma unroll
+            for (int ct = 0; ct < S::COLS; ++ct)
+#pragma unroll
+                for (int kk = 0; kk < KA; ++kk) left[ct][kk] = M::of_state(&state[ct][kk * PER]);
+#pragma unroll
+            for (int it = 0; it < NT; ++it) {
+                if (it >= tiles) break;
+                const int i = 16 * it + l;
+                const bool sees = (cuts & (~0ull >> (63 - i))) == 0;
+                const float w = power[i + enters];
+                f32x4 x[S::COLS];
+#pragma unroll
+                for (int ct = 0; ct < S::COLS; ++ct) x[ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int kk = 0; kk < KA; ++kk) {
+                    const Frag right = M::rows_as_state(tile_a, S::SA, 16 * it, kk * M::K);
+#pragma unroll
+                    for (int ct = 0; ct < S::COLS; ++ct) x[ct] = M::product(left[ct][kk], right, x[ct]);
+                }
+#pragma unroll
+                for (int ct = 0; ct < S::COLS; ++ct)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) x[ct][r] = sees ? x[ct][r] * w : 0.f;
+#pragma unroll
+                for (int kk = 0; kk <= it / PER; ++kk) {
+                    const Frag right = M::rows(tile_p, S::SP, 16 * it, kk * M::K);
+#pragma unroll
+                    for (int ct = 0; ct < S::COLS; ++ct) x[ct] = M::product(M::columns(tile_c, S::SC, kk * M::K, column + 16 * ct), right, x[ct]);
+                }
+                if (i < places) {
+#pragma unroll
+                    for (int ct = 0; ct < S::COLS; ++ct) {
+                        const int j = column + 16 * ct + 4 * g;
+                        float y[4];
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) y[r] = x[ct][r] * s.out_scale;
+                        if (VEC) {
+                            if (j < s.dc) store_pack<T, 4>(out + token(i) + j, y);
+                        } else
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                if (j + r < s.dc) out[token(i) + j + r] = (T)y[r];
+                    }
+                }
+            }
+        }
+        // the state: what comes in decays by the whole chunk, place j by what lies behind it
+        const int last_cut = cuts ? 63 - __builtin_clzll(cuts) : 0;
+        const float whole = power[places - 1 + enters];
+#pragma unroll
+        for (int ct = 0; ct < S::COLS; ++ct)
+#pragma unroll
+            for (int t = 0; t < DT; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) state[ct][t][r] = cuts ? 0.f : state[ct][t][r] * whole;
+#pragma unroll
+        for (int kk = 0; kk < KC; ++kk) {
+            if (kk * M::K >= places) break;
+            Frag right[S::COLS][M::SPLITS];
+            float w[M::K / 4];
+#pragma unroll
+            for (int e = 0; e < M::K / 4; ++e) {
+                const int j = kk * M::K + M::place(e);
+                w[e] = j >= last_cut && j < places ? power[places - 1 - j] * s.in_scale : 0.f;
+            }
+#pragma unroll
+            for (int ct = 0; ct < S::COLS; ++ct) M::weighted(M::columns(tile_c, S::SC, kk * M::K, column + 16 * ct), w, right[ct]);
+#pragma unroll
+            for (int t = 0; t < DT; ++t) {
+                const Frag left = M::columns(tile_b, S::SA, kk * M::K, 16 * t);
+#pragma unroll
+                for (int ct = 0; ct < S::COLS; ++ct)
+#pragma unroll
+                    for (int i = 0; i < M::SPLITS; ++i) state[ct][t] = M::product(left, right[ct][i], state[ct][t]);
+            }
+        }
+        __syncthreads();
+    }
+
+    if (OUT && part == s.parts - 1)  // rows behind the last token
+        for (int64_t t = length + threadIdx.x / 32; t < s.steps; t += S::THREADS / 32)
+            for (int j = threadIdx.x % 32; j < s.dc; j += 32) out[t * s.out.st + j] = (T)0.f;
+    if (!OUT && threadIdx.x == 0) s.cut_out[which] = any_cut != 0;
+    if (s.state_out) {
+        const bool leaves = REVERSE && s.parts == 1 && length > 0, cut = leaves && reset && reset[0];
+        const float carry = leaves ? power[1] : 1.f;
+#pragma unroll
+        for (int ct = 0; ct < S::COLS; ++ct)
+#pragma unroll
+            for (int t = 0; t < DT; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int i = 16 * t + 4 * g + r, j = column + 16 * ct + l;
+                    if (i < s.da && j < s.dc) s.state_out[which * matrix + i * s.out_row + j * s.out_col] = cut ? 0.f : state[ct][t][r] * carry;
+                }
+    }
+}
+
+template <class T, int CH, int DA, int DC, bool VEC>
+int scan_launch(const Scan& s, bool reverse, hipStream_t stream) {
+    const dim3 grid((unsigned)(s.envs * s.heads * s.parts));
+    constexpr int threads = Shape<T, CH, DA, DC>::THREADS;
+    if (s.out.data && reverse)
+        scan_chunks<T, CH, DA, DC, true, true, VEC><<<grid, threads, 0, stream>>>(s);
+    else if (s.out.data)
+        scan_chunks<T, CH, DA, DC, false, true, VEC><<<grid, threads, 0, stream>>>(s);
+    else if (reverse)
+        scan_chunks<T, CH, DA, DC, true, false, VEC><<<grid, threads, 0, stream>>>(s);
+    else
+        scan_chunks<T, CH, DA, DC, false, false, VEC><<<grid, threads, 0, stream>>>(s);
+    return launched();
+}
+
+template <class T, int CH, int DA, int DC>
+int scan_aligned(const Scan& s, bool reverse, hipStream_t stream) {
+    constexpr int W = 16 / sizeof(T);
+    bool wide = s.da % W == 0 && s.dc % W == 0 && aligned(s.out.data, 16);
+    for (const Rows* r : {&s.a, &s.b, &s.c}) wide = wide && aligned(r->data, 16) && r->st % W == 0 && r->sn % W == 0 && r->sh % W == 0;
+    wide = wide && s.out.st % 4 == 0 && s.out.sn % 4 == 0 && s.out.sh % 4 == 0;
+    return wide ? scan_launch<T, CH, DA, DC, true>(s, reverse, stream) : scan_launch<T, CH, DA, DC, false>(s, reverse, stream);
+}
+
+template <class T, int DA>
+int scan_rows(const Scan& s, bool reverse, hipStream_t stream) {
+    if (s.dc <= 32) return scan_aligned<T, 64, DA, 32>(s, reverse, stream);
+    if (s.dc <= 64) return scan_aligned<T, 64, DA, 64>(s, reverse, stream);
+    return scan_aligned<T, 64, DA, 128>(s, reverse, stream);
+}
+
+template int scan_rows<LOBPOLICY_TYPE, LOBPOLICY_ROWS>(const Scan&, bool, hipStream_t);
+
+}  // namespace lobpolicy

@@ -238,6 +238,22 @@ def test_a_long_axis(ops, dtype):
     check(run(ops, p, dout, dlast), p, dout, dlast)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("size", [(48, 80), (128, 64), (30, 21)], ids=str)
+def test_a_long_axis_with_masks(ops, size, dtype):
+    """lengths that end before, at and behind the borders of its parts; resets there; a part without one"""
+    lengths = [0, 1, 255, 256, 257, 511, 512, 1000, 1023, 1024, 1100, 1099]
+    p, dout, dlast = problem(15, 1100, len(lengths), 1, *size, dtype)
+    p["lengths"] = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    p["reset"] = torch.zeros(1100, len(lengths), dtype=torch.bool, device="cuda")
+    for t, n in ((256, 7), (255, 8), (512, 9), (513, 9), (1023, 10), (0, 10), (100, 6), (1098, 11), (1099, 11), (843, 11), (844, 10), (588, 11), (75, 10)):
+        p["reset"][t, n] = True
+    p["log_decay"] = torch.tensor([-0.002], device="cuda")
+    check(run(ops, p, dout, dlast), p, dout, dlast)
+    one = {**p, **{key: p[key][:, 3:4] for key in ("q", "k", "v", "reset")}, "state": p["state"][3:4], "lengths": None}
+    check(run(ops, one, dout[:, 3:4], dlast[3:4]), one, dout[:, 3:4], dlast[3:4])
+
+
 def test_empty(ops):
     for shape in ((0, 3, 2), (5, 0, 2)):
         q, v, s = torch.zeros(*shape, 8, device="cuda"), torch.zeros(*shape, 4, device="cuda", requires_grad=True), normal(1, shape[1], 2, 8, 4).requires_grad_(True)

@@ -31,6 +31,13 @@ typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
+// a lane's place in a 16 x 16 tile.  `fresh` makes it a value that the compiler knows nothing of: what is worked out from it inside the walk
+// (addresses, comparisons) is then worked out where it is used, and not kept in registers from chunk to chunk
+struct Lane {
+    int l, g;
+    __device__ __forceinline__ void fresh() { asm volatile("" : "+v"(l), "+v"(g)); }
+};
+
 template <class T>
 struct Tile;
 
@@ -43,19 +50,17 @@ struct Tile<float> {  // a fragment: 16 of the summed index, places 4 (lane / 16
         for (int r = 0; r < 4; ++r) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r], b[r], c, 0, 0, 0);
         return c;
     }
-    static __device__ __forceinline__ Frag rows(const float* tile, int stride, int row, int k) {  // tile[row + lane % 16][k ..]
-        const int l = threadIdx.x % 16, g = threadIdx.x % 64 / 16;
-        return *reinterpret_cast<const f32x4*>(tile + (row + l) * stride + k + 4 * g);
+    static __device__ __forceinline__ Frag rows(Lane at, const float* tile, int stride, int row, int k) {  // tile[row + lane % 16][k ..]
+        return *reinterpret_cast<const f32x4*>(tile + (row + at.l) * stride + k + 4 * at.g);
     }
-    static __device__ __forceinline__ Frag rows_as_state(const float* tile, int stride, int row, int k) { return rows(tile, stride, row, k); }
-    static __device__ __forceinline__ Frag columns(const float* tile, int stride, int k, int column) {  // tile[k ..][column + lane % 16]
-        const int l = threadIdx.x % 16, g = threadIdx.x % 64 / 16;
+    static __device__ __forceinline__ Frag rows_as_state(Lane at, const float* tile, int stride, int row, int k) { return rows(at, tile, stride, row, k); }
+    static __device__ __forceinline__ Frag columns(Lane at, const float* tile, int stride, int k, int column) {  // tile[k ..][column + lane % 16]
         Frag f;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) f[r] = tile[(k + 4 * g + r) * stride + column + l];
+        for (int r = 0; r < 4; ++r) f[r] = tile[(k + 4 * at.g + r) * stride + column + at.l];
         return f;
     }
-    static __device__ __forceinline__ int place(int e) { return 4 * (threadIdx.x % 64 / 16) + e; }  // of a fragment's element e in `columns`
+    static __device__ __forceinline__ int place(Lane at, int e) { return 4 * at.g + e; }  // of a fragment's element e in `columns`
     static __device__ __forceinline__ Frag of_state(const f32x4* s) { return s[0]; }
     static constexpr int SPLITS = 1;
     // c's columns times w, as SPLITS fragments whose sum is the product
@@ -70,26 +75,23 @@ struct Tile<bf16> {  // a fragment: 32 of the summed index, places 8 (lane / 16)
     typedef bf16x8 Frag;
     static constexpr int K = 32, PAD = 8;
     static __device__ __forceinline__ f32x4 product(Frag a, Frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
-    static __device__ __forceinline__ Frag rows(const bf16* tile, int stride, int row, int k) {
-        const int l = threadIdx.x % 16, g = threadIdx.x % 64 / 16;
-        return *reinterpret_cast<const bf16x8*>(tile + (row + l) * stride + k + 8 * g);
+    static __device__ __forceinline__ Frag rows(Lane at, const bf16* tile, int stride, int row, int k) {
+        return *reinterpret_cast<const bf16x8*>(tile + (row + at.l) * stride + k + 8 * at.g);
     }
     // the order in which two accumulators one above the other hold the summed index: 4 (lane / 16) + r, then 16 more
-    static __device__ __forceinline__ Frag rows_as_state(const bf16* tile, int stride, int row, int k) {
-        const int l = threadIdx.x % 16, g = threadIdx.x % 64 / 16;
-        const bf16x4 lo = *reinterpret_cast<const bf16x4*>(tile + (row + l) * stride + k + 4 * g), hi = *reinterpret_cast<const bf16x4*>(tile + (row + l) * stride + k + 16 + 4 * g);
+    static __device__ __forceinline__ Frag rows_as_state(Lane at, const bf16* tile, int stride, int row, int k) {
+        const bf16x4 lo = *reinterpret_cast<const bf16x4*>(tile + (row + at.l) * stride + k + 4 * at.g), hi = *reinterpret_cast<const bf16x4*>(tile + (row + at.l) * stride + k + 16 + 4 * at.g);
         return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     }
     // 16 lanes that address 4 rows of 16 elements, 4 elements each, get a column each
-    static __device__ __forceinline__ Frag columns(const bf16* tile, int stride, int k, int column) {
-        const int l = threadIdx.x % 16, g = threadIdx.x % 64 / 16;
+    static __device__ __forceinline__ Frag columns(Lane at, const bf16* tile, int stride, int k, int column) {
         typedef __attribute__((address_space(3))) s16x4 lds;
-        const bf16* at = tile + (k + 8 * g + l / 4) * stride + column + l % 4 * 4;
-        const bf16x4 lo = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds*)(at)));
-        const bf16x4 hi = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds*)(at + 4 * stride)));
+        const bf16* from = tile + (k + 8 * at.g + at.l / 4) * stride + column + at.l % 4 * 4;
+        const bf16x4 lo = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds*)(from)));
+        const bf16x4 hi = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds*)(from + 4 * stride)));
         return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     }
-    static __device__ __forceinline__ int place(int e) { return 8 * (threadIdx.x % 64 / 16) + e; }
+    static __device__ __forceinline__ int place(Lane at, int e) { return 8 * at.g + e; }
     static __device__ __forceinline__ Frag of_state(const f32x4* s) {
         Frag f;
 #pragma unroll
@@ -109,9 +111,8 @@ struct Tile<bf16> {  // a fragment: 32 of the summed index, places 8 (lane / 16)
 
 template <class T, int CH, int DA, int DC>
 struct Shape {
-    static constexpr int WAVES = DC == 32 ? 2 : 4, THREADS = 64 * WAVES;
-    static constexpr int COLS = DC / 16 / WAVES;  // tiles of 16 of the state's columns per wave
-    static constexpr int PAD = Tile<T>::PAD, SA = DA + PAD, SC = DC + PAD, SP = CH + PAD, VW = 16 / (int)sizeof(T);
+    static constexpr int WAVES = DC / 16, THREADS = 64 * WAVES;  // a wave per 16 of the state's columns
+    static constexpr int PAD = Tile<T>::PAD, SA = DA + PAD, SC = DC + PAD, SP = CH + PAD;
 };
 
 // whether one of the 16 bytes' numbers has all exponent bits set
@@ -123,52 +124,79 @@ __device__ __forceinline__ uint32_t not_finite(uint4 x) {
 template <class T>
 constexpr uint32_t NOT_FINITE = sizeof(T) == 2 ? 0x80008000u : 0x80000000u;
 
-// A tile's share of a thread, on its way: places first .. first + CH - 1 in the order of the walk, 16 bytes at a time.  The walk goes
-// over the tokens 0 .. length - 1 or backwards; places from `end` on are 0.
-template <class T, int CH, int D, int THREADS, bool VEC, bool REVERSE>
+// A tile's share of a thread, on its way: CH places in the order of the walk, 16 bytes at a time.  `at` is the thread's first row in the chunk to be
+// loaded next, `step` the bytes from place to place (negative where the walk goes backwards).
+template <class T, int CH, int D, int THREADS, bool VEC>
 struct Moving {
-    static constexpr int VW = 16 / (int)sizeof(T), PACKS = CH * D / VW, N = PACKS / THREADS;
-    static_assert(PACKS % THREADS == 0, "");
+    static constexpr int VW = 16 / (int)sizeof(T), ROW = D / VW, ROWS = THREADS / ROW, N = CH > ROWS ? CH / ROWS : 1;
+    static_assert(THREADS % ROW == 0 && (CH % ROWS == 0 || ROWS % CH == 0), "");
+    static __device__ __forceinline__ bool takes_part() { return ROWS <= CH || (int)(threadIdx.x / ROW) < CH; }
     uint4 x[N];
+    const char* at;
+    int64_t step;
+    int width;
 
-    __device__ __forceinline__ void load(const T* base, int64_t st, int64_t first, int64_t end, int64_t length, int width) {
+    __device__ __forceinline__ void begin(const void* base, int64_t st, int64_t first_token, bool reverse, int elements) {
+        step = (reverse ? -st : st) * (int64_t)sizeof(T);
+        width = elements;
+        at = (const char*)base + (first_token * st + threadIdx.x % ROW * VW) * (int64_t)sizeof(T) + (int)(threadIdx.x / ROW) * step;
+    }
+    __device__ __forceinline__ uint4 row(int n) const {
+        const T* from = (const T*)(at + n * ROWS * step);
+        if (VEC) return *reinterpret_cast<const uint4*>(from);
+        Pack<T, VW> one;
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const int pack = n * THREADS + threadIdx.x, row = pack / (D / VW), col = pack % (D / VW) * VW;
-            const int64_t p = first + row;
-            x[n] = make_uint4(0, 0, 0, 0);
-            if (p < end && col < width) {
-                const T* from = base + (REVERSE ? length - 1 - p : p) * st + col;
-                if (VEC)
-                    x[n] = *reinterpret_cast<const uint4*>(from);
-                else {
-                    Pack<T, VW> one;
+        for (int e = 0; e < VW; ++e) one.v[e] = (int)(threadIdx.x % ROW * VW) + e < width ? from[e] : (T)0.f;
+        return __builtin_bit_cast(uint4, one);
+    }
+    __device__ __forceinline__ void load(int places) {  // and on to the next chunk
 #pragma unroll
-                    for (int e = 0; e < VW; ++e) one.v[e] = col + e < width ? from[e] : (T)0.f;
-                    x[n] = __builtin_bit_cast(uint4, one);
-                }
+        for (int n = 0; n < N; ++n) x[n] = make_uint4(0, 0, 0, 0);
+        if ((int)(threadIdx.x % ROW * VW) < width && takes_part()) {
+            if (places == CH) {
+#pragma unroll
+                for (int n = 0; n < N; ++n) x[n] = row(n);
+            } else {
+#pragma unroll
+                for (int n = 0; n < N; ++n)
+                    if ((int)(threadIdx.x / ROW) + n * ROWS < places) x[n] = row(n);
             }
         }
+        at += CH * step;
     }
     __device__ __forceinline__ uint32_t store(T* tile, int stride) const {
         uint32_t bad = 0;
+        if (!takes_part()) return bad;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int pack = n * THREADS + threadIdx.x, row = pack / (D / VW), col = pack % (D / VW) * VW;
-            *reinterpret_cast<uint4*>(tile + row * stride + col) = x[n];
+            *reinterpret_cast<uint4*>(tile + (threadIdx.x / ROW + n * ROWS) * stride + threadIdx.x % ROW * VW) = x[n];
             bad |= not_finite<T>(x[n]);
         }
         return bad;
     }
 };
 
+// A column of a state's matrix, by buffer instructions: a load from behind the buffer's end gives 0, a store there does nothing
+struct Column {
+    __amdgpu_buffer_rsrc_t buffer;
+    int at, row, rows;  // bytes
+    __device__ __forceinline__ Column(const float* base, const Scan& s, int64_t row_stride, int64_t col_stride, int column)
+        : buffer(__builtin_amdgcn_make_buffer_rsrc((void*)base, 0, s.da * s.dc * 4, 0x27000)), at(column < s.dc ? column * (int)col_stride * 4 : 0x40000000), row((int)row_stride * 4), rows(s.da) {}
+    __device__ __forceinline__ int offset(int i) const {
+        const int inside = at + i * row;
+        return i < rows ? inside : 0x40000000;
+    }
+    __device__ __forceinline__ float load(int i) const { return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(buffer, offset(i), 0, 0)); }
+    __device__ __forceinline__ void store(int i, float x) const { __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, x), buffer, offset(i), 0, 0); }
+};
+
 // OUT: the walk's outputs; without it the state behind each part alone, from a state of 0 in front of it
 template <class T, int CH, int DA, int DC, bool REVERSE, bool OUT, bool VEC>
-__global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS)) void scan_chunks(Scan s) {
+__global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS), 2) void scan_chunks(Scan s) {
     typedef Shape<T, CH, DA, DC> S;
     typedef Tile<T> M;
     typedef typename M::Frag Frag;
-    constexpr int NT = CH / 16, KA = DA / M::K, KC = CH / M::K, DT = DA / 16, PER = M::K / 16;
+    constexpr int KA = DA / M::K, KC = CH / M::K, DT = DA / 16, PER = M::K / 16;
     __shared__ __align__(16) T tile_a[OUT ? CH * S::SA : 8];
     __shared__ __align__(16) T tile_b[CH * S::SA];
     __shared__ __align__(16) T tile_c[CH * S::SC];
@@ -177,17 +205,16 @@ __global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS)) void scan_chunks(S
     __shared__ uint32_t spoiled[2];
 
     // neighbouring workgroups run on different dies, each with a cache of its own: every die gets a run of neighbouring units
-    const int64_t blocks = gridDim.x, die = blockIdx.x % 8, each = blocks / 8, more = blocks % 8;
-    const int64_t index = die * each + (die < more ? die : more) + blockIdx.x / 8;
-    const int64_t units = s.envs * s.heads, unit = index % units, part = index / units, n = unit / s.heads;
-    const int h = (int)(unit % s.heads);
-    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, l = lane % 16, g = lane / 16, column = wave * S::COLS * 16;
+    const uint32_t units = (uint32_t)(s.envs * s.heads), each = gridDim.x / 8, more = gridDim.x % 8, die = blockIdx.x % 8;
+    const uint32_t index = die * each + (die < more ? die : more) + blockIdx.x / 8;
+    const int64_t unit = index % units, part = index / units, n = (uint32_t)unit / (uint32_t)s.heads;
+    const int h = (int)((uint32_t)unit % (uint32_t)s.heads);
+    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, column = wave * 16, mine = column + lane % 16;
+    Lane at = {lane % 16, lane / 16};
 
     const int64_t length = length_of(s, n), begin = part * s.part_steps;
     const int64_t end = begin + s.part_steps < length ? begin + s.part_steps : length;
-    const T* a = (const T*)s.a.data + n * s.a.sn + h * s.a.sh;
-    const T* b = (const T*)s.b.data + n * s.b.sn + h * s.b.sh;
-    const T* c = (const T*)s.c.data + n * s.c.sn + h * s.c.sh;
+    const int64_t first_token = REVERSE ? length - 1 - begin : begin;
     T* out = OUT ? (T*)s.out.data + n * s.out.sn + h * s.out.sh : nullptr;
     const uint8_t* reset = s.reset ? s.reset + n * s.reset_sn : nullptr;
     // of the chunk from place `first` on: whether nothing in front of place first + lane reaches it
@@ -203,35 +230,42 @@ __global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS)) void scan_chunks(S
     float w_diagonal[4], w_below[4];  // of a score tile on the diagonal, and of the one below it
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-        const int gap = l - 4 * g - r;
+        const int gap = at.l - 4 * at.g - r;
         w_diagonal[r] = gap >= 0 ? decay_of(gap) * s.in_scale : 0.f;
         w_below[r] = decay_of(16 + gap) * s.in_scale;
     }
 
+    Moving<T, CH, DA, S::THREADS, VEC> move_a, move_b;
+    Moving<T, CH, DC, S::THREADS, VEC> move_c;
+    uint32_t flag = 0;
+    if (OUT) move_a.begin((const T*)s.a.data + n * s.a.sn + h * s.a.sh, s.a.st, first_token, REVERSE, s.da);
+    move_b.begin((const T*)s.b.data + n * s.b.sn + h * s.b.sh, s.b.st, first_token, REVERSE, s.da);
+    move_c.begin((const T*)s.c.data + n * s.c.sn + h * s.c.sh, s.c.st, first_token, REVERSE, s.dc);
+    auto load = [&](int64_t first) {
+        const int places = end - first < CH ? (int)(end - first) : CH;
+        if (OUT) move_a.load(places);
+        move_b.load(places);
+        move_c.load(places);
+        flag = load_flag(first);
+    };
+    if (begin < end) load(begin);
+
     const int64_t matrix = (int64_t)s.da * s.dc, which = s.parts == 1 ? unit : unit * s.parts + part;
-    f32x4 state[S::COLS][DT];  // rows 16 t + 4 g + r, column `column` + 16 ct + l
+    f32x4 state[DT];  // rows 16 t + 4 g + r, column `mine`
 #pragma unroll
-    for (int ct = 0; ct < S::COLS; ++ct)
+    for (int t = 0; t < DT; ++t) state[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (s.state_in) {
+        const Column from(s.state_in + which * matrix, s, s.in_row, s.in_col, mine);
 #pragma unroll
         for (int t = 0; t < DT; ++t)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int i = 16 * t + 4 * g + r, j = column + 16 * ct + l;
-                state[ct][t][r] = s.state_in && i < s.da && j < s.dc ? s.state_in[which * matrix + i * s.in_row + j * s.in_col] : 0.f;
-            }
-
-    Moving<T, CH, DA, S::THREADS, VEC, REVERSE> move_a, move_b;
-    Moving<T, CH, DC, S::THREADS, VEC, REVERSE> move_c;
-    uint32_t flag = 0;
-    if (begin < end) {
-        if (OUT) move_a.load(a, s.a.st, begin, end, length, s.da);
-        move_b.load(b, s.b.st, begin, end, length, s.da);
-        move_c.load(c, s.c.st, begin, end, length, s.dc);
-        flag = load_flag(begin);
+            for (int r = 0; r < 4; ++r) state[t][r] = from.load(16 * t + 4 * at.g + r);
     }
+
     int parity = 0;
     uint64_t any_cut = 0;
     for (int64_t first = begin; first < end; first += CH, parity ^= 1) {
+        at.fresh();
         const int places = end - first < CH ? (int)(end - first) : CH;
         uint32_t bad = OUT ? move_a.store(tile_a, S::SA) : 0;
         bad |= move_b.store(tile_b, S::SA);
@@ -242,39 +276,31 @@ __global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS)) void scan_chunks(S
         __syncthreads();
         const bool by_token = spoiled[parity] != 0;
         if (threadIdx.x == 0) spoiled[parity ^ 1] = 0;
-        if (first + CH < end) {
-            if (OUT) move_a.load(a, s.a.st, first + CH, end, length, s.da);
-            move_b.load(b, s.b.st, first + CH, end, length, s.da);
-            move_c.load(c, s.c.st, first + CH, end, length, s.dc);
-            flag = load_flag(first + CH);
-        }
+        if (first + CH < end) load(first + CH);
         const int enters = REVERSE && first == 0 ? 0 : 1;  // decays between what comes into the chunk and its first place
         auto token = [&](int p) { return (REVERSE ? length - 1 - (first + p) : first + p) * s.out.st; };
 
         if (by_token) {
+#pragma unroll 1
             for (int p = 0; p < places; ++p) {
                 const bool cut = cuts >> p & 1;
-                const float carry = power[p == 0 ? enters : 1];
+                const float carry = power[p == 0 ? enters : 1], value = (float)tile_c[p * S::SC + mine] * s.in_scale;
+                const int rows = s.da;
+                at.fresh();
+                float sum = 0.f;
 #pragma unroll
-                for (int ct = 0; ct < S::COLS; ++ct) {
-                    const int j = column + 16 * ct + l;
-                    const float value = (float)tile_c[p * S::SC + j] * s.in_scale;
-                    float sum = 0.f;
+                for (int t = 0; t < DT; ++t)
 #pragma unroll
-                    for (int t = 0; t < DT; ++t)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const int i = 16 * t + 4 * g + r;
-                            if (i < s.da) {
-                                state[ct][t][r] = (cut ? 0.f : state[ct][t][r] * carry) + (float)tile_b[p * S::SA + i] * value;
-                                if (OUT) sum += (float)tile_a[p * S::SA + i] * state[ct][t][r];
-                            }
-                        }
-                    if (OUT) {
-                        sum += __shfl_xor(sum, 16);
-                        sum += __shfl_xor(sum, 32);
-                        if (g == 0 && j < s.dc) out[token(p) + j] = (T)(sum * s.out_scale);
+                    for (int r = 0; r < 4; ++r) {
+                        const int i = 16 * t + 4 * at.g + r;
+                        const float x = (cut ? 0.f : state[t][r] * carry) + (float)tile_b[p * S::SA + i] * value;
+                        state[t][r] = i < rows ? x : 0.f;
+                        if (OUT) sum += i < rows ? (float)tile_a[p * S::SA + i] * x : 0.f;
                     }
+                if (OUT) {
+                    sum += __shfl_xor(sum, 16);
+                    sum += __shfl_xor(sum, 32);
+                    if (at.g == 0 && mine < s.dc) out[token(p) + mine] = (T)(sum * s.out_scale);
                 }
             }
             __syncthreads();
@@ -282,74 +308,62 @@ __global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS)) void scan_chunks(S
         }
 
         const int tiles = (places + 15) / 16;
+        Frag values[KC];  // c, by columns
+#pragma unroll
+        for (int kk = 0; kk < KC; ++kk) values[kk] = M::columns(at, tile_c, S::SC, kk * M::K, column);
         if (OUT) {
             // scores: tile (it, jt) holds rows j = 16 jt + .., columns i = 16 it + ..
             for (int k = wave; k < tiles * (tiles + 1) / 2; k += S::WAVES) {
-                const int it = k >= 6 ? 3 : k >= 3 ? 2 : k >= 1 ? 1 : 0, jt = k - it * (it + 1) / 2, i = 16 * it + l;
+                const int it = k >= 6 ? 3 : k >= 3 ? 2 : k >= 1 ? 1 : 0, jt = k - it * (it + 1) / 2, i = 16 * it + at.l;
                 f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int kk = 0; kk < KA; ++kk) x = M::product(M::rows(tile_b, S::SA, 16 * jt, kk * M::K), M::rows(tile_a, S::SA, 16 * it, kk * M::K), x);
+                for (int kk = 0; kk < KA; ++kk) x = M::product(M::rows(at, tile_b, S::SA, 16 * jt, kk * M::K), M::rows(at, tile_a, S::SA, 16 * it, kk * M::K), x);
                 const uint64_t before = cuts & (~0ull >> (63 - i));
                 const int from = before ? 63 - __builtin_clzll(before) : 0;  // the first place that i sees
                 const float far = it - jt > 1 ? power[16 * (it - jt - 1)] : 1.f;
                 Pack<T, 4> p;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int j = 16 * jt + 4 * g + r;
+                    const int j = 16 * jt + 4 * at.g + r;
                     const float w = it == jt ? w_diagonal[r] : w_below[r] * far;
                     p.v[r] = (T)(j <= i && j >= from ? x[r] * w : 0.f);
                 }
-                *reinterpret_cast<Pack<T, 4>*>(tile_p + i * S::SP + 16 * jt + 4 * g) = p;
+                *reinterpret_cast<Pack<T, 4>*>(tile_p + i * S::SP + 16 * jt + 4 * at.g) = p;
                 if (PER == 2 && it == jt && it % 2 == 0) {  // the tile above the diagonal that shares a fragment with it
 #pragma unroll
                     for (int r = 0; r < 4; ++r) p.v[r] = (T)0.f;
-                    *reinterpret_cast<Pack<T, 4>*>(tile_p + i * S::SP + 16 * jt + 16 + 4 * g) = p;
+                    *reinterpret_cast<Pack<T, 4>*>(tile_p + i * S::SP + 16 * jt + 16 + 4 * at.g) = p;
                 }
             }
             __syncthreads();
-            Frag left[S::COLS][KA];
+            Frag left[KA];
 #pragma unroll
-            for (int ct = 0; ct < S::COLS; ++ct)
+            for (int kk = 0; kk < KA; ++kk) left[kk] = M::of_state(&state[kk * PER]);
+#pragma unroll 1
+            for (int it = 0; it < tiles; ++it) {
+                at.fresh();
+                const int i = 16 * it + at.l;
+                f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int kk = 0; kk < KA; ++kk) left[ct][kk] = M::of_state(&state[ct][kk * PER]);
-#pragma unroll
-            for (int it = 0; it < NT; ++it) {
-                if (it >= tiles) break;
-                const int i = 16 * it + l;
+                for (int kk = 0; kk < KA; ++kk) x = M::product(left[kk], M::rows_as_state(at, tile_a, S::SA, 16 * it, kk * M::K), x);
                 const bool sees = (cuts & (~0ull >> (63 - i))) == 0;
                 const float w = power[i + enters];
-                f32x4 x[S::COLS];
 #pragma unroll
-                for (int ct = 0; ct < S::COLS; ++ct) x[ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int r = 0; r < 4; ++r) x[r] = sees ? x[r] * w : 0.f;
 #pragma unroll
-                for (int kk = 0; kk < KA; ++kk) {
-                    const Frag right = M::rows_as_state(tile_a, S::SA, 16 * it, kk * M::K);
-#pragma unroll
-                    for (int ct = 0; ct < S::COLS; ++ct) x[ct] = M::product(left[ct][kk], right, x[ct]);
-                }
-#pragma unroll
-                for (int ct = 0; ct < S::COLS; ++ct)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) x[ct][r] = sees ? x[ct][r] * w : 0.f;
-#pragma unroll
-                for (int kk = 0; kk <= it / PER; ++kk) {
-                    const Frag right = M::rows(tile_p, S::SP, 16 * it, kk * M::K);
-#pragma unroll
-                    for (int ct = 0; ct < S::COLS; ++ct) x[ct] = M::product(M::columns(tile_c, S::SC, kk * M::K, column + 16 * ct), right, x[ct]);
-                }
+                for (int kk = 0; kk < KC; ++kk)
+                    if (kk * PER <= it) x = M::product(values[kk], M::rows(at, tile_p, S::SP, 16 * it, kk * M::K), x);
                 if (i < places) {
+                    const int j = column + 4 * at.g;
+                    float y[4];
 #pragma unroll
-                    for (int ct = 0; ct < S::COLS; ++ct) {
-                        const int j = column + 16 * ct + 4 * g;
-                        float y[4];
+                    for (int r = 0; r < 4; ++r) y[r] = x[r] * s.out_scale;
+                    if (VEC) {
+                        if (j < s.dc) store_pack<T, 4>(out + token(i) + j, y);
+                    } else {
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) y[r] = x[ct][r] * s.out_scale;
-                        if (VEC) {
-                            if (j < s.dc) store_pack<T, 4>(out + token(i) + j, y);
-                        } else
-#pragma unroll
-                            for (int r = 0; r < 4; ++r)
-                                if (j + r < s.dc) out[token(i) + j + r] = (T)y[r];
+                        for (int r = 0; r < 4; ++r)
+                            if (j + r < s.dc) out[token(i) + j + r] = (T)y[r];
                     }
                 }
             }
@@ -358,30 +372,25 @@ __global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS)) void scan_chunks(S
         const int last_cut = cuts ? 63 - __builtin_clzll(cuts) : 0;
         const float whole = power[places - 1 + enters];
 #pragma unroll
-        for (int ct = 0; ct < S::COLS; ++ct)
+        for (int t = 0; t < DT; ++t)
 #pragma unroll
-            for (int t = 0; t < DT; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) state[ct][t][r] = cuts ? 0.f : state[ct][t][r] * whole;
+            for (int r = 0; r < 4; ++r) state[t][r] = cuts ? 0.f : state[t][r] * whole;
 #pragma unroll
         for (int kk = 0; kk < KC; ++kk) {
             if (kk * M::K >= places) break;
-            Frag right[S::COLS][M::SPLITS];
+            Frag right[M::SPLITS];
             float w[M::K / 4];
 #pragma unroll
             for (int e = 0; e < M::K / 4; ++e) {
-                const int j = kk * M::K + M::place(e);
+                const int j = kk * M::K + M::place(at, e);
                 w[e] = j >= last_cut && j < places ? power[places - 1 - j] * s.in_scale : 0.f;
             }
-#pragma unroll
-            for (int ct = 0; ct < S::COLS; ++ct) M::weighted(M::columns(tile_c, S::SC, kk * M::K, column + 16 * ct), w, right[ct]);
+            M::weighted(values[kk], w, right);
 #pragma unroll
             for (int t = 0; t < DT; ++t) {
-                const Frag left = M::columns(tile_b, S::SA, kk * M::K, 16 * t);
+                const Frag left = M::columns(at, tile_b, S::SA, kk * M::K, 16 * t);
 #pragma unroll
-                for (int ct = 0; ct < S::COLS; ++ct)
-#pragma unroll
-                    for (int i = 0; i < M::SPLITS; ++i) state[ct][t] = M::product(left, right[ct][i], state[ct][t]);
+                for (int i = 0; i < M::SPLITS; ++i) state[t] = M::product(left, right[i], state[t]);
             }
         }
         __syncthreads();
@@ -394,15 +403,11 @@ __global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS)) void scan_chunks(S
     if (s.state_out) {
         const bool leaves = REVERSE && s.parts == 1 && length > 0, cut = leaves && reset && reset[0];
         const float carry = leaves ? power[1] : 1.f;
+        const Column to(s.state_out + which * matrix, s, s.out_row, s.out_col, mine);
 #pragma unroll
-        for (int ct = 0; ct < S::COLS; ++ct)
+        for (int t = 0; t < DT; ++t)
 #pragma unroll
-            for (int t = 0; t < DT; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int i = 16 * t + 4 * g + r, j = column + 16 * ct + l;
-                    if (i < s.da && j < s.dc) s.state_out[which * matrix + i * s.out_row + j * s.out_col] = cut ? 0.f : state[ct][t][r] * carry;
-                }
+            for (int r = 0; r < 4; ++r) to.store(16 * t + 4 * at.g + r, cut ? 0.f : state[t][r] * carry);
     }
 }
 

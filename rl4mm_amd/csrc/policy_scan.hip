@@ -111,7 +111,10 @@ struct Tile<bf16> {  // a fragment: 32 of the summed index, places 8 (lane / 16)
 
 template <class T, int CH, int DA, int DC>
 struct Shape {
-    static constexpr int WAVES = DC / 16, THREADS = 64 * WAVES;  // a wave per 16 of the state's columns
+    static constexpr int COLS = DC == 128 ? 2 : 1;  // tiles of 16 of the state's columns to a wave
+    static constexpr int WAVES = DC / 16 / COLS, THREADS = 64 * WAVES;
+    static constexpr int LEAST_WAVES = DA <= 64 && DC <= 64 ? 4 : 2;  // per SIMD: bounds the registers
+    static constexpr bool AHEAD = DA + DC < 256;  // whether the next chunk is on its way while one is computed
     static constexpr int PAD = Tile<T>::PAD, SA = DA + PAD, SC = DC + PAD, SP = CH + PAD;
 };
 
@@ -150,29 +153,29 @@ struct Moving {
         return __builtin_bit_cast(uint4, one);
     }
     __device__ __forceinline__ void load(int places) {  // and on to the next chunk
+        const bool inside = (int)(threadIdx.x % ROW * VW) < width && takes_part();
+        if (places == CH && inside) {
 #pragma unroll
-        for (int n = 0; n < N; ++n) x[n] = make_uint4(0, 0, 0, 0);
-        if ((int)(threadIdx.x % ROW * VW) < width && takes_part()) {
-            if (places == CH) {
+            for (int n = 0; n < N; ++n) x[n] = row(n);
+        } else {
 #pragma unroll
-                for (int n = 0; n < N; ++n) x[n] = row(n);
-            } else {
-#pragma unroll
-                for (int n = 0; n < N; ++n)
-                    if ((int)(threadIdx.x / ROW) + n * ROWS < places) x[n] = row(n);
+            for (int n = 0; n < N; ++n) {
+                x[n] = make_uint4(0, 0, 0, 0);
+                if (inside && (int)(threadIdx.x / ROW) + n * ROWS < places) x[n] = row(n);
             }
         }
         at += CH * step;
     }
-    __device__ __forceinline__ uint32_t store(T* tile, int stride) const {
-        uint32_t bad = 0;
-        if (!takes_part()) return bad;
+    __device__ __forceinline__ void store(T* tile, int stride) const {
+        if (!takes_part()) return;
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-            *reinterpret_cast<uint4*>(tile + (threadIdx.x / ROW + n * ROWS) * stride + threadIdx.x % ROW * VW) = x[n];
-            bad |= not_finite<T>(x[n]);
-        }
-        return bad;
+        for (int n = 0; n < N; ++n) *reinterpret_cast<uint4*>(tile + (threadIdx.x / ROW + n * ROWS) * stride + threadIdx.x % ROW * VW) = x[n];
+    }
+    __device__ __forceinline__ uint32_t bad() const {
+        uint32_t any = 0;
+#pragma unroll
+        for (int n = 0; n < N; ++n) any |= not_finite<T>(x[n]);
+        return takes_part() ? any : 0;
     }
 };
 
@@ -192,7 +195,7 @@ struct Column {
 
 // OUT: the walk's outputs; without it the state behind each part alone, from a state of 0 in front of it
 template <class T, int CH, int DA, int DC, bool REVERSE, bool OUT, bool VEC>
-__global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS), 2) void scan_chunks(Scan s) {
+__global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS), (Shape<T, CH, DA, DC>::LEAST_WAVES)) void scan_chunks(Scan s) {
     typedef Shape<T, CH, DA, DC> S;
     typedef Tile<T> M;
     typedef typename M::Frag Frag;
@@ -209,7 +212,7 @@ __global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS), 2) void scan_chunk
     const uint32_t index = die * each + (die < more ? die : more) + blockIdx.x / 8;
     const int64_t unit = index % units, part = index / units, n = (uint32_t)unit / (uint32_t)s.heads;
     const int h = (int)((uint32_t)unit % (uint32_t)s.heads);
-    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, column = wave * 16, mine = column + lane % 16;
+    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, column = wave * S::COLS * 16;
     Lane at = {lane % 16, lane / 16};
 
     const int64_t length = length_of(s, n), begin = part * s.part_steps;
@@ -248,18 +251,21 @@ __global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS), 2) void scan_chunk
         move_c.load(places);
         flag = load_flag(first);
     };
-    if (begin < end) load(begin);
+    if (S::AHEAD && begin < end) load(begin);
 
     const int64_t matrix = (int64_t)s.da * s.dc, which = s.parts == 1 ? unit : unit * s.parts + part;
-    f32x4 state[DT];  // rows 16 t + 4 g + r, column `mine`
+    f32x4 state[S::COLS][DT];  // rows 16 t + 4 g + r, column `column` + 16 ct + l
 #pragma unroll
-    for (int t = 0; t < DT; ++t) state[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (s.state_in) {
-        const Column from(s.state_in + which * matrix, s, s.in_row, s.in_col, mine);
+    for (int ct = 0; ct < S::COLS; ++ct) {
 #pragma unroll
-        for (int t = 0; t < DT; ++t)
+        for (int t = 0; t < DT; ++t) state[ct][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (s.state_in) {
+            const Column from(s.state_in + which * matrix, s, s.in_row, s.in_col, column + 16 * ct + at.l);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) state[t][r] = from.load(16 * t + 4 * at.g + r);
+            for (int t = 0; t < DT; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) state[ct][t][r] = from.load(16 * t + 4 * at.g + r);
+        }
     }
 
     int parity = 0;
@@ -267,51 +273,30 @@ __global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS), 2) void scan_chunk
     for (int64_t first = begin; first < end; first += CH, parity ^= 1) {
         at.fresh();
         const int places = end - first < CH ? (int)(end - first) : CH;
-        uint32_t bad = OUT ? move_a.store(tile_a, S::SA) : 0;
-        bad |= move_b.store(tile_b, S::SA);
-        bad |= move_c.store(tile_c, S::SC);
-        if (bad & NOT_FINITE<T>) spoiled[parity] = 1;
+        if (!S::AHEAD) load(first);
+        if (OUT) move_a.store(tile_a, S::SA);
+        move_b.store(tile_b, S::SA);
+        move_c.store(tile_c, S::SC);
         const uint64_t cuts = __ballot(flag != 0);
         any_cut |= cuts;
+        // (without outputs only a cut can take away what is not finite)
+        if (!OUT && cuts && ((move_b.bad() | move_c.bad()) & NOT_FINITE<T>)) spoiled[parity] = 1;
         __syncthreads();
-        const bool by_token = spoiled[parity] != 0;
-        if (threadIdx.x == 0) spoiled[parity ^ 1] = 0;
-        if (first + CH < end) load(first + CH);
+        if (S::AHEAD && first + CH < end) load(first + CH);
         const int enters = REVERSE && first == 0 ? 0 : 1;  // decays between what comes into the chunk and its first place
-        auto token = [&](int p) { return (REVERSE ? length - 1 - (first + p) : first + p) * s.out.st; };
-
-        if (by_token) {
-#pragma unroll 1
-            for (int p = 0; p < places; ++p) {
-                const bool cut = cuts >> p & 1;
-                const float carry = power[p == 0 ? enters : 1], value = (float)tile_c[p * S::SC + mine] * s.in_scale;
-                const int rows = s.da;
-                at.fresh();
-                float sum = 0.f;
-#pragma unroll
-                for (int t = 0; t < DT; ++t)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int i = 16 * t + 4 * at.g + r;
-                        const float x = (cut ? 0.f : state[t][r] * carry) + (float)tile_b[p * S::SA + i] * value;
-                        state[t][r] = i < rows ? x : 0.f;
-                        if (OUT) sum += i < rows ? (float)tile_a[p * S::SA + i] * x : 0.f;
-                    }
-                if (OUT) {
-                    sum += __shfl_xor(sum, 16);
-                    sum += __shfl_xor(sum, 32);
-                    if (at.g == 0 && mine < s.dc) out[token(p) + mine] = (T)(sum * s.out_scale);
-                }
-            }
-            __syncthreads();
-            continue;
-        }
-
         const int tiles = (places + 15) / 16;
-        Frag values[KC];  // c, by columns
+        Frag values[S::COLS][KC];  // c, by columns
 #pragma unroll
-        for (int kk = 0; kk < KC; ++kk) values[kk] = M::columns(at, tile_c, S::SC, kk * M::K, column);
+        for (int ct = 0; ct < S::COLS; ++ct)
+#pragma unroll
+            for (int kk = 0; kk < KC; ++kk) values[ct][kk] = M::columns(at, tile_c, S::SC, kk * M::K, column + 16 * ct);
         if (OUT) {
+            uint32_t bad = 0;
+#pragma unroll
+            for (int ct = 0; ct < S::COLS; ++ct)
+#pragma unroll
+                for (int kk = 0; kk < KC; ++kk) bad |= not_finite<T>(__builtin_bit_cast(uint4, values[ct][kk]));
+            bool spoils = bad & NOT_FINITE<T>;
             // scores: tile (it, jt) holds rows j = 16 jt + .., columns i = 16 it + ..
             for (int k = wave; k < tiles * (tiles + 1) / 2; k += S::WAVES) {
                 const int it = k >= 6 ? 3 : k >= 3 ? 2 : k >= 1 ? 1 : 0, jt = k - it * (it + 1) / 2, i = 16 * it + at.l;
@@ -327,6 +312,7 @@ __global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS), 2) void scan_chunk
                     const int j = 16 * jt + 4 * at.g + r;
                     const float w = it == jt ? w_diagonal[r] : w_below[r] * far;
                     p.v[r] = (T)(j <= i && j >= from ? x[r] * w : 0.f);
+                    spoils |= !(fabsf(x[r]) < INFINITY);  // (the tiles on the diagonal see every row of a and b)
                 }
                 *reinterpret_cast<Pack<T, 4>*>(tile_p + i * S::SP + 16 * jt + 4 * at.g) = p;
                 if (PER == 2 && it == jt && it % 2 == 0) {  // the tile above the diagonal that shares a fragment with it
@@ -335,35 +321,92 @@ __global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS), 2) void scan_chunk
                     *reinterpret_cast<Pack<T, 4>*>(tile_p + i * S::SP + 16 * jt + 16 + 4 * at.g) = p;
                 }
             }
+            if (spoils) spoiled[parity] = 1;
             __syncthreads();
-            Frag left[KA];
-#pragma unroll
-            for (int kk = 0; kk < KA; ++kk) left[kk] = M::of_state(&state[kk * PER]);
+        }
+        const bool by_token = spoiled[parity] != 0;
+        if (threadIdx.x == 0) spoiled[parity ^ 1] = 0;
+        auto token = [&](int p) { return (REVERSE ? length - 1 - (first + p) : first + p) * s.out.st; };
+
+        if (by_token) {
 #pragma unroll 1
-            for (int it = 0; it < tiles; ++it) {
+            for (int p = 0; p < places; ++p) {
+                const bool cut = cuts >> p & 1;
+                const float carry = power[p == 0 ? enters : 1];
+                at.fresh();
+#pragma unroll
+                for (int ct = 0; ct < S::COLS; ++ct) {
+                    const int j = column + 16 * ct + at.l;
+                    const float value = (float)tile_c[p * S::SC + j] * s.in_scale;
+                    float sum = 0.f;
+#pragma unroll
+                    for (int t = 0; t < DT; ++t)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const int i = 16 * t + 4 * at.g + r;
+                            const float x = (cut ? 0.f : state[ct][t][r] * carry) + (float)tile_b[p * S::SA + i] * value;
+                            state[ct][t][r] = i < s.da ? x : 0.f;
+                            if (OUT) sum += i < s.da ? (float)tile_a[p * S::SA + i] * x : 0.f;
+                        }
+                    if (OUT) {
+                        sum += __shfl_xor(sum, 16);
+                        sum += __shfl_xor(sum, 32);
+                        if (at.g == 0 && j < s.dc) out[token(p) + j] = (T)(sum * s.out_scale);
+                    }
+                }
+            }
+            __syncthreads();
+            continue;
+        }
+
+        if (OUT) {
+            Frag left[S::COLS][KA];
+#pragma unroll
+            for (int ct = 0; ct < S::COLS; ++ct)
+#pragma unroll
+                for (int kk = 0; kk < KA; ++kk) left[ct][kk] = M::of_state(&state[ct][kk * PER]);
+            T* to = out + token(at.l) + column + 4 * at.g;
+            const int64_t on = (REVERSE ? -16 : 16) * s.out.st;
+#pragma unroll 1
+            for (int it = 0; it < tiles; ++it, to += on) {
                 at.fresh();
                 const int i = 16 * it + at.l;
-                f32x4 x = {0.f, 0.f, 0.f, 0.f};
+                f32x4 x[S::COLS];
 #pragma unroll
-                for (int kk = 0; kk < KA; ++kk) x = M::product(left[kk], M::rows_as_state(at, tile_a, S::SA, 16 * it, kk * M::K), x);
+                for (int ct = 0; ct < S::COLS; ++ct) x[ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int kk = 0; kk < KA; ++kk) {
+                    const Frag right = M::rows_as_state(at, tile_a, S::SA, 16 * it, kk * M::K);
+#pragma unroll
+                    for (int ct = 0; ct < S::COLS; ++ct) x[ct] = M::product(left[ct][kk], right, x[ct]);
+                }
                 const bool sees = (cuts & (~0ull >> (63 - i))) == 0;
                 const float w = power[i + enters];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) x[r] = sees ? x[r] * w : 0.f;
+                for (int ct = 0; ct < S::COLS; ++ct)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) x[ct][r] = sees ? x[ct][r] * w : 0.f;
 #pragma unroll
                 for (int kk = 0; kk < KC; ++kk)
-                    if (kk * PER <= it) x = M::product(values[kk], M::rows(at, tile_p, S::SP, 16 * it, kk * M::K), x);
+                    if (kk * PER <= it) {
+                        const Frag right = M::rows(at, tile_p, S::SP, 16 * it, kk * M::K);
+#pragma unroll
+                        for (int ct = 0; ct < S::COLS; ++ct) x[ct] = M::product(values[ct][kk], right, x[ct]);
+                    }
                 if (i < places) {
-                    const int j = column + 4 * at.g;
-                    float y[4];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) y[r] = x[r] * s.out_scale;
-                    if (VEC) {
-                        if (j < s.dc) store_pack<T, 4>(out + token(i) + j, y);
-                    } else {
+                    for (int ct = 0; ct < S::COLS; ++ct) {
+                        const int j = column + 16 * ct + 4 * at.g;
+                        float y[4];
 #pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (j + r < s.dc) out[token(i) + j + r] = (T)y[r];
+                        for (int r = 0; r < 4; ++r) y[r] = x[ct][r] * s.out_scale;
+                        if (VEC) {
+                            if (j < s.dc) store_pack<T, 4>(to + 16 * ct, y);
+                        } else {
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                if (j + r < s.dc) to[16 * ct + r] = (T)y[r];
+                        }
                     }
                 }
             }
@@ -371,26 +414,36 @@ __global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS), 2) void scan_chunk
         // the state: what comes in decays by the whole chunk, place j by what lies behind it
         const int last_cut = cuts ? 63 - __builtin_clzll(cuts) : 0;
         const float whole = power[places - 1 + enters];
+        if (cuts) {
 #pragma unroll
-        for (int t = 0; t < DT; ++t)
+            for (int ct = 0; ct < S::COLS; ++ct)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) state[t][r] = cuts ? 0.f : state[t][r] * whole;
+                for (int t = 0; t < DT; ++t) state[ct][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        } else {
+#pragma unroll
+            for (int ct = 0; ct < S::COLS; ++ct)
+#pragma unroll
+                for (int t = 0; t < DT; ++t) state[ct][t] *= whole;
+        }
 #pragma unroll
         for (int kk = 0; kk < KC; ++kk) {
             if (kk * M::K >= places) break;
-            Frag right[M::SPLITS];
+            Frag right[S::COLS][M::SPLITS];
             float w[M::K / 4];
 #pragma unroll
             for (int e = 0; e < M::K / 4; ++e) {
                 const int j = kk * M::K + M::place(at, e);
                 w[e] = j >= last_cut && j < places ? power[places - 1 - j] * s.in_scale : 0.f;
             }
-            M::weighted(values[kk], w, right);
+#pragma unroll
+            for (int ct = 0; ct < S::COLS; ++ct) M::weighted(values[ct][kk], w, right[ct]);
 #pragma unroll
             for (int t = 0; t < DT; ++t) {
                 const Frag left = M::columns(at, tile_b, S::SA, kk * M::K, 16 * t);
 #pragma unroll
-                for (int i = 0; i < M::SPLITS; ++i) state[t] = M::product(left, right[i], state[t]);
+                for (int ct = 0; ct < S::COLS; ++ct)
+#pragma unroll
+                    for (int i = 0; i < M::SPLITS; ++i) state[ct][t] = M::product(left, right[ct][i], state[ct][t]);
             }
         }
         __syncthreads();
@@ -403,11 +456,14 @@ __global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS), 2) void scan_chunk
     if (s.state_out) {
         const bool leaves = REVERSE && s.parts == 1 && length > 0, cut = leaves && reset && reset[0];
         const float carry = leaves ? power[1] : 1.f;
-        const Column to(s.state_out + which * matrix, s, s.out_row, s.out_col, mine);
 #pragma unroll
-        for (int t = 0; t < DT; ++t)
+        for (int ct = 0; ct < S::COLS; ++ct) {
+            const Column to(s.state_out + which * matrix, s, s.out_row, s.out_col, column + 16 * ct + at.l);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) to.store(16 * t + 4 * at.g + r, cut ? 0.f : state[t][r] * carry);
+            for (int t = 0; t < DT; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) to.store(16 * t + 4 * at.g + r, cut ? 0.f : state[ct][t][r] * carry);
+        }
     }
 }
 

@@ -89,7 +89,7 @@ struct Scan {
     float in_scale, out_scale;
     int64_t part_steps;  // the steps are split into `parts` of this many, each a workgroup's; state_in and state_out are then [unit][part]
     int parts;
-    uint8_t* cut_out;  // [unit][part]: whether a reset lies in the part (where out.data is NULL: the walk for the states alone)
+    float* carry_out;  // [unit][part]: what comes into the part times this goes out of it, negative: a reset lies in it (the walk without outputs)
 };
 
 __device__ __forceinline__ int64_t length_of(const Scan& s, int64_t n) {

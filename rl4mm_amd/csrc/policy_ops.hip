@@ -31,35 +31,49 @@ struct Parts {
     int64_t steps;
     int count;
     Parts(const lobpolicy_attention* a) {
-        const int64_t units = a->envs * a->heads;
-        int64_t n = a->steps < 512 || units >= 512 ? 1 : ceil_div(1024, units);
-        n = n < ceil_div(a->steps, 256) ? n : ceil_div(a->steps, 256);
+        const int64_t units = a->envs * a->heads, wanted = a->dk > 64 || a->dv > 64 ? 512 : 1024;
+        int64_t n = a->steps < 512 || units >= 512 ? 1 : ceil_div(wanted, units);
+        n = n < ceil_div(a->steps, 128) ? n : ceil_div(a->steps, 128);
         steps = ceil_div(ceil_div(a->steps, n), 64) * 64;
         count = (int)ceil_div(a->steps, steps);
     }
     int64_t matrices(const lobpolicy_attention* a) const { return a->envs * a->heads * count; }
-    int64_t bytes(const lobpolicy_attention* a) const { return count == 1 ? 0 : matrices(a) * (a->dk * a->dv * (int64_t)sizeof(float) + 1); }
+    int64_t bytes(const lobpolicy_attention* a) const { return count == 1 ? 0 : matrices(a) * (a->dk * a->dv + 1) * (int64_t)sizeof(float); }
 };
 
 // grid (elements / 256, units): `states` [unit][part] from what each part adds to what is in front of it; the state behind the last to state_out
 template <bool REVERSE>
-__global__ __launch_bounds__(256) void join_parts(Scan s, float* states, const uint8_t* cut) {
+__global__ __launch_bounds__(256) void join_parts(Scan s, float* states, const float* __restrict__ carries) {
     const int64_t unit = blockIdx.y, matrix = (int64_t)s.da * s.dc, e = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (e >= matrix) return;
-    const int64_t n = unit / s.heads, length = length_of(s, n), row = e / s.dc, col = e % s.dc;
-    const float log_decay = s.log_decay[unit % s.heads];
+    const int64_t row = e / s.dc, col = e % s.dc;
     float state = s.state_in ? s.state_in[unit * matrix + row * s.in_row + col * s.in_col] : 0.f;
-    float* at = states + unit * s.parts * matrix + e;
-#pragma unroll 4
-    for (int part = 0; part < s.parts; ++part) {
-        const int64_t left = length - part * s.part_steps, places = left < 0 ? 0 : left < s.part_steps ? left : s.part_steps;
-        const int64_t decays = places - (REVERSE && part == 0 && places ? 1 : 0);  // (backwards nothing decays in front of the first place)
-        const float added = at[part * matrix];
-        at[part * matrix] = state;
-        state = (cut[unit * s.parts + part] ? 0.f : decays ? state * expf(log_decay * (float)decays) : state) + added;
+    const float* carry = carries + unit * s.parts;
+    // buffer instructions: what lies behind the last part reads as 0 and is not written, without a branch that would wait for the loads in flight.
+    // AT_ONCE parts at a time, the next ones on their way before these are stored (a wait for a load waits for the stores in front of it too)
+    constexpr int AT_ONCE = 8;
+    const __amdgpu_buffer_rsrc_t buffer = __builtin_amdgcn_make_buffer_rsrc(states + unit * s.parts * matrix, 0, (int)(s.parts * matrix * 4), 0x27000);
+    const int at = (int)e * 4, step = (int)matrix * 4;
+    float added[AT_ONCE], next[AT_ONCE];
+#pragma unroll
+    for (int k = 0; k < AT_ONCE; ++k) next[k] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(buffer, at + k * step, 0, 0));
+    for (int first = 0; first < s.parts; first += AT_ONCE) {
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k) {
+            added[k] = next[k];
+            next[k] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(buffer, at + (first + AT_ONCE + k) * step, 0, 0));
+        }
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k) {
+            const int part = first + k;
+            const float c = part < s.parts ? carry[part] : 1.f;
+            __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, state), buffer, at + part * step, 0, 0);
+            state = (c < 0.f ? 0.f : state * c) + added[k];
+        }
     }
     if (s.state_out) {
-        if (REVERSE && length > 0) state = s.reset && s.reset[n * s.reset_sn] ? 0.f : state * expf(log_decay);
+        const int64_t n = unit / s.heads;
+        if (REVERSE && length_of(s, n) > 0) state = s.reset && s.reset[n * s.reset_sn] ? 0.f : state * expf(s.log_decay[unit % s.heads]);
         s.state_out[unit * matrix + row * s.out_row + col * s.out_col] = state;
     }
 }
@@ -72,16 +86,16 @@ int walk(const lobpolicy_attention* a, const Scan& s, bool reverse, hipStream_t 
 int part_states(const lobpolicy_attention* a, Scan s, bool reverse, hipStream_t stream) {
     const Parts parts(a);
     float* states = (float*)a->workspace;
-    uint8_t* cut = (uint8_t*)(states + parts.matrices(a) * a->dk * a->dv);
+    float* carries = states + parts.matrices(a) * a->dk * a->dv;
     Scan first = s;
     first.a = first.b, first.out = {};
-    first.state_in = nullptr, first.state_out = states, first.out_row = s.dc, first.out_col = 1, first.cut_out = cut;
+    first.state_in = nullptr, first.state_out = states, first.out_row = s.dc, first.out_col = 1, first.carry_out = carries;
     if (int e = walk(a, first, reverse, stream)) return e;
     const dim3 grid((unsigned)ceil_div((int64_t)s.da * s.dc, 256), (unsigned)(a->envs * a->heads));
     if (reverse)
-        join_parts<true><<<grid, 256, 0, stream>>>(s, states, cut);
+        join_parts<true><<<grid, 256, 0, stream>>>(s, states, carries);
     else
-        join_parts<false><<<grid, 256, 0, stream>>>(s, states, cut);
+        join_parts<false><<<grid, 256, 0, stream>>>(s, states, carries);
     return launched();
 }
 

@@ -452,7 +452,7 @@ __global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS), (Shape<T, CH, DA, 
     if (OUT && part == s.parts - 1)  // rows behind the last token
         for (int64_t t = length + threadIdx.x / 32; t < s.steps; t += S::THREADS / 32)
             for (int j = threadIdx.x % 32; j < s.dc; j += 32) out[t * s.out.st + j] = (T)0.f;
-    if (!OUT && threadIdx.x == 0) s.cut_out[which] = any_cut != 0;
+    if (!OUT && threadIdx.x == 0) s.carry_out[which] = any_cut ? -1.f : decay_of(begin < end ? (int)(end - begin) - (REVERSE && begin == 0 ? 1 : 0) : 0);
     if (s.state_out) {
         const bool leaves = REVERSE && s.parts == 1 && length > 0, cut = leaves && reset && reset[0];
         const float carry = leaves ? power[1] : 1.f;
@@ -493,9 +493,10 @@ int scan_aligned(const Scan& s, bool reverse, hipStream_t stream) {
 
 template <class T, int DA>
 int scan_rows(const Scan& s, bool reverse, hipStream_t stream) {
-    if (s.dc <= 32) return scan_aligned<T, 64, DA, 32>(s, reverse, stream);
-    if (s.dc <= 64) return scan_aligned<T, 64, DA, 64>(s, reverse, stream);
-    return scan_aligned<T, 64, DA, 128>(s, reverse, stream);
+    constexpr int CH = sizeof(T) == 4 ? 32 : 64;
+    if (s.dc <= 32) return scan_aligned<T, CH, DA, 32>(s, reverse, stream);
+    if (s.dc <= 64) return scan_aligned<T, CH, DA, 64>(s, reverse, stream);
+    return scan_aligned<T, CH, DA, 128>(s, reverse, stream);
 }
 
 template int scan_rows<LOBPOLICY_TYPE, LOBPOLICY_ROWS>(const Scan&, bool, hipStream_t);

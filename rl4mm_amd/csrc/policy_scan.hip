@@ -29,6 +29,7 @@ namespace lobpolicy {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 // a lane's place in a 16 x 16 tile.  `fresh` makes it a value that the compiler knows nothing of: what is worked out from it inside the walk
@@ -101,10 +102,16 @@ struct Tile<bf16> {  // a fragment: 32 of the summed index, places 8 (lane / 16)
     static constexpr int SPLITS = 3;
     static __device__ __forceinline__ void weighted(Frag c, const float* w, Frag* f) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            float x = (float)c[e] * w[e];
+        for (int e = 0; e < 8; e += 2) {
+            uint32_t x = __builtin_bit_cast(uint32_t, (float)c[e] * w[e]), y = __builtin_bit_cast(uint32_t, (float)c[e + 1] * w[e + 1]);
 #pragma unroll
-            for (int i = 0; i < 3; ++i) f[i][e] = (bf16)x, x -= (float)f[i][e];
+            for (int i = 0; i < 3; ++i) {  // the upper 8 bits of what is left, exactly (cut off, not rounded), two at a time
+                const uint32_t both = __builtin_amdgcn_perm(y, x, 0x07060302);
+                const bf16x2 two = __builtin_bit_cast(bf16x2, both);
+                f[i][e] = two[0], f[i][e + 1] = two[1];
+                x = __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, x) - __builtin_bit_cast(float, x & 0xffff0000u));
+                y = __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, y) - __builtin_bit_cast(float, y & 0xffff0000u));
+            }
         }
     }
 };
@@ -204,7 +211,8 @@ __global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS), (Shape<T, CH, DA, 
     __shared__ __align__(16) T tile_b[CH * S::SA];
     __shared__ __align__(16) T tile_c[CH * S::SC];
     __shared__ __align__(16) T tile_p[OUT ? CH * S::SP : 8];
-    __shared__ float power[CH + 1];
+    __shared__ float power[CH + 1], enter[CH + 1];     // l^k, and times out_scale
+    __shared__ __align__(16) float leave[CH];          // l^(CH - 1 - j) in_scale
     __shared__ uint32_t spoiled[2];
 
     // neighbouring workgroups run on different dies, each with a cache of its own: every die gets a run of neighbouring units
@@ -228,14 +236,19 @@ __global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS), (Shape<T, CH, DA, 
 
     const float log_decay = s.log_decay[h];
     auto decay_of = [&](int k) { return k == 0 ? 1.f : expf(log_decay * (float)k); };  // (k = 0: not 0 * infinity)
-    for (int k = threadIdx.x; k <= CH; k += S::THREADS) power[k] = decay_of(k);
+    for (int k = threadIdx.x; k <= CH; k += S::THREADS) {
+        const float x = decay_of(k);
+        power[k] = x;
+        enter[k] = x * s.out_scale;
+        if (k < CH) leave[CH - 1 - k] = x * s.in_scale;
+    }
     if (threadIdx.x < 2) spoiled[threadIdx.x] = 0;
     float w_diagonal[4], w_below[4];  // of a score tile on the diagonal, and of the one below it
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         const int gap = at.l - 4 * at.g - r;
-        w_diagonal[r] = gap >= 0 ? decay_of(gap) * s.in_scale : 0.f;
-        w_below[r] = decay_of(16 + gap) * s.in_scale;
+        w_diagonal[r] = gap >= 0 ? decay_of(gap) * s.in_scale * s.out_scale : 0.f;
+        w_below[r] = decay_of(16 + gap) * s.in_scale * s.out_scale;
     }
 
     Moving<T, CH, DA, S::THREADS, VEC> move_a, move_b;
@@ -291,29 +304,28 @@ __global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS), (Shape<T, CH, DA, 
 #pragma unroll
             for (int kk = 0; kk < KC; ++kk) values[ct][kk] = M::columns(at, tile_c, S::SC, kk * M::K, column + 16 * ct);
         if (OUT) {
-            uint32_t bad = 0;
-#pragma unroll
-            for (int ct = 0; ct < S::COLS; ++ct)
-#pragma unroll
-                for (int kk = 0; kk < KC; ++kk) bad |= not_finite<T>(__builtin_bit_cast(uint4, values[ct][kk]));
-            bool spoils = bad & NOT_FINITE<T>;
+            float spoils = 0.f;  // becomes NaN with the first number that is none, or infinite
             // scores: tile (it, jt) holds rows j = 16 jt + .., columns i = 16 it + ..
             for (int k = wave; k < tiles * (tiles + 1) / 2; k += S::WAVES) {
                 const int it = k >= 6 ? 3 : k >= 3 ? 2 : k >= 1 ? 1 : 0, jt = k - it * (it + 1) / 2, i = 16 * it + at.l;
                 f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int kk = 0; kk < KA; ++kk) x = M::product(M::rows(at, tile_b, S::SA, 16 * jt, kk * M::K), M::rows(at, tile_a, S::SA, 16 * it, kk * M::K), x);
-                const uint64_t before = cuts & (~0ull >> (63 - i));
-                const int from = before ? 63 - __builtin_clzll(before) : 0;  // the first place that i sees
                 const float far = it - jt > 1 ? power[16 * (it - jt - 1)] : 1.f;
-                Pack<T, 4> p;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int j = 16 * jt + 4 * at.g + r;
-                    const float w = it == jt ? w_diagonal[r] : w_below[r] * far;
-                    p.v[r] = (T)(j <= i && j >= from ? x[r] * w : 0.f);
-                    spoils |= !(fabsf(x[r]) < INFINITY);  // (the tiles on the diagonal see every row of a and b)
+                    spoils = fmaf(x[r], 0.f, spoils);  // (the tiles on the diagonal see every row of a and b)
+                    x[r] *= it == jt ? w_diagonal[r] : w_below[r] * far;
                 }
+                if (cuts) {
+                    const uint64_t before = cuts & (~0ull >> (63 - i));
+                    const int from = before ? 63 - __builtin_clzll(before) : 0;  // the first place that i sees
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) x[r] = 16 * jt + 4 * at.g + r >= from ? x[r] : 0.f;
+                }
+                Pack<T, 4> p;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) p.v[r] = (T)x[r];
                 *reinterpret_cast<Pack<T, 4>*>(tile_p + i * S::SP + 16 * jt + 4 * at.g) = p;
                 if (PER == 2 && it == jt && it % 2 == 0) {  // the tile above the diagonal that shares a fragment with it
 #pragma unroll
@@ -321,13 +333,79 @@ __global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS), (Shape<T, CH, DA, 
                     *reinterpret_cast<Pack<T, 4>*>(tile_p + i * S::SP + 16 * jt + 16 + 4 * at.g) = p;
                 }
             }
-            if (spoils) spoiled[parity] = 1;
+            if (spoils != 0.f) spoiled[parity] = 1;
             __syncthreads();
         }
-        const bool by_token = spoiled[parity] != 0;
+        bool by_token = spoiled[parity] != 0;
         if (threadIdx.x == 0) spoiled[parity ^ 1] = 0;
         auto token = [&](int p) { return (REVERSE ? length - 1 - (first + p) : first + p) * s.out.st; };
 
+        if (OUT && !by_token) {
+            Frag left[S::COLS][KA];
+#pragma unroll
+            for (int ct = 0; ct < S::COLS; ++ct)
+#pragma unroll
+                for (int kk = 0; kk < KA; ++kk) left[ct][kk] = M::of_state(&state[ct][kk * PER]);
+            T* to = out + token(at.l) + column + 4 * at.g;
+            const int64_t on = (REVERSE ? -16 : 16) * s.out.st;
+            float spoils = 0.f;
+#pragma unroll 1
+            for (int it = 0; it < tiles; ++it, to += on) {
+                at.fresh();
+                const int i = 16 * it + at.l;
+                f32x4 x[S::COLS];
+#pragma unroll
+                for (int ct = 0; ct < S::COLS; ++ct) x[ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int kk = 0; kk < KA; ++kk) {
+                    const Frag right = M::rows_as_state(at, tile_a, S::SA, 16 * it, kk * M::K);
+#pragma unroll
+                    for (int ct = 0; ct < S::COLS; ++ct) x[ct] = M::product(left[ct][kk], right, x[ct]);
+                }
+                const float w = enter[i + enters];
+#pragma unroll
+                for (int ct = 0; ct < S::COLS; ++ct) x[ct] *= w;
+                if (cuts) {
+                    const bool sees = (cuts & (~0ull >> (63 - i))) == 0;
+#pragma unroll
+                    for (int ct = 0; ct < S::COLS; ++ct)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) x[ct][r] = sees ? x[ct][r] : 0.f;
+                }
+#pragma unroll
+                for (int kk = 0; kk < KC; ++kk)
+                    if (kk * PER <= it) {
+                        const Frag right = M::rows(at, tile_p, S::SP, 16 * it, kk * M::K);
+#pragma unroll
+                        for (int ct = 0; ct < S::COLS; ++ct) x[ct] = M::product(values[ct][kk], right, x[ct]);
+                    }
+                if (it == tiles - 1) {
+#pragma unroll
+                    for (int ct = 0; ct < S::COLS; ++ct)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) spoils = fmaf(x[ct][r], 0.f, spoils);
+                }
+                if (i < places) {
+#pragma unroll
+                    for (int ct = 0; ct < S::COLS; ++ct) {
+                        const int j = column + 16 * ct + 4 * at.g;
+                        Pack<T, 4> y;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) y.v[r] = (T)x[ct][r];
+                        if (VEC) {
+                            if (j < s.dc) *reinterpret_cast<Pack<T, 4>*>(to + 16 * ct) = y;
+                        } else {
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                if (j + r < s.dc) to[16 * ct + r] = y.v[r];
+                        }
+                    }
+                }
+            }
+            // the last tile's products see every c: one that is not finite in this wave's columns (or the state) shows in them, and the wave, whose
+            // columns are its own, begins again token by token
+            by_token = __ballot(spoils != 0.f) != 0;
+        }
         if (by_token) {
 #pragma unroll 1
             for (int p = 0; p < places; ++p) {
@@ -355,95 +433,45 @@ __global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS), (Shape<T, CH, DA, 
                     }
                 }
             }
-            __syncthreads();
-            continue;
-        }
-
-        if (OUT) {
-            Frag left[S::COLS][KA];
-#pragma unroll
-            for (int ct = 0; ct < S::COLS; ++ct)
-#pragma unroll
-                for (int kk = 0; kk < KA; ++kk) left[ct][kk] = M::of_state(&state[ct][kk * PER]);
-            T* to = out + token(at.l) + column + 4 * at.g;
-            const int64_t on = (REVERSE ? -16 : 16) * s.out.st;
-#pragma unroll 1
-            for (int it = 0; it < tiles; ++it, to += on) {
-                at.fresh();
-                const int i = 16 * it + at.l;
-                f32x4 x[S::COLS];
-#pragma unroll
-                for (int ct = 0; ct < S::COLS; ++ct) x[ct] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int kk = 0; kk < KA; ++kk) {
-                    const Frag right = M::rows_as_state(at, tile_a, S::SA, 16 * it, kk * M::K);
-#pragma unroll
-                    for (int ct = 0; ct < S::COLS; ++ct) x[ct] = M::product(left[ct][kk], right, x[ct]);
-                }
-                const bool sees = (cuts & (~0ull >> (63 - i))) == 0;
-                const float w = power[i + enters];
-#pragma unroll
-                for (int ct = 0; ct < S::COLS; ++ct)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) x[ct][r] = sees ? x[ct][r] * w : 0.f;
-#pragma unroll
-                for (int kk = 0; kk < KC; ++kk)
-                    if (kk * PER <= it) {
-                        const Frag right = M::rows(at, tile_p, S::SP, 16 * it, kk * M::K);
-#pragma unroll
-                        for (int ct = 0; ct < S::COLS; ++ct) x[ct] = M::product(values[ct][kk], right, x[ct]);
-                    }
-                if (i < places) {
-#pragma unroll
-                    for (int ct = 0; ct < S::COLS; ++ct) {
-                        const int j = column + 16 * ct + 4 * at.g;
-                        float y[4];
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) y[r] = x[ct][r] * s.out_scale;
-                        if (VEC) {
-                            if (j < s.dc) store_pack<T, 4>(to + 16 * ct, y);
-                        } else {
-#pragma unroll
-                            for (int r = 0; r < 4; ++r)
-                                if (j + r < s.dc) to[16 * ct + r] = (T)y[r];
-                        }
-                    }
-                }
-            }
-        }
-        // the state: what comes in decays by the whole chunk, place j by what lies behind it
-        const int last_cut = cuts ? 63 - __builtin_clzll(cuts) : 0;
-        const float whole = power[places - 1 + enters];
-        if (cuts) {
-#pragma unroll
-            for (int ct = 0; ct < S::COLS; ++ct)
-#pragma unroll
-                for (int t = 0; t < DT; ++t) state[ct][t] = f32x4{0.f, 0.f, 0.f, 0.f};
         } else {
-#pragma unroll
-            for (int ct = 0; ct < S::COLS; ++ct)
-#pragma unroll
-                for (int t = 0; t < DT; ++t) state[ct][t] *= whole;
-        }
-#pragma unroll
-        for (int kk = 0; kk < KC; ++kk) {
-            if (kk * M::K >= places) break;
-            Frag right[S::COLS][M::SPLITS];
-            float w[M::K / 4];
-#pragma unroll
-            for (int e = 0; e < M::K / 4; ++e) {
-                const int j = kk * M::K + M::place(at, e);
-                w[e] = j >= last_cut && j < places ? power[places - 1 - j] * s.in_scale : 0.f;
-            }
-#pragma unroll
-            for (int ct = 0; ct < S::COLS; ++ct) M::weighted(values[ct][kk], w, right[ct]);
-#pragma unroll
-            for (int t = 0; t < DT; ++t) {
-                const Frag left = M::columns(at, tile_b, S::SA, kk * M::K, 16 * t);
+            // the state: what comes in decays by the whole chunk, place j by what lies behind it
+            const int last_cut = cuts ? 63 - __builtin_clzll(cuts) : 0;
+            const float whole = power[places - 1 + enters];
+            if (cuts) {
 #pragma unroll
                 for (int ct = 0; ct < S::COLS; ++ct)
 #pragma unroll
-                    for (int i = 0; i < M::SPLITS; ++i) state[ct][t] = M::product(left, right[ct][i], state[ct][t]);
+                    for (int t = 0; t < DT; ++t) state[ct][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+            } else {
+#pragma unroll
+                for (int ct = 0; ct < S::COLS; ++ct)
+#pragma unroll
+                    for (int t = 0; t < DT; ++t) state[ct][t] *= whole;
+            }
+#pragma unroll
+            for (int kk = 0; kk < KC; ++kk) {
+                if (kk * M::K >= places) break;
+                Frag right[S::COLS][M::SPLITS];
+                float w[M::K / 4];
+                if (places == CH && !cuts)
+                    load_pack<float, M::K / 4>(leave + kk * M::K + M::place(at, 0), w);
+                else {
+#pragma unroll
+                    for (int e = 0; e < M::K / 4; ++e) {
+                        const int j = kk * M::K + M::place(at, e);
+                        w[e] = j >= last_cut && j < places ? power[places - 1 - j] * s.in_scale : 0.f;
+                    }
+                }
+#pragma unroll
+                for (int ct = 0; ct < S::COLS; ++ct) M::weighted(values[ct][kk], w, right[ct]);
+#pragma unroll
+                for (int t = 0; t < DT; ++t) {
+                    const Frag left = M::columns(at, tile_b, S::SA, kk * M::K, 16 * t);
+#pragma unroll
+                    for (int ct = 0; ct < S::COLS; ++ct)
+#pragma unroll
+                        for (int i = 0; i < M::SPLITS; ++i) state[ct][t] = M::product(left, right[ct][i], state[ct][t]);
+                }
             }
         }
         __syncthreads();

@@ -120,7 +120,7 @@ template <class T, int CH, int DA, int DC>
 struct Shape {
     static constexpr int COLS = DC == 128 ? 2 : 1;  // tiles of 16 of the state's columns to a wave
     static constexpr int WAVES = DC / 16 / COLS, THREADS = 64 * WAVES;
-    static constexpr int LEAST_WAVES = DA <= 64 && DC <= 64 ? 4 : 2;  // per SIMD: bounds the registers
+    static constexpr int LEAST_WAVES = DA <= 64 && DC <= 64 ? 3 : 2;  // per SIMD: bounds the registers
     static constexpr bool AHEAD = DA + DC < 256;  // whether the next chunk is on its way while one is computed
     static constexpr int PAD = Tile<T>::PAD, SA = DA + PAD, SC = DC + PAD, SP = CH + PAD;
 };
@@ -135,50 +135,53 @@ template <class T>
 constexpr uint32_t NOT_FINITE = sizeof(T) == 2 ? 0x80008000u : 0x80000000u;
 
 // A tile's share of a thread, on its way: CH places in the order of the walk, 16 bytes at a time.  `at` is the thread's first row in the chunk to be
-// loaded next, `step` the bytes from place to place (negative where the walk goes backwards).
+// loaded next, `step` the bytes from place to place (negative where the walk goes backwards).  Rows behind the last place are loaded from the
+// chunk's first row instead and become 0 when they are stored: a branch around a load would make the next wait one for every load.
 template <class T, int CH, int D, int THREADS, bool VEC>
 struct Moving {
     static constexpr int VW = 16 / (int)sizeof(T), ROW = D / VW, ROWS = THREADS / ROW, N = CH > ROWS ? CH / ROWS : 1;
     static_assert(THREADS % ROW == 0 && (CH % ROWS == 0 || ROWS % CH == 0), "");
-    static __device__ __forceinline__ bool takes_part() { return ROWS <= CH || (int)(threadIdx.x / ROW) < CH; }
+    static __device__ __forceinline__ int first_row() { return threadIdx.x / ROW; }
+    static __device__ __forceinline__ int column() { return threadIdx.x % ROW * VW; }
+    static __device__ __forceinline__ bool takes_part() { return ROWS <= CH || first_row() < CH; }
     uint4 x[N];
-    const char* at;
+    const char *origin, *at;  // the chunk's first row, and the thread's
     int64_t step;
     int width;
 
     __device__ __forceinline__ void begin(const void* base, int64_t st, int64_t first_token, bool reverse, int elements) {
         step = (reverse ? -st : st) * (int64_t)sizeof(T);
         width = elements;
-        at = (const char*)base + (first_token * st + threadIdx.x % ROW * VW) * (int64_t)sizeof(T) + (int)(threadIdx.x / ROW) * step;
-    }
-    __device__ __forceinline__ uint4 row(int n) const {
-        const T* from = (const T*)(at + n * ROWS * step);
-        if (VEC) return *reinterpret_cast<const uint4*>(from);
-        Pack<T, VW> one;
-#pragma unroll
-        for (int e = 0; e < VW; ++e) one.v[e] = (int)(threadIdx.x % ROW * VW) + e < width ? from[e] : (T)0.f;
-        return __builtin_bit_cast(uint4, one);
+        origin = (const char*)base + first_token * st * (int64_t)sizeof(T);
+        at = origin + first_row() * step + (column() < width ? column() : 0) * (int)sizeof(T);
     }
     __device__ __forceinline__ void load(int places) {  // and on to the next chunk
-        const bool inside = (int)(threadIdx.x % ROW * VW) < width && takes_part();
-        if (places == CH && inside) {
 #pragma unroll
-            for (int n = 0; n < N; ++n) x[n] = row(n);
-        } else {
+        for (int n = 0; n < N; ++n) {
+            const char* from = first_row() + n * ROWS < places ? at + n * ROWS * step : origin;
+            if (VEC)
+                x[n] = *reinterpret_cast<const uint4*>(from);
+            else {
+                Pack<T, VW> one;
 #pragma unroll
-            for (int n = 0; n < N; ++n) {
-                x[n] = make_uint4(0, 0, 0, 0);
-                if (inside && (int)(threadIdx.x / ROW) + n * ROWS < places) x[n] = row(n);
+                for (int e = 0; e < VW; ++e) one.v[e] = column() + e < width ? reinterpret_cast<const T*>(from)[e] : (T)0.f;
+                x[n] = __builtin_bit_cast(uint4, one);
             }
         }
+        origin += CH * step;
         at += CH * step;
     }
-    __device__ __forceinline__ void store(T* tile, int stride) const {
+    __device__ __forceinline__ void store(T* tile, int stride, int places) {
+        if (places < CH || width < D) {
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+                if (first_row() + n * ROWS >= places || column() >= width) x[n] = make_uint4(0, 0, 0, 0);
+        }
         if (!takes_part()) return;
 #pragma unroll
-        for (int n = 0; n < N; ++n) *reinterpret_cast<uint4*>(tile + (threadIdx.x / ROW + n * ROWS) * stride + threadIdx.x % ROW * VW) = x[n];
+        for (int n = 0; n < N; ++n) *reinterpret_cast<uint4*>(tile + (first_row() + n * ROWS) * stride + column()) = x[n];
     }
-    __device__ __forceinline__ uint32_t bad() const {
+    __device__ __forceinline__ uint32_t bad() const {  // of what was stored last
         uint32_t any = 0;
 #pragma unroll
         for (int n = 0; n < N; ++n) any |= not_finite<T>(x[n]);
@@ -227,12 +230,12 @@ __global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS), (Shape<T, CH, DA, 
     const int64_t end = begin + s.part_steps < length ? begin + s.part_steps : length;
     const int64_t first_token = REVERSE ? length - 1 - begin : begin;
     T* out = OUT ? (T*)s.out.data + n * s.out.sn + h * s.out.sh : nullptr;
-    const uint8_t* reset = s.reset ? s.reset + n * s.reset_sn : nullptr;
-    // of the chunk from place `first` on: whether nothing in front of place first + lane reaches it
-    auto load_flag = [&](int64_t first) -> uint32_t {
-        const int64_t p = first + lane;
-        return reset && lane < CH && p < end && (!REVERSE || p > 0) ? reset[(REVERSE ? length - p : p) * s.reset_st] : 0;
-    };
+    // (without resets some byte that is there is loaded, and not used: no branch around the load)
+    const uint8_t* reset = s.reset ? s.reset + n * s.reset_sn : (const uint8_t*)s.log_decay;
+    const int64_t reset_st = s.reset ? s.reset_st : 0;
+    // of the chunk from place `first` on: whether nothing in front of place first + lane reaches it, loaded ahead and looked at later
+    auto has_flag = [&](int64_t first) { return s.reset && lane < CH && first + lane < end && (!REVERSE || first + lane > 0); };
+    auto load_flag = [&](int64_t first) -> uint32_t { return reset[(has_flag(first) ? (REVERSE ? length - (first + lane) : first + lane) : 0) * reset_st]; };
 
     const float log_decay = s.log_decay[h];
     auto decay_of = [&](int k) { return k == 0 ? 1.f : expf(log_decay * (float)k); };  // (k = 0: not 0 * infinity)
@@ -281,16 +284,22 @@ __global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS), (Shape<T, CH, DA, 
         }
     }
 
+    // (the state has arrived before the walk begins: inside, a wait for it would be one for the loads ahead too)
+#pragma unroll
+    for (int ct = 0; ct < S::COLS; ++ct)
+#pragma unroll
+        for (int t = 0; t < DT; ++t) asm volatile("" : "+v"(state[ct][t]));
+
     int parity = 0;
     uint64_t any_cut = 0;
     for (int64_t first = begin; first < end; first += CH, parity ^= 1) {
         at.fresh();
         const int places = end - first < CH ? (int)(end - first) : CH;
         if (!S::AHEAD) load(first);
-        if (OUT) move_a.store(tile_a, S::SA);
-        move_b.store(tile_b, S::SA);
-        move_c.store(tile_c, S::SC);
-        const uint64_t cuts = __ballot(flag != 0);
+        if (OUT) move_a.store(tile_a, S::SA, places);
+        move_b.store(tile_b, S::SA, places);
+        move_c.store(tile_c, S::SC, places);
+        const uint64_t cuts = __ballot(has_flag(first) && flag != 0);
         any_cut |= cuts;
         // (without outputs only a cut can take away what is not finite)
         if (!OUT && cuts && ((move_b.bad() | move_c.bad()) & NOT_FINITE<T>)) spoiled[parity] = 1;
@@ -305,32 +314,46 @@ __global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS), (Shape<T, CH, DA, 
             for (int kk = 0; kk < KC; ++kk) values[ct][kk] = M::columns(at, tile_c, S::SC, kk * M::K, column + 16 * ct);
         if (OUT) {
             float spoils = 0.f;  // becomes NaN with the first number that is none, or infinite
-            // scores: tile (it, jt) holds rows j = 16 jt + .., columns i = 16 it + ..
-            for (int k = wave; k < tiles * (tiles + 1) / 2; k += S::WAVES) {
-                const int it = k >= 6 ? 3 : k >= 3 ? 2 : k >= 1 ? 1 : 0, jt = k - it * (it + 1) / 2, i = 16 * it + at.l;
-                f32x4 x = {0.f, 0.f, 0.f, 0.f};
+            // scores: tile k = (it, jt), jt <= it, holds rows j = 16 jt + .., columns i = 16 it + ..; two at once, whose latencies overlap
+            const int count = tiles * (tiles + 1) / 2;
+            for (int k0 = wave; k0 < count; k0 += 2 * S::WAVES) {
+                int it[2], jt[2];
+                f32x4 x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-                for (int kk = 0; kk < KA; ++kk) x = M::product(M::rows(at, tile_b, S::SA, 16 * jt, kk * M::K), M::rows(at, tile_a, S::SA, 16 * it, kk * M::K), x);
-                const float far = it - jt > 1 ? power[16 * (it - jt - 1)] : 1.f;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    spoils = fmaf(x[r], 0.f, spoils);  // (the tiles on the diagonal see every row of a and b)
-                    x[r] *= it == jt ? w_diagonal[r] : w_below[r] * far;
+                for (int u = 0; u < 2; ++u) {
+                    const int k = k0 + u * S::WAVES < count ? k0 + u * S::WAVES : k0;
+                    it[u] = k >= 6 ? 3 : k >= 3 ? 2 : k >= 1 ? 1 : 0, jt[u] = k - it[u] * (it[u] + 1) / 2;
                 }
-                if (cuts) {
-                    const uint64_t before = cuts & (~0ull >> (63 - i));
-                    const int from = before ? 63 - __builtin_clzll(before) : 0;  // the first place that i sees
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) x[r] = 16 * jt + 4 * at.g + r >= from ? x[r] : 0.f;
-                }
-                Pack<T, 4> p;
+                for (int kk = 0; kk < KA; ++kk)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) p.v[r] = (T)x[r];
-                *reinterpret_cast<Pack<T, 4>*>(tile_p + i * S::SP + 16 * jt + 4 * at.g) = p;
-                if (PER == 2 && it == jt && it % 2 == 0) {  // the tile above the diagonal that shares a fragment with it
+                    for (int u = 0; u < 2; ++u)
+                        x[u] = M::product(M::rows(at, tile_b, S::SA, 16 * jt[u], kk * M::K), M::rows(at, tile_a, S::SA, 16 * it[u], kk * M::K), x[u]);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) p.v[r] = (T)0.f;
-                    *reinterpret_cast<Pack<T, 4>*>(tile_p + i * S::SP + 16 * jt + 16 + 4 * at.g) = p;
+                for (int u = 0; u < 2; ++u) {
+                    const int i = 16 * it[u] + at.l;
+                    const bool diagonal = it[u] == jt[u];
+                    const float far = it[u] - jt[u] > 1 ? power[16 * (it[u] - jt[u] - 1)] : 1.f;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        spoils = fmaf(x[u][r], 0.f, spoils);  // (the tiles on the diagonal see every row of a and b)
+                        x[u][r] *= diagonal ? w_diagonal[r] : w_below[r] * far;
+                    }
+                    if (cuts) {
+                        const uint64_t before = cuts & (~0ull >> (63 - i));
+                        const int from = before ? 63 - __builtin_clzll(before) : 0;  // the first place that i sees
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) x[u][r] = 16 * jt[u] + 4 * at.g + r >= from ? x[u][r] : 0.f;
+                    }
+                    Pack<T, 4> p;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) p.v[r] = (T)x[u][r];
+                    *reinterpret_cast<Pack<T, 4>*>(tile_p + i * S::SP + 16 * jt[u] + 4 * at.g) = p;
+                    if (PER == 2 && diagonal && it[u] % 2 == 0) {  // the tile above the diagonal that shares a fragment with it
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) p.v[r] = (T)0.f;
+                        *reinterpret_cast<Pack<T, 4>*>(tile_p + i * S::SP + 16 * jt[u] + 16 + 4 * at.g) = p;
+                    }
                 }
             }
             if (spoils != 0.f) spoiled[parity] = 1;
@@ -350,56 +373,69 @@ __global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS), (Shape<T, CH, DA, 
             const int64_t on = (REVERSE ? -16 : 16) * s.out.st;
             float spoils = 0.f;
 #pragma unroll 1
-            for (int it = 0; it < tiles; ++it, to += on) {
+            for (int pair = 0; pair < tiles; pair += 2) {  // two tiles at once; a second one behind the last is computed, and dropped
                 at.fresh();
-                const int i = 16 * it + at.l;
-                f32x4 x[S::COLS];
+                f32x4 x[2][S::COLS];
 #pragma unroll
-                for (int ct = 0; ct < S::COLS; ++ct) x[ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int kk = 0; kk < KA; ++kk) {
-                    const Frag right = M::rows_as_state(at, tile_a, S::SA, 16 * it, kk * M::K);
+                    for (int ct = 0; ct < S::COLS; ++ct) x[u][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int ct = 0; ct < S::COLS; ++ct) x[ct] = M::product(left[ct][kk], right, x[ct]);
-                }
-                const float w = enter[i + enters];
+                for (int kk = 0; kk < KA; ++kk)
 #pragma unroll
-                for (int ct = 0; ct < S::COLS; ++ct) x[ct] *= w;
-                if (cuts) {
-                    const bool sees = (cuts & (~0ull >> (63 - i))) == 0;
+                    for (int u = 0; u < 2; ++u) {
+                        const Frag right = M::rows_as_state(at, tile_a, S::SA, 16 * (pair + u), kk * M::K);
 #pragma unroll
-                    for (int ct = 0; ct < S::COLS; ++ct)
+                        for (int ct = 0; ct < S::COLS; ++ct) x[u][ct] = M::product(left[ct][kk], right, x[u][ct]);
+                    }
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) x[ct][r] = sees ? x[ct][r] : 0.f;
+                for (int u = 0; u < 2; ++u) {
+                    const int i = 16 * (pair + u) + at.l;
+                    const float w = enter[i + enters];
+#pragma unroll
+                    for (int ct = 0; ct < S::COLS; ++ct) x[u][ct] *= w;
+                    if (cuts) {
+                        const bool sees = (cuts & (~0ull >> (63 - i))) == 0;
+#pragma unroll
+                        for (int ct = 0; ct < S::COLS; ++ct)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) x[u][ct][r] = sees ? x[u][ct][r] : 0.f;
+                    }
                 }
 #pragma unroll
                 for (int kk = 0; kk < KC; ++kk)
-                    if (kk * PER <= it) {
-                        const Frag right = M::rows(at, tile_p, S::SP, 16 * it, kk * M::K);
 #pragma unroll
-                        for (int ct = 0; ct < S::COLS; ++ct) x[ct] = M::product(values[ct][kk], right, x[ct]);
+                    for (int u = 0; u < 2; ++u)
+                        if (kk * PER <= pair + (PER == 2 ? 0 : u)) {
+                            const Frag right = M::rows(at, tile_p, S::SP, 16 * (pair + u), kk * M::K);
+#pragma unroll
+                            for (int ct = 0; ct < S::COLS; ++ct) x[u][ct] = M::product(values[ct][kk], right, x[u][ct]);
+                        }
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    if (pair + u == tiles - 1) {
+#pragma unroll
+                        for (int ct = 0; ct < S::COLS; ++ct)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) spoils = fmaf(x[u][ct][r], 0.f, spoils);
                     }
-                if (it == tiles - 1) {
+                    if (16 * (pair + u) + at.l < places) {
 #pragma unroll
-                    for (int ct = 0; ct < S::COLS; ++ct)
+                        for (int ct = 0; ct < S::COLS; ++ct) {
+                            const int j = column + 16 * ct + 4 * at.g;
+                            Pack<T, 4> y;
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) spoils = fmaf(x[ct][r], 0.f, spoils);
-                }
-                if (i < places) {
+                            for (int r = 0; r < 4; ++r) y.v[r] = (T)x[u][ct][r];
+                            if (VEC) {
+                                if (j < s.dc) *reinterpret_cast<Pack<T, 4>*>(to + 16 * ct) = y;
+                            } else {
 #pragma unroll
-                    for (int ct = 0; ct < S::COLS; ++ct) {
-                        const int j = column + 16 * ct + 4 * at.g;
-                        Pack<T, 4> y;
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) y.v[r] = (T)x[ct][r];
-                        if (VEC) {
-                            if (j < s.dc) *reinterpret_cast<Pack<T, 4>*>(to + 16 * ct) = y;
-                        } else {
-#pragma unroll
-                            for (int r = 0; r < 4; ++r)
-                                if (j + r < s.dc) to[16 * ct + r] = y.v[r];
+                                for (int r = 0; r < 4; ++r)
+                                    if (j + r < s.dc) to[16 * ct + r] = y.v[r];
+                            }
                         }
                     }
+                    to += on;
                 }
             }
             // the last tile's products see every c: one that is not finite in this wave's columns (or the state) shows in them, and the wave, whose
@@ -448,22 +484,24 @@ __global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS), (Shape<T, CH, DA, 
 #pragma unroll
                     for (int t = 0; t < DT; ++t) state[ct][t] *= whole;
             }
+            float w[KC][M::K / 4];
+            if (places == CH && !cuts) {
 #pragma unroll
-            for (int kk = 0; kk < KC; ++kk) {
-                if (kk * M::K >= places) break;
-                Frag right[S::COLS][M::SPLITS];
-                float w[M::K / 4];
-                if (places == CH && !cuts)
-                    load_pack<float, M::K / 4>(leave + kk * M::K + M::place(at, 0), w);
-                else {
+                for (int kk = 0; kk < KC; ++kk) load_pack<float, M::K / 4>(leave + kk * M::K + M::place(at, 0), w[kk]);
+            } else {
+#pragma unroll
+                for (int kk = 0; kk < KC; ++kk)
 #pragma unroll
                     for (int e = 0; e < M::K / 4; ++e) {
                         const int j = kk * M::K + M::place(at, e);
-                        w[e] = j >= last_cut && j < places ? power[places - 1 - j] * s.in_scale : 0.f;
+                        w[kk][e] = j >= last_cut && j < places ? power[places - 1 - j] * s.in_scale : 0.f;
                     }
-                }
+            }
 #pragma unroll
-                for (int ct = 0; ct < S::COLS; ++ct) M::weighted(values[ct][kk], w, right[ct]);
+            for (int kk = 0; kk < KC; ++kk) {
+                Frag right[S::COLS][M::SPLITS];
+#pragma unroll
+                for (int ct = 0; ct < S::COLS; ++ct) M::weighted(values[ct][kk], w[kk], right[ct]);
 #pragma unroll
                 for (int t = 0; t < DT; ++t) {
                     const Frag left = M::columns(at, tile_b, S::SA, kk * M::K, 16 * t);
@@ -482,7 +520,7 @@ __global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS), (Shape<T, CH, DA, 
             for (int j = threadIdx.x % 32; j < s.dc; j += 32) out[t * s.out.st + j] = (T)0.f;
     if (!OUT && threadIdx.x == 0) s.carry_out[which] = any_cut ? -1.f : decay_of(begin < end ? (int)(end - begin) - (REVERSE && begin == 0 ? 1 : 0) : 0);
     if (s.state_out) {
-        const bool leaves = REVERSE && s.parts == 1 && length > 0, cut = leaves && reset && reset[0];
+        const bool leaves = REVERSE && s.parts == 1 && length > 0, cut = leaves && s.reset && reset[0];
         const float carry = leaves ? power[1] : 1.f;
 #pragma unroll
         for (int ct = 0; ct < S::COLS; ++ct) {

@@ -58,9 +58,10 @@ typedef struct lobpolicy_attention {
     float scale;
     void* workspace;
     int64_t workspace_bytes;
+    const void* forward_workspace;    /* backward: the workspace that the forward call left, unchanged (the states in front of each part) */
 } lobpolicy_attention;
 
-int64_t lobpolicy_attention_workspace(const lobpolicy_attention* a, int32_t backward); /* bytes; negative: lobpolicy_error */
+int64_t lobpolicy_attention_workspace(const lobpolicy_attention* a); /* bytes, of either call; negative: lobpolicy_error */
 int lobpolicy_attention_forward(const lobpolicy_attention* a, void* stream);
 int lobpolicy_attention_backward(const lobpolicy_attention* a, void* stream);
 int lobpolicy_attention_step(const lobpolicy_attention* a, void* stream); /* one token of every environment: steps is 1 */

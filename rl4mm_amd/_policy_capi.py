@@ -23,7 +23,7 @@ class Attention(C.Structure):
         ("log_decay", C.c_void_p), ("reset", C.c_void_p), ("reset_stride_t", C.c_int64), ("reset_stride_n", C.c_int64),
         ("lengths", C.c_void_p), ("skip", C.c_void_p),
         ("state_in", C.c_void_p), ("state_out", C.c_void_p), ("grad_state_out", C.c_void_p), ("grad_state_in", C.c_void_p),
-        ("scale", C.c_float), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+        ("scale", C.c_float), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64), ("forward_workspace", C.c_void_p),
     ]  # fmt: skip
 
 
@@ -45,7 +45,7 @@ _PA, _PB = C.POINTER(Attention), C.POINTER(Block)
 PROTOTYPES = {
     "abi_version": (C.c_int, []),
     "last_error": (C.c_char_p, []),
-    "attention_workspace": (C.c_int64, [_PA, C.c_int32]),
+    "attention_workspace": (C.c_int64, [_PA]),
     "attention_forward": (C.c_int, [_PA, C.c_void_p]),
     "attention_backward": (C.c_int, [_PA, C.c_void_p]),
     "attention_step": (C.c_int, [_PA, C.c_void_p]),

@@ -86,6 +86,7 @@ struct Scan {
     int64_t in_row, in_col, out_row, out_col;
     int64_t steps, envs;
     int heads, da, dc;
+    bool reverse;
     float in_scale, out_scale;
     int64_t part_steps;  // the steps are split into `parts` of this many, each a workgroup's; state_in and state_out are then [unit][part]
     int parts;
@@ -98,8 +99,15 @@ __device__ __forceinline__ int64_t length_of(const Scan& s, int64_t n) {
     return l < 0 ? 0 : (l > s.steps ? s.steps : l);
 }
 
-// one kernel family per type and rows of the state (DA = 32, 64 or 128 holds s.da)
+// Up to three walks over the same steps in one launch: what one reads the others find in the cache, and few environments fill more of the card.
+struct Walks {
+    Scan walk[3];
+    int count;
+};
+
+// One family per type and rows of the state: DA = 32, 64 or 128 holds da.  Every walk's da and dc are the first one's, or (`swapped`: the second and
+// third) the first one's the other way round.
 template <class T, int DA>
-int scan_rows(const Scan& s, bool reverse, hipStream_t stream);
+int scan_rows(const Walks& w, bool swapped, hipStream_t stream);
 
 }  // namespace lobpolicy

@@ -19,10 +19,11 @@ int fail(int code, const char* format, ...) {
 }
 
 template <class T>
-int scan_typed(const Scan& s, bool reverse, hipStream_t stream) {
-    if (s.da <= 32) return scan_rows<T, 32>(s, reverse, stream);
-    if (s.da <= 64) return scan_rows<T, 64>(s, reverse, stream);
-    return scan_rows<T, 128>(s, reverse, stream);
+int scan_typed(const Walks& w, bool swapped, hipStream_t stream) {
+    const int da = w.walk[0].da;
+    if (da <= 32) return scan_rows<T, 32>(w, swapped, stream);
+    if (da <= 64) return scan_rows<T, 64>(w, swapped, stream);
+    return scan_rows<T, 128>(w, swapped, stream);
 }
 
 // Few environments and heads, many steps: the steps are split into parts.  A first walk finds what each part adds to the state, join_parts
@@ -42,7 +43,6 @@ struct Parts {
 };
 
 // grid (elements / 256, units): `states` [unit][part] from what each part adds to what is in front of it; the state behind the last to state_out
-template <bool REVERSE>
 __global__ __launch_bounds__(256) void join_parts(Scan s, float* states, const float* __restrict__ carries) {
     const int64_t unit = blockIdx.y, matrix = (int64_t)s.da * s.dc, e = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (e >= matrix) return;
@@ -73,29 +73,26 @@ __global__ __launch_bounds__(256) void join_parts(Scan s, float* states, const f
     }
     if (s.state_out) {
         const int64_t n = unit / s.heads;
-        if (REVERSE && length_of(s, n) > 0) state = s.reset && s.reset[n * s.reset_sn] ? 0.f : state * expf(s.log_decay[unit % s.heads]);
+        if (s.reverse && length_of(s, n) > 0) state = s.reset && s.reset[n * s.reset_sn] ? 0.f : state * expf(s.log_decay[unit % s.heads]);
         s.state_out[unit * matrix + row * s.out_row + col * s.out_col] = state;
     }
 }
 
-int walk(const lobpolicy_attention* a, const Scan& s, bool reverse, hipStream_t stream) {
-    return a->dtype == LOBPOLICY_BF16 ? scan_typed<bf16>(s, reverse, stream) : scan_typed<float>(s, reverse, stream);
+int walk(const lobpolicy_attention* a, const Walks& w, bool swapped, hipStream_t stream) {
+    return a->dtype == LOBPOLICY_BF16 ? scan_typed<bf16>(w, swapped, stream) : scan_typed<float>(w, swapped, stream);
 }
 
-// the states in front of each part, to the workspace (which holds them by rows, whatever s.in_row says); s.state_out
-int part_states(const lobpolicy_attention* a, Scan s, bool reverse, hipStream_t stream) {
+// the states in front of each part of a walk with da = dk and dc = dv, to the workspace; s.state_out
+int part_states(const lobpolicy_attention* a, const Scan& s, hipStream_t stream) {
     const Parts parts(a);
     float* states = (float*)a->workspace;
     float* carries = states + parts.matrices(a) * a->dk * a->dv;
-    Scan first = s;
-    first.a = first.b, first.out = {};
-    first.state_in = nullptr, first.state_out = states, first.out_row = s.dc, first.out_col = 1, first.carry_out = carries;
-    if (int e = walk(a, first, reverse, stream)) return e;
-    const dim3 grid((unsigned)ceil_div((int64_t)s.da * s.dc, 256), (unsigned)(a->envs * a->heads));
-    if (reverse)
-        join_parts<true><<<grid, 256, 0, stream>>>(s, states, carries);
-    else
-        join_parts<false><<<grid, 256, 0, stream>>>(s, states, carries);
+    Walks first = {{s}, 1};
+    Scan& w = first.walk[0];
+    w.a = w.b, w.out = {};
+    w.state_in = nullptr, w.state_out = states, w.carry_out = carries;
+    if (int e = walk(a, first, false, stream)) return e;
+    join_parts<<<dim3((unsigned)ceil_div((int64_t)s.da * s.dc, 256), (unsigned)(a->envs * a->heads)), 256, 0, stream>>>(s, states, carries);
     return launched();
 }
 
@@ -662,8 +659,7 @@ extern "C" {
 int lobpolicy_abi_version(void) { return LOBPOLICY_ABI_VERSION; }
 const char* lobpolicy_last_error(void) { return g_error; }
 
-int64_t lobpolicy_attention_workspace(const lobpolicy_attention* a, int32_t backward) {
-    (void)backward;
+int64_t lobpolicy_attention_workspace(const lobpolicy_attention* a) {
     if (int e = check_attention(a)) return e;
     return Parts(a).bytes(a);
 }
@@ -679,10 +675,10 @@ int lobpolicy_attention_forward(const lobpolicy_attention* a, void* stream) {
     s.state_in = a->state_in, s.state_out = a->state_out;
     s.in_row = s.out_row = a->dv, s.in_col = s.out_col = 1;
     if (s.parts > 1) {
-        if (int e = part_states(a, s, false, (hipStream_t)stream)) return e;
+        if (int e = part_states(a, s, (hipStream_t)stream)) return e;
         s.state_in = (const float*)a->workspace, s.state_out = nullptr;
     }
-    return walk(a, s, false, (hipStream_t)stream);
+    return walk(a, Walks{{s}, 1}, false, (hipStream_t)stream);
 }
 
 int lobpolicy_attention_backward(const lobpolicy_attention* a, void* stream) {
@@ -690,35 +686,26 @@ int lobpolicy_attention_backward(const lobpolicy_attention* a, void* stream) {
     REQUIRE(a->q.data && a->k.data && a->v.data && a->out.data, "an operand is missing");
     REQUIRE(a->grad_q.data && a->grad_k.data && a->grad_v.data, "a gradient is missing");
     if (int e = check_workspace(a)) return e;
-    hipStream_t st = (hipStream_t)stream;
     const Rows q = rows_of(a->q), k = rows_of(a->k), v = rows_of(a->v), d = rows_of(a->out);
-    const float* states = (const float*)a->workspace;
-    // forwards: the state, for dq
+    // backwards, the state's gradient: for dv, and transposed for dk; forwards, the state, transposed: for dq
     Scan s = scan_of(a);
-    s.state_in = a->state_in;
-    if (s.parts > 1) {
-        s.b = k, s.c = v, s.da = a->dk, s.dc = a->dv, s.in_row = a->dv, s.in_col = 1;
-        if (int e = part_states(a, s, false, st)) return e;
-        s.state_in = states;
-    }
-    s.a = d, s.b = v, s.c = k, s.out = rows_of(a->grad_q);
-    s.da = a->dv, s.dc = a->dk, s.in_row = 1, s.in_col = a->dv;
-    s.out_scale = a->scale;
-    if (int e = walk(a, s, false, st)) return e;
-    // backwards: its gradient, for dv and dk
-    s.out_scale = 1.f, s.in_scale = a->scale;
-    s.state_in = a->grad_state_out, s.state_out = a->grad_state_in;
     s.a = k, s.b = q, s.c = d, s.out = rows_of(a->grad_v);
     s.da = a->dk, s.dc = a->dv, s.in_row = s.out_row = a->dv, s.in_col = s.out_col = 1;
+    s.reverse = true, s.in_scale = a->scale;
+    s.state_in = a->grad_state_out, s.state_out = a->grad_state_in;
+    const float* states = a->state_in;
     if (s.parts > 1) {
-        if (int e = part_states(a, s, true, st)) return e;
-        s.state_in = states, s.state_out = nullptr;
+        REQUIRE(a->forward_workspace && aligned(a->forward_workspace, 16), "no forward_workspace");
+        if (int e = part_states(a, s, (hipStream_t)stream)) return e;
+        s.state_in = (const float*)a->workspace, s.state_out = nullptr;
+        states = (const float*)a->forward_workspace;
     }
-    if (int e = walk(a, s, true, st)) return e;
-    s.state_out = nullptr;
-    s.a = v, s.b = d, s.c = q, s.out = rows_of(a->grad_k);
-    s.da = a->dv, s.dc = a->dk, s.in_row = 1, s.in_col = a->dv;
-    return walk(a, s, true, st);
+    Walks w = {{s, s, s}, 3};
+    for (int i = 1; i < 3; ++i) w.walk[i].da = a->dv, w.walk[i].dc = a->dk, w.walk[i].in_row = 1, w.walk[i].in_col = a->dv, w.walk[i].state_out = nullptr;
+    w.walk[1].a = v, w.walk[1].b = d, w.walk[1].c = q, w.walk[1].out = rows_of(a->grad_k);
+    w.walk[2].a = d, w.walk[2].b = v, w.walk[2].c = k, w.walk[2].out = rows_of(a->grad_q);
+    w.walk[2].reverse = false, w.walk[2].in_scale = 1.f, w.walk[2].out_scale = a->scale, w.walk[2].state_in = states;
+    return walk(a, w, true, (hipStream_t)stream);
 }
 
 int lobpolicy_attention_step(const lobpolicy_attention* a, void* stream) {

@@ -203,39 +203,45 @@ struct Column {
     __device__ __forceinline__ void store(int i, float x) const { __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, x), buffer, offset(i), 0, 0); }
 };
 
-// OUT: the walk's outputs; without it the state behind each part alone, from a state of 0 in front of it
-template <class T, int CH, int DA, int DC, bool REVERSE, bool OUT, bool VEC>
-__global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS), (Shape<T, CH, DA, DC>::LEAST_WAVES)) void scan_chunks(Scan s) {
+// What a workgroup keeps in LDS
+template <class T, int CH, int DA, int DC, bool OUT>
+struct Room {
+    typedef Shape<T, CH, DA, DC> S;
+    alignas(16) T a[OUT ? CH * S::SA : 8];
+    alignas(16) T b[CH * S::SA];
+    alignas(16) T c[CH * S::SC];
+    alignas(16) T p[OUT ? CH * S::SP : 8];
+    alignas(16) float leave[CH];              // l^(CH - 1 - j) in_scale
+    float power[CH + 1], enter[CH + 1];       // l^k, and times out_scale
+    uint32_t spoiled[2];
+};
+
+// One part of one walk.  OUT: its outputs; without it the state behind the part alone, from a state of 0 in front of it
+template <class T, int CH, int DA, int DC, bool OUT, bool VEC>
+__device__ __forceinline__ void walk_part(const Scan& s, int64_t unit, int64_t part, Room<T, CH, DA, DC, OUT>& room) {
     typedef Shape<T, CH, DA, DC> S;
     typedef Tile<T> M;
     typedef typename M::Frag Frag;
     constexpr int KA = DA / M::K, KC = CH / M::K, DT = DA / 16, PER = M::K / 16;
-    __shared__ __align__(16) T tile_a[OUT ? CH * S::SA : 8];
-    __shared__ __align__(16) T tile_b[CH * S::SA];
-    __shared__ __align__(16) T tile_c[CH * S::SC];
-    __shared__ __align__(16) T tile_p[OUT ? CH * S::SP : 8];
-    __shared__ float power[CH + 1], enter[CH + 1];     // l^k, and times out_scale
-    __shared__ __align__(16) float leave[CH];          // l^(CH - 1 - j) in_scale
-    __shared__ uint32_t spoiled[2];
-
-    // neighbouring workgroups run on different dies, each with a cache of its own: every die gets a run of neighbouring units
-    const uint32_t units = (uint32_t)(s.envs * s.heads), each = gridDim.x / 8, more = gridDim.x % 8, die = blockIdx.x % 8;
-    const uint32_t index = die * each + (die < more ? die : more) + blockIdx.x / 8;
-    const int64_t unit = index % units, part = index / units, n = (uint32_t)unit / (uint32_t)s.heads;
+    T *const tile_a = room.a, *const tile_b = room.b, *const tile_c = room.c, *const tile_p = room.p;
+    float *const power = room.power, *const enter = room.enter, *const leave = room.leave;
+    uint32_t* const spoiled = room.spoiled;
+    const bool reverse = s.reverse;
+    const int64_t n = (uint32_t)unit / (uint32_t)s.heads;
     const int h = (int)((uint32_t)unit % (uint32_t)s.heads);
     const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, column = wave * S::COLS * 16;
     Lane at = {lane % 16, lane / 16};
 
     const int64_t length = length_of(s, n), begin = part * s.part_steps;
     const int64_t end = begin + s.part_steps < length ? begin + s.part_steps : length;
-    const int64_t first_token = REVERSE ? length - 1 - begin : begin;
+    const int64_t first_token = reverse ? length - 1 - begin : begin;
     T* out = OUT ? (T*)s.out.data + n * s.out.sn + h * s.out.sh : nullptr;
     // (without resets some byte that is there is loaded, and not used: no branch around the load)
     const uint8_t* reset = s.reset ? s.reset + n * s.reset_sn : (const uint8_t*)s.log_decay;
     const int64_t reset_st = s.reset ? s.reset_st : 0;
     // of the chunk from place `first` on: whether nothing in front of place first + lane reaches it, loaded ahead and looked at later
-    auto has_flag = [&](int64_t first) { return s.reset && lane < CH && first + lane < end && (!REVERSE || first + lane > 0); };
-    auto load_flag = [&](int64_t first) -> uint32_t { return reset[(has_flag(first) ? (REVERSE ? length - (first + lane) : first + lane) : 0) * reset_st]; };
+    auto has_flag = [&](int64_t first) { return s.reset && lane < CH && first + lane < end && (!reverse || first + lane > 0); };
+    auto load_flag = [&](int64_t first) -> uint32_t { return reset[(has_flag(first) ? (reverse ? length - (first + lane) : first + lane) : 0) * reset_st]; };
 
     const float log_decay = s.log_decay[h];
     auto decay_of = [&](int k) { return k == 0 ? 1.f : expf(log_decay * (float)k); };  // (k = 0: not 0 * infinity)
@@ -257,9 +263,9 @@ __global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS), (Shape<T, CH, DA, 
     Moving<T, CH, DA, S::THREADS, VEC> move_a, move_b;
     Moving<T, CH, DC, S::THREADS, VEC> move_c;
     uint32_t flag = 0;
-    if (OUT) move_a.begin((const T*)s.a.data + n * s.a.sn + h * s.a.sh, s.a.st, first_token, REVERSE, s.da);
-    move_b.begin((const T*)s.b.data + n * s.b.sn + h * s.b.sh, s.b.st, first_token, REVERSE, s.da);
-    move_c.begin((const T*)s.c.data + n * s.c.sn + h * s.c.sh, s.c.st, first_token, REVERSE, s.dc);
+    if (OUT) move_a.begin((const T*)s.a.data + n * s.a.sn + h * s.a.sh, s.a.st, first_token, reverse, s.da);
+    move_b.begin((const T*)s.b.data + n * s.b.sn + h * s.b.sh, s.b.st, first_token, reverse, s.da);
+    move_c.begin((const T*)s.c.data + n * s.c.sn + h * s.c.sh, s.c.st, first_token, reverse, s.dc);
     auto load = [&](int64_t first) {
         const int places = end - first < CH ? (int)(end - first) : CH;
         if (OUT) move_a.load(places);
@@ -305,7 +311,7 @@ __global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS), (Shape<T, CH, DA, 
         if (!OUT && cuts && ((move_b.bad() | move_c.bad()) & NOT_FINITE<T>)) spoiled[parity] = 1;
         __syncthreads();
         if (S::AHEAD && first + CH < end) load(first + CH);
-        const int enters = REVERSE && first == 0 ? 0 : 1;  // decays between what comes into the chunk and its first place
+        const int enters = reverse && first == 0 ? 0 : 1;  // decays between what comes into the chunk and its first place
         const int tiles = (places + 15) / 16;
         Frag values[S::COLS][KC];  // c, by columns
 #pragma unroll
@@ -361,7 +367,7 @@ __global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS), (Shape<T, CH, DA, 
         }
         bool by_token = spoiled[parity] != 0;
         if (threadIdx.x == 0) spoiled[parity ^ 1] = 0;
-        auto token = [&](int p) { return (REVERSE ? length - 1 - (first + p) : first + p) * s.out.st; };
+        auto token = [&](int p) { return (reverse ? length - 1 - (first + p) : first + p) * s.out.st; };
 
         if (OUT && !by_token) {
             Frag left[S::COLS][KA];
@@ -370,7 +376,7 @@ __global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS), (Shape<T, CH, DA, 
 #pragma unroll
                 for (int kk = 0; kk < KA; ++kk) left[ct][kk] = M::of_state(&state[ct][kk * PER]);
             T* to = out + token(at.l) + column + 4 * at.g;
-            const int64_t on = (REVERSE ? -16 : 16) * s.out.st;
+            const int64_t on = (reverse ? -16 : 16) * s.out.st;
             float spoils = 0.f;
 #pragma unroll 1
             for (int pair = 0; pair < tiles; pair += 2) {  // two tiles at once; a second one behind the last is computed, and dropped
@@ -518,9 +524,9 @@ __global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS), (Shape<T, CH, DA, 
     if (OUT && part == s.parts - 1)  // rows behind the last token
         for (int64_t t = length + threadIdx.x / 32; t < s.steps; t += S::THREADS / 32)
             for (int j = threadIdx.x % 32; j < s.dc; j += 32) out[t * s.out.st + j] = (T)0.f;
-    if (!OUT && threadIdx.x == 0) s.carry_out[which] = any_cut ? -1.f : decay_of(begin < end ? (int)(end - begin) - (REVERSE && begin == 0 ? 1 : 0) : 0);
+    if (!OUT && threadIdx.x == 0) s.carry_out[which] = any_cut ? -1.f : decay_of(begin < end ? (int)(end - begin) - (reverse && begin == 0 ? 1 : 0) : 0);
     if (s.state_out) {
-        const bool leaves = REVERSE && s.parts == 1 && length > 0, cut = leaves && s.reset && reset[0];
+        const bool leaves = reverse && s.parts == 1 && length > 0, cut = leaves && s.reset && reset[0];
         const float carry = leaves ? power[1] : 1.f;
 #pragma unroll
         for (int ct = 0; ct < S::COLS; ++ct) {
@@ -533,38 +539,62 @@ __global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS), (Shape<T, CH, DA, 
     }
 }
 
-template <class T, int CH, int DA, int DC, bool VEC>
-int scan_launch(const Scan& s, bool reverse, hipStream_t stream) {
-    const dim3 grid((unsigned)(s.envs * s.heads * s.parts));
-    constexpr int threads = Shape<T, CH, DA, DC>::THREADS;
-    if (s.out.data && reverse)
-        scan_chunks<T, CH, DA, DC, true, true, VEC><<<grid, threads, 0, stream>>>(s);
-    else if (s.out.data)
-        scan_chunks<T, CH, DA, DC, false, true, VEC><<<grid, threads, 0, stream>>>(s);
-    else if (reverse)
-        scan_chunks<T, CH, DA, DC, true, false, VEC><<<grid, threads, 0, stream>>>(s);
-    else
-        scan_chunks<T, CH, DA, DC, false, false, VEC><<<grid, threads, 0, stream>>>(s);
+// BOTH: the second and third walk have da and dc the other way round
+template <class T, int CH, int DA, int DC, bool BOTH, bool OUT, bool VEC>
+__global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS > Shape<T, CH, DC, DA>::THREADS && BOTH ? Shape<T, CH, DA, DC>::THREADS : BOTH ? Shape<T, CH, DC, DA>::THREADS : Shape<T, CH, DA, DC>::THREADS), (Shape<T, CH, DA, DC>::LEAST_WAVES)) void scan_chunks(Walks w) {
+    union Shared {
+        Room<T, CH, DA, DC, OUT> one;
+        Room<T, CH, BOTH ? DC : DA, BOTH ? DA : DC, OUT> other;
+    };
+    __shared__ __align__(16) char room[sizeof(Shared)];
+    Shared& shared = *reinterpret_cast<Shared*>(room);
+    // neighbouring workgroups run on different dies, each with a cache of its own: every die gets a run of neighbouring units, and all walks of a unit
+    const uint32_t units = (uint32_t)(w.walk[0].envs * w.walk[0].heads), each = gridDim.x / 8, more = gridDim.x % 8, die = blockIdx.x % 8;
+    const uint32_t index = die * each + (die < more ? die : more) + blockIdx.x / 8;
+    const uint32_t which = index % (uint32_t)w.count, place = index / (uint32_t)w.count;
+    const Scan& s = w.walk[which];
+    if (!BOTH || which == 0) {
+        if (threadIdx.x < Shape<T, CH, DA, DC>::THREADS) walk_part<T, CH, DA, DC, OUT, VEC>(s, place % units, place / units, shared.one);
+    } else if (BOTH) {
+        if (threadIdx.x < Shape<T, CH, DC, DA>::THREADS) walk_part<T, CH, BOTH ? DC : DA, BOTH ? DA : DC, OUT, VEC>(s, place % units, place / units, shared.other);
+    }
+}
+
+template <class T, int CH, int DA, int DC, bool BOTH, bool VEC>
+int scan_launch(const Walks& w, hipStream_t stream) {
+    const Scan& s = w.walk[0];
+    const dim3 grid((unsigned)(s.envs * s.heads * s.parts * w.count));
+    constexpr int one = Shape<T, CH, DA, DC>::THREADS, other = BOTH ? Shape<T, CH, DC, DA>::THREADS : one, threads = one > other ? one : other;
+    if (s.out.data)
+        scan_chunks<T, CH, DA, DC, BOTH, true, VEC><<<grid, threads, 0, stream>>>(w);
+    else if constexpr (!BOTH)
+        scan_chunks<T, CH, DA, DC, false, false, VEC><<<grid, threads, 0, stream>>>(w);
     return launched();
 }
 
 template <class T, int CH, int DA, int DC>
-int scan_aligned(const Scan& s, bool reverse, hipStream_t stream) {
+int scan_aligned(const Walks& w, bool swapped, hipStream_t stream) {
     constexpr int W = 16 / sizeof(T);
-    bool wide = s.da % W == 0 && s.dc % W == 0 && aligned(s.out.data, 16);
-    for (const Rows* r : {&s.a, &s.b, &s.c}) wide = wide && aligned(r->data, 16) && r->st % W == 0 && r->sn % W == 0 && r->sh % W == 0;
-    wide = wide && s.out.st % 4 == 0 && s.out.sn % 4 == 0 && s.out.sh % 4 == 0;
-    return wide ? scan_launch<T, CH, DA, DC, true>(s, reverse, stream) : scan_launch<T, CH, DA, DC, false>(s, reverse, stream);
+    bool wide = true;
+    for (int i = 0; i < w.count; ++i) {
+        const Scan& s = w.walk[i];
+        wide = wide && s.da % W == 0 && s.dc % W == 0 && aligned(s.out.data, 16) && s.out.st % 4 == 0 && s.out.sn % 4 == 0 && s.out.sh % 4 == 0;
+        for (const Rows* r : {&s.a, &s.b, &s.c}) wide = wide && aligned(r->data, 16) && r->st % W == 0 && r->sn % W == 0 && r->sh % W == 0;
+    }
+    if constexpr (DA != DC)
+        if (swapped) return wide ? scan_launch<T, CH, DA, DC, true, true>(w, stream) : scan_launch<T, CH, DA, DC, true, false>(w, stream);
+    return wide ? scan_launch<T, CH, DA, DC, false, true>(w, stream) : scan_launch<T, CH, DA, DC, false, false>(w, stream);
 }
 
 template <class T, int DA>
-int scan_rows(const Scan& s, bool reverse, hipStream_t stream) {
+int scan_rows(const Walks& w, bool swapped, hipStream_t stream) {
     constexpr int CH = sizeof(T) == 4 ? 32 : 64;
-    if (s.dc <= 32) return scan_aligned<T, CH, DA, 32>(s, reverse, stream);
-    if (s.dc <= 64) return scan_aligned<T, CH, DA, 64>(s, reverse, stream);
-    return scan_aligned<T, CH, DA, 128>(s, reverse, stream);
+    const int dc = w.walk[0].dc;
+    if (dc <= 32) return scan_aligned<T, CH, DA, 32>(w, swapped, stream);
+    if (dc <= 64) return scan_aligned<T, CH, DA, 64>(w, swapped, stream);
+    return scan_aligned<T, CH, DA, 128>(w, swapped, stream);
 }
 
-template int scan_rows<LOBPOLICY_TYPE, LOBPOLICY_ROWS>(const Scan&, bool, hipStream_t);
+template int scan_rows<LOBPOLICY_TYPE, LOBPOLICY_ROWS>(const Walks&, bool, hipStream_t);
 
 }  // namespace lobpolicy

@@ -117,9 +117,9 @@ def _describe(q, k, v, log_decay, reset, lengths, scale):
     return a
 
 
-def _workspace(a, backward, lib, device):
-    """The description's workspace -> the tensor that holds it (to be kept until the launch is made)."""
-    need = lib.check(lib.fn["attention_workspace"](C.byref(a), backward), "attention_workspace")
+def _workspace(a, lib, device):
+    """The description's workspace -> the tensor that holds it (to be kept until the launch is made), or None."""
+    need = lib.check(lib.fn["attention_workspace"](C.byref(a)), "attention_workspace")
     held = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     a.workspace, a.workspace_bytes = _ptr(held), need
     return held
@@ -132,23 +132,24 @@ def _attention_forward(q, k, v, log_decay, state, reset, lengths, scale):
     a = _describe(q, k, v, log_decay, reset, lengths, scale)
     a.out, a.state_in, a.state_out = _operand(out), _ptr(state), last.data_ptr()
     with _on(q.device) as stream:
-        held = _workspace(a, 0, lib, q.device)  # noqa: F841
+        held = _workspace(a, lib, q.device)
         lib.check(lib.fn["attention_forward"](C.byref(a), stream), "attention_forward")
-    return out, last
+    return out, last, held
 
 
 class _DecayAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, log_decay, state, reset, lengths, scale):
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(q, k, v, log_decay, state, reset, lengths)
+        out, last, held = _attention_forward(q, k, v, log_decay, state, reset, lengths, scale)
+        ctx.save_for_backward(q, k, v, log_decay, state, reset, lengths, held)
         ctx.scale = scale
-        return _attention_forward(q, k, v, log_decay, state, reset, lengths, scale)
+        return out, last
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout, dlast):
-        q, k, v, log_decay, state, reset, lengths = ctx.saved_tensors
+        q, k, v, log_decay, state, reset, lengths, forward = ctx.saved_tensors
         if dout is None and dlast is None:
             return (None,) * 8
         dout = torch.zeros(v.shape, dtype=v.dtype, device=v.device) if dout is None else _lined(dout)
@@ -160,7 +161,8 @@ class _DecayAttention(torch.autograd.Function):
         a.out, a.state_in, a.grad_state_out = _operand(dout), _ptr(state), _ptr(dlast)
         a.grad_q, a.grad_k, a.grad_v, a.grad_state_in = _operand(dq), _operand(dk), _operand(dv), _ptr(dstate)
         with _on(q.device) as stream:
-            held = _workspace(a, 1, lib, q.device)  # noqa: F841
+            held = _workspace(a, lib, q.device)  # noqa: F841
+            a.forward_workspace = _ptr(forward)
             lib.check(lib.fn["attention_backward"](C.byref(a), stream), "attention_backward")
         need = ctx.needs_input_grad
         return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, dstate, None, None, None
@@ -190,7 +192,7 @@ def decay_attention(q, k, v, log_decay, *, initial_state=None, reset=None, lengt
     args = (_lined(q), _lined(k), _lined(v), log_decay, state, reset, lengths, scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (state is not None and state.requires_grad)):
         return _DecayAttention.apply(*args)
-    return _attention_forward(*args)
+    return _attention_forward(*args)[:2]
 
 
 def decay_attention_step(q, k, v, log_decay, state, *, reset=None, skip=None, scale=None):

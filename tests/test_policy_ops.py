@@ -55,9 +55,8 @@ def test_attention_entries_refuse(wrong):
     for name in ("attention_forward", "attention_backward", "attention_step"):
         assert lib.fn[name](C.byref(a), None) == -1 and lib.fn["last_error"]()  # ({}: no operands)
     if wrong:
-        for backward in (0, 1):
-            assert lib.fn["attention_workspace"](C.byref(a), backward) == -1
-    assert lib.fn["attention_forward"](None, None) == -1 and lib.fn["attention_workspace"](None, 0) == -1
+        assert lib.fn["attention_workspace"](C.byref(a)) == -1
+    assert lib.fn["attention_forward"](None, None) == -1 and lib.fn["attention_workspace"](None) == -1
     with pytest.raises(_capi.LobsimError, match="attention_forward"):
         lib.check(lib.fn["attention_forward"](None, None), "attention_forward")
 

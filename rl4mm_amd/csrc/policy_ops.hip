@@ -412,7 +412,7 @@ __global__ __launch_bounds__(1024) void column_sums(const float* partial, int pa
     }
 }
 
-constexpr int64_t BLOCK_PARTS = 512;
+constexpr int64_t BLOCK_PARTS = 1024;
 
 int block_rows(int64_t width) { return width <= 1024 ? 4 : 1; }  // rows a workgroup holds at once
 int64_t block_parts(const lobpolicy_block* b) {
@@ -486,7 +486,7 @@ Block block_of(const lobpolicy_block* b) {
 
 constexpr int CLIP_TENSORS = 128;        // per launch: 3 KB of arguments
 constexpr int64_t CLIP_CHUNK = 8192;     // elements
-constexpr int64_t CLIP_PARTS = 1024;     // workgroups per launch, at most
+constexpr int64_t CLIP_PARTS = 2048;     // workgroups per launch, at most
 
 struct ClipTable {
     void* data[CLIP_TENSORS];
@@ -577,7 +577,9 @@ __global__ __launch_bounds__(256) void clip_kernel(ClipTable t, const double* pa
     const double ratio = max_norm / (norm + 1e-6);
     const float by = ratio > 1.0 ? 1.f : (float)ratio;  // (not a number stays one)
     if (by == 1.f) return;  // times one: the elements stay as they are
-    for (uint32_t chunk = blockIdx.x; chunk < t.first[t.n]; chunk += gridDim.x) {
+    // backwards: what the first pass read last is what the caches still hold
+    for (uint32_t back = blockIdx.x; back < t.first[t.n]; back += gridDim.x) {
+        const uint32_t chunk = t.first[t.n] - 1 - back;
         const int i = find_tensor(t, chunk);
         auto go = [&](auto* data) {
             using T = std::remove_pointer_t<decltype(data)>;

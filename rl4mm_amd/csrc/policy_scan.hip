@@ -252,14 +252,6 @@ __device__ __forceinline__ void walk_part(const Scan& s, int64_t unit, int64_t p
         if (k < CH) leave[CH - 1 - k] = x * s.in_scale;
     }
     if (threadIdx.x < 2) spoiled[threadIdx.x] = 0;
-    float w_diagonal[4], w_below[4];  // of a score tile on the diagonal, and of the one below it
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int gap = at.l - 4 * at.g - r;
-        w_diagonal[r] = gap >= 0 ? decay_of(gap) * s.in_scale * s.out_scale : 0.f;
-        w_below[r] = decay_of(16 + gap) * s.in_scale * s.out_scale;
-    }
-
     Moving<T, CH, DA, S::THREADS, VEC> move_a, move_b;
     Moving<T, CH, DC, S::THREADS, VEC> move_c;
     uint32_t flag = 0;
@@ -295,6 +287,15 @@ __device__ __forceinline__ void walk_part(const Scan& s, int64_t unit, int64_t p
     for (int ct = 0; ct < S::COLS; ++ct)
 #pragma unroll
         for (int t = 0; t < DT; ++t) asm volatile("" : "+v"(state[ct][t]));
+
+    __syncthreads();
+    float w_diagonal[4], w_below[4];  // of a score tile on the diagonal, and of the one below it
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int gap = at.l - 4 * at.g - r;
+        w_diagonal[r] = gap >= 0 ? enter[gap >= 0 ? gap : 0] * s.in_scale : 0.f;
+        w_below[r] = enter[16 + gap] * s.in_scale;
+    }
 
     int parity = 0;
     uint64_t any_cut = 0;

@@ -23,8 +23,11 @@ _DTYPES = {torch.float32: capi.F32, torch.bfloat16: capi.BF16}
 _NONE = capi.Operand(None, 0, 0, 0)
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream  # torch.cuda.current_stream(index).cuda_stream without the object around it
+
+
 class _on:
-    """The raw current stream of `device`, with that device current inside the block."""
+    """The raw current stream of a device, with that device current inside the block."""
 
     __slots__ = ("index", "before")
 
@@ -35,11 +38,16 @@ class _on:
         self.before = torch.cuda.current_device()
         if self.before != self.index:
             torch.cuda.set_device(self.index)
-        return torch.cuda.current_stream(self.index).cuda_stream
+        return _raw_stream(self.index)
 
     def __exit__(self, *exc):
         if self.before != self.index:
             torch.cuda.set_device(self.before)
+
+
+def _new(t):
+    """An empty tensor of t's shape and type, without gaps."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _need(ok, message, kind=ValueError):
@@ -66,7 +74,8 @@ def _lined(t):
 
 
 def _operand(t):  # [T, N, H, D] or [N, H, D]
-    return capi.Operand(t.data_ptr(), *t.stride()[:3]) if t.dim() == 4 else capi.Operand(t.data_ptr(), 0, *t.stride()[:2])
+    st = t.stride()
+    return capi.Operand(t.data_ptr(), st[0], st[1], st[2]) if len(st) == 4 else capi.Operand(t.data_ptr(), 0, st[0], st[1])
 
 
 def _ptr(t):
@@ -81,28 +90,42 @@ def _changed(tensors):
 
 
 def _flags(t, name, shape, device):
-    if t is None:
-        return None
+    if t is None or (type(t) is torch.Tensor and t.dtype is torch.bool and t.device == device and t.shape == shape and t.layout is torch.strided):
+        return t
     _tensor(t, name, (torch.bool, torch.uint8), device, shape)
     return t
 
 
 def _heads(q, k, v, log_decay, state, scale, dims):
     """Checks what the two forms have in common -> (log_decay, scale)."""
-    _tensor(q, "q", _DTYPES)
-    _need(q.dim() == len(dims), f"q is [{', '.join(dims)}], got {tuple(q.shape)}")
-    _tensor(k, "k", (q.dtype,), q.device, q.shape)
-    _tensor(v, "v", (q.dtype,), q.device)
-    _need(v.shape[:-1] == q.shape[:-1], f"v is [{', '.join(dims[:-1])}, dv] beside q {tuple(q.shape)}, got {tuple(v.shape)}")
-    heads, dk, dv = q.shape[-2], q.shape[-1], v.shape[-1]
-    _need(heads >= 1 and 1 <= dk <= capi.MAX_HEAD and 1 <= dv <= capi.MAX_HEAD, f"{heads} heads of dk = {dk} and dv = {dv}: one head or more, dk and dv 1 to {capi.MAX_HEAD}")
-    _tensor(log_decay, "log_decay", (torch.float32,), q.device, (heads,))
-    _need(not log_decay.requires_grad, "log_decay takes no gradient: the decays are constants of the policy")
-    if state is not None:
-        _tensor(state, "the state", (torch.float32,), q.device, (q.shape[-3], heads, dk, dv))
+    try:  # one look at all of it; what is wrong is found out below
+        device, shape = q.device, q.shape
+        heads, dk, dv = shape[-2], shape[-1], v.shape[-1]
+        fine = (
+            q.is_cuda and q.dtype in _DTYPES and q.layout is torch.strided and len(shape) == len(dims) and heads >= 1 and 1 <= dk <= capi.MAX_HEAD and 1 <= dv <= capi.MAX_HEAD
+            and k.dtype is q.dtype and k.device == device and k.shape == shape and k.layout is torch.strided
+            and v.dtype is q.dtype and v.device == device and v.shape[:-1] == shape[:-1] and v.layout is torch.strided
+            and log_decay.dtype is torch.float32 and log_decay.device == device and log_decay.shape == (heads,) and log_decay.is_contiguous() and not log_decay.requires_grad
+            and (state is None or (state.dtype is torch.float32 and state.device == device and state.shape == (shape[-3], heads, dk, dv) and state.layout is torch.strided))
+        )  # fmt: skip
+    except (AttributeError, IndexError, TypeError):
+        fine = False
+    if not fine:
+        _tensor(q, "q", _DTYPES)
+        _need(q.dim() == len(dims), f"q is [{', '.join(dims)}], got {tuple(q.shape)}")
+        _tensor(k, "k", (q.dtype,), q.device, q.shape)
+        _tensor(v, "v", (q.dtype,), q.device)
+        _need(v.shape[:-1] == q.shape[:-1], f"v is [{', '.join(dims[:-1])}, dv] beside q {tuple(q.shape)}, got {tuple(v.shape)}")
+        heads, dk, dv = q.shape[-2], q.shape[-1], v.shape[-1]
+        _need(heads >= 1 and 1 <= dk <= capi.MAX_HEAD and 1 <= dv <= capi.MAX_HEAD, f"{heads} heads of dk = {dk} and dv = {dv}: one head or more, dk and dv 1 to {capi.MAX_HEAD}")
+        _tensor(log_decay, "log_decay", (torch.float32,), q.device, (heads,))
+        _need(not log_decay.requires_grad, "log_decay takes no gradient: the decays are constants of the policy")
+        if state is not None:
+            _tensor(state, "the state", (torch.float32,), q.device, (q.shape[-3], heads, dk, dv))
+        log_decay = log_decay.contiguous()
     scale = dk**-0.5 if scale is None else float(scale)
-    _need(math.isfinite(scale), f"scale = {scale}")
-    return log_decay.contiguous(), scale
+    _need(math.isfinite(scale), "the scale is not finite")
+    return log_decay, scale
 
 
 def _describe(q, k, v, log_decay, reset, lengths, scale):
@@ -113,7 +136,8 @@ def _describe(q, k, v, log_decay, reset, lengths, scale):
     if reset is not None:
         a.reset = reset.data_ptr()
         a.reset_stride_t, a.reset_stride_n = reset.stride() if reset.dim() == 2 else (0, reset.stride(0))
-    a.lengths = _ptr(lengths)
+    if lengths is not None:
+        a.lengths = lengths.data_ptr()
     return a
 
 
@@ -126,7 +150,7 @@ def _workspace(a, lib, device):
 
 
 def _attention_forward(q, k, v, log_decay, state, reset, lengths, scale):
-    out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+    out = _new(v)
     last = torch.empty((q.shape[1], q.shape[2], q.shape[3], v.shape[3]), dtype=torch.float32, device=q.device)
     lib = _lib.policy_binding()
     a = _describe(q, k, v, log_decay, reset, lengths, scale)
@@ -154,8 +178,8 @@ class _DecayAttention(torch.autograd.Function):
             return (None,) * 8
         dout = torch.zeros(v.shape, dtype=v.dtype, device=v.device) if dout is None else _lined(dout)
         dlast = None if dlast is None else dlast.contiguous()
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        dstate = torch.empty(state.shape, dtype=torch.float32, device=q.device) if ctx.needs_input_grad[4] else None
+        dq, dk, dv = _new(q), _new(k), _new(v)
+        dstate = _new(state) if ctx.needs_input_grad[4] else None
         lib = _lib.policy_binding()
         a = _describe(q, k, v, log_decay, reset, lengths, ctx.scale)
         a.out, a.state_in, a.grad_state_out = _operand(dout), _ptr(state), _ptr(dlast)
@@ -207,7 +231,7 @@ def decay_attention_step(q, k, v, log_decay, state, *, reset=None, skip=None, sc
     _need(not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad)),
           "decay_attention_step has no gradient: call it under torch.no_grad(), or decay_attention for the gradients")  # fmt: skip
     reset, skip = _flags(reset, "reset", q.shape[:1], q.device), _flags(skip, "skip", q.shape[:1], q.device)
-    out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+    out = _new(v)
     if q.shape[0] == 0:
         return out
     q, k, v = _lined(q), _lined(k), _lined(v)
@@ -240,7 +264,7 @@ def _describe_block(x, block, gate, post, res, pre, eps):
 
 
 def _block_forward(x, block, gate, post, res, pre, eps):
-    y, z = torch.empty(x.shape, dtype=x.dtype, device=x.device), torch.empty(x.shape, dtype=block.dtype, device=x.device)
+    y, z = _new(x), _new(block)
     lib = _lib.policy_binding()
     b = _describe_block(x, block, gate, post, res, pre, eps)
     b.y, b.z = y.data_ptr(), z.data_ptr()
@@ -264,9 +288,9 @@ class _GatedResidualNorm(torch.autograd.Function):
         if dy is None and dz is None:
             return (None,) * 7
         dy, dz = (None if d is None else _lined(d) for d in (dy, dz))
-        dx, dblock = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (x, block))
-        dgate = None if gate is None else torch.empty_like(dblock)
-        dpost, dres, dpre = torch.empty((3, x.shape[1]), dtype=torch.float32, device=x.device)
+        dx, dblock = _new(x), _new(block)
+        dgate = None if gate is None else _new(block)
+        dpost, dres, dpre = _new(post), _new(res), _new(pre)
         lib = _lib.policy_binding()
         b = _describe_block(x, block, gate, post, res, pre, ctx.eps)
         b.grad_y, b.grad_z = _ptr(dy), _ptr(dz)
@@ -289,18 +313,30 @@ def gated_residual_norm(x, block, gate, post_weight, residual_scale, pre_weight,
     x: the residual stream, float32 or bfloat16, y its type.  block: what the block put out; gate: its gate's logits (None: no gate); z has their type,
     float32 or bfloat16, and is taken from y before that is rounded.  The three weights: float32 [width].  width: 1 to 8192; rows of any stride.
     Differentiable in all six; the weights' gradients are summed in a fixed order."""
-    _tensor(x, "x", _DTYPES)
-    _need(x.dim() >= 1, "x is [..., width], got a single number")
-    width = x.shape[-1]
-    _need(1 <= width <= capi.MAX_WIDTH, f"width = {width}: 1 to {capi.MAX_WIDTH}")
-    _tensor(block, "block", _DTYPES, x.device, x.shape)
-    if gate is not None:
-        _tensor(gate, "gate", (block.dtype,), x.device, x.shape)
     weights = (post_weight, residual_scale, pre_weight)
-    for t, name in zip(weights, ("post_weight", "residual_scale", "pre_weight")):
-        _tensor(t, name, (torch.float32,), x.device, (width,))
+    try:  # one look at all of it; what is wrong is found out below
+        device, shape = x.device, x.shape
+        width = shape[-1]
+        fine = (
+            x.is_cuda and x.dtype in _DTYPES and x.layout is torch.strided and 1 <= width <= capi.MAX_WIDTH
+            and block.dtype in _DTYPES and block.device == device and block.shape == shape and block.layout is torch.strided
+            and (gate is None or (gate.dtype is block.dtype and gate.device == device and gate.shape == shape and gate.layout is torch.strided))
+            and all(w.dtype is torch.float32 and w.device == device and w.shape == (width,) for w in weights)
+        )  # fmt: skip
+    except (AttributeError, IndexError, TypeError):
+        fine = False
+    if not fine:
+        _tensor(x, "x", _DTYPES)
+        _need(x.dim() >= 1, "x is [..., width], got a single number")
+        width = x.shape[-1]
+        _need(1 <= width <= capi.MAX_WIDTH, f"width = {width}: 1 to {capi.MAX_WIDTH}")
+        _tensor(block, "block", _DTYPES, x.device, x.shape)
+        if gate is not None:
+            _tensor(gate, "gate", (block.dtype,), x.device, x.shape)
+        for t, name in zip(weights, ("post_weight", "residual_scale", "pre_weight")):
+            _tensor(t, name, (torch.float32,), x.device, (width,))
     eps = float(eps)
-    _need(math.isfinite(eps) and eps > 0.0, f"eps = {eps}")
+    _need(math.isfinite(eps) and eps > 0.0, "eps is a positive number")
     shape, wanted = x.shape, torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, block, gate, *weights))
     rows = [_rows(t, width) if t is not None else None for t in (x, block, gate)]
     if x.numel() == 0:  # (nothing to compute, and the gradients are zeros: torch's own operations say so)
@@ -342,11 +378,13 @@ def clip_grad_norm(grads, max_norm, norm_type=2.0):
         return torch.zeros(())
     device, spans = getattr(grads[0], "device", None), []
     for i, g in enumerate(grads):
-        _tensor(g, f"gradient {i}", _DTYPES, device)
-        _need(not g.requires_grad, f"gradient {i} requires a gradient itself: it is scaled outside autograd (detach it)")
-        _need(_dense(g), f"gradient {i} is not dense in memory (shape {tuple(g.shape)}, strides {g.stride()}): it could not be scaled in place")
-        if g.numel():
-            spans.append((g.data_ptr(), g.numel() * g.element_size(), i))
+        if not (type(g) is torch.Tensor and g.dtype in _DTYPES and g.device == device and g.is_cuda and not g.requires_grad and g.is_contiguous()):
+            _tensor(g, f"gradient {i}", _DTYPES, device)
+            _need(not g.requires_grad, f"gradient {i} requires a gradient itself: it is scaled outside autograd (detach it)")
+            _need(_dense(g), f"gradient {i} is not dense in memory (shape {tuple(g.shape)}, strides {g.stride()}): it could not be scaled in place")
+        count = g.numel()
+        if count:
+            spans.append((g.data_ptr(), count * g.itemsize, i))
     spans.sort()
     for (p, size, i), (q, _, j) in zip(spans, spans[1:]):
         _need(p + size <= q, f"gradients {min(i, j)} and {max(i, j)} share memory: each element is counted and scaled once")

@@ -32,14 +32,50 @@ def policy_of(agent, action_dim: int, n_envs: int, n_steps: int):
     raise TypeError(f"no device policy for {type(agent).__name__}: step the env from the host (HistoricalOrderbookVectorEnv.vector_step)")
 
 
+def _policy_trajectories(policy, venv, T: int) -> Dict[str, np.ndarray]:
+    """The episode of a SequencePolicy: its memory and actions on the device, one env step per action (T = 1 launches, whose trace row goes into the series)."""
+    import torch
+
+    sim, n = venv.sim, venv.num_envs
+    t = venv._tensors()
+    dev = t["dev"]
+    obs = venv.vector_reset_tensors().double()
+    memory = policy.memory(n)
+    row = torch.empty((1, n, _capi.TRACE_DIM), dtype=torch.float64, device=dev)
+    trace = torch.empty((T, n, _capi.TRACE_DIM), dtype=torch.float64, device=dev)
+    reward, done = torch.zeros(n, dtype=torch.float64, device=dev), torch.zeros(n, dtype=torch.uint8, device=dev)
+    steps = torch.zeros(n, dtype=torch.int32, device=dev)
+    sim.set_trace_buffer(row.data_ptr(), 1)
+    try:
+        for k in range(T):
+            active = (done == 0).to(torch.uint8)
+            actions = policy.act(obs, memory, skip=done)
+            row.fill_(float("nan"))  # (an env that does not step, or whose step ends with a status bit, writes none)
+            cur, target = venv._bind_stream(t)
+            sim.rollout_device(_capi.POLICY_GIVEN, [], 1, actions.data_ptr(), active.data_ptr(), obs.data_ptr(), 0, reward.data_ptr(), done.data_ptr())
+            if target is not cur:
+                cur.wait_stream(target)
+            trace[k] = row[0]
+            steps += active
+        torch.cuda.synchronize(dev)
+    finally:
+        sim.set_trace_buffer(0, 0)
+    venv._dones[:] = done.cpu().numpy().astype(bool)
+    venv._any_done = bool(venv._dones.any())
+    return dict(steps=steps.cpu().numpy(), trace=trace.cpu().numpy(), observations=obs.cpu().numpy(), rewards=reward.cpu().numpy(), dones=done.cpu().numpy().astype(bool))
+
+
 def generate_trajectories(agent, venv, n_steps: Optional[int] = None) -> Dict[str, np.ndarray]:
-    """One episode of every env of ``venv`` (HistoricalOrderbookVectorEnv) under ``agent``, in one launch.
+    """One episode of every env of ``venv`` (HistoricalOrderbookVectorEnv) under ``agent``: in one launch for the rule-based agents, step by step on the
+    device for a ``policy.SequencePolicy``.
     -> dict(steps [N], trace [T, N, TRACE_DIM], final observation / reward / done).  Trace rows beyond an env's steps are NaN; so
     is the row of a step that ended with a status bit (counted in `steps`, where the reference would have raised)."""
     import torch
 
     sim, n = venv.sim, venv.num_envs
     T = int(n_steps or round(venv.episode_length / venv.step_size))
+    if hasattr(agent, "memory") and hasattr(agent, "act"):  # (a SequencePolicy: its module needs torch)
+        return _policy_trajectories(agent, venv, T)
     venv.vector_reset()
     policy, params, acts = policy_of(agent, sim.action_dim, n, T)
     dev = torch.device("cuda", sim.cfg.device_id)

@@ -240,7 +240,11 @@ __device__ __forceinline__ void row_sums(float* v, int count, float* shared) {
         if (threadIdx.x % 64 == 0)
             for (int i = 0; i < count; ++i) shared[(threadIdx.x / 64) * 2 + i] = v[i];
         __syncthreads();
-        for (int i = 0; i < count; ++i) v[i] = shared[i] + shared[2 + i] + shared[4 + i] + shared[6 + i];
+        for (int i = 0; i < count; ++i) {
+            v[i] = 0.f;
+#pragma unroll
+            for (int k = 0; k < TPR / 64; ++k) v[i] += shared[2 * k + i];
+        }
     }
 }
 
@@ -266,13 +270,44 @@ __device__ __forceinline__ void store_row(T* row, int width, int lane, const flo
     }
 }
 
-__device__ __forceinline__ float sigmoid(float u) { return 1.f / (1.f + expf(-u)); }
+// one instruction each for 2^x and 1 / x, both within a step of their type: off by about (1 + |u|) 2^-23 of its value
+__device__ __forceinline__ float sigmoid(float u) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * u)); }
+
+// A row as it lies in memory, in registers; numbers are converted where they are used, so that the next row fits beside this one
+template <class T, int VW, int E, int TPR>
+struct RawRow {
+    Pack<T, VW> x[E / VW];
+    __device__ __forceinline__ void load(const T* row, int width, int lane) {
+#pragma unroll
+        for (int s = 0; s < E / VW; ++s) {
+            const int col = (s * TPR + lane) * VW;
+            if (row && col < width)
+                x[s] = *reinterpret_cast<const Pack<T, VW>*>(row + col);
+            else
+#pragma unroll
+                for (int i = 0; i < VW; ++i) x[s].v[i] = (T)0.f;
+        }
+    }
+    __device__ __forceinline__ float operator[](int i) const { return (float)x[i / VW].v[i % VW]; }
+    __device__ __forceinline__ void again() {  // (the compiler is to convert once more, rather than keep the numbers converted)
+        if constexpr (sizeof(T) == 2 && VW % 2 == 0)
+#pragma unroll
+            for (int s = 0; s < E / VW; ++s) {
+                typedef uint32_t words __attribute__((ext_vector_type(VW / 2)));
+                words w = __builtin_bit_cast(words, x[s]);
+                asm volatile("" : "+v"(w));
+                x[s] = __builtin_bit_cast(Pack<T, VW>, w);
+            }
+    }
+};
 
 template <class X, class B, int VW, int E, int TPR>
-__global__ __launch_bounds__(256) void block_forward_kernel(Block p) {
-    __shared__ float shared[8];
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void block_forward_kernel(Block p) {
+    __shared__ float shared[TPR > 64 ? TPR / 32 : 1];
+    constexpr int RPB = TPR > 256 ? 1 : 256 / TPR;
     const int lane = threadIdx.x % TPR;
-    for (int64_t row = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR; row < p.rows; row += (int64_t)gridDim.x * (256 / TPR)) {
+    const float share = 1.f / p.width;
+    for (int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR; row < p.rows; row += (int64_t)gridDim.x * RPB) {
         float x[E], b[E], g[E], w[E];
         load_row<X, VW, E, TPR>((const X*)p.x + row * p.x_sr, p.width, lane, x);
         load_row<B, VW, E, TPR>((const B*)p.block + row * p.block_sr, p.width, lane, b);
@@ -281,7 +316,7 @@ __global__ __launch_bounds__(256) void block_forward_kernel(Block p) {
 #pragma unroll
         for (int i = 0; i < E; ++i) sum += b[i] * b[i];
         row_sums<TPR>(&sum, 1, shared);
-        const float rb = 1.f / sqrtf(sum / p.width + p.eps);
+        const float rb = 1.f / sqrtf(sum * share + p.eps);
 #pragma unroll
         for (int i = 0; i < E; ++i) b[i] *= rb * (p.gate ? sigmoid(g[i]) : 1.f);
         load_row<float, VW, E, TPR>(p.post, p.width, lane, w);
@@ -294,7 +329,7 @@ __global__ __launch_bounds__(256) void block_forward_kernel(Block p) {
         }
         store_row<X, VW, E, TPR>((X*)p.y + row * p.width, p.width, lane, x);
         row_sums<TPR>(&sum, 1, shared);
-        const float ry = 1.f / sqrtf(sum / p.width + p.eps);
+        const float ry = 1.f / sqrtf(sum * share + p.eps);
         load_row<float, VW, E, TPR>(p.pre, p.width, lane, w);
 #pragma unroll
         for (int i = 0; i < E; ++i) x[i] = x[i] * ry * w[i];
@@ -309,66 +344,76 @@ __global__ __launch_bounds__(256) void block_forward_kernel(Block p) {
 // y is worked out again from x, b and the gate, which costs no memory.  A workgroup keeps its share of the two column sums in registers
 // over all its rows and writes it once; column_sums adds the workgroups' shares in their order.
 template <class X, class B, int VW, int E, int TPR>
-__global__ __launch_bounds__(256) void block_backward_kernel(Block p) {
-    constexpr int RPB = 256 / TPR;
-    __shared__ float shared[8];
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void block_backward_kernel(Block p) {
+    constexpr int RPB = TPR > 256 ? 1 : 256 / TPR;
+    __shared__ float shared[TPR > 64 ? TPR / 32 : 1];
     __shared__ float fold[TPR == 64 ? 4 * 64 * E : 1];
     const int lane = threadIdx.x % TPR;
+    const float share = 1.f / p.width;
     float sum_m[E], sum_p[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) sum_m[i] = sum_p[i] = 0.f;
-    for (int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR; row < p.rows; row += (int64_t)gridDim.x * RPB) {
-        float x[E], b[E], g[E], dy[E], dz[E], w[E], sums[2];
-        load_row<X, VW, E, TPR>((const X*)p.x + row * p.x_sr, p.width, lane, x);
-        load_row<B, VW, E, TPR>((const B*)p.block + row * p.block_sr, p.width, lane, b);
-        load_row<B, VW, E, TPR>(p.gate ? (const B*)p.gate + row * p.gate_sr : nullptr, p.width, lane, g);
-        load_row<X, VW, E, TPR>(p.grad_y ? (const X*)p.grad_y + row * p.grad_y_sr : nullptr, p.width, lane, dy);
-        load_row<B, VW, E, TPR>(p.grad_z ? (const B*)p.grad_z + row * p.grad_z_sr : nullptr, p.width, lane, dz);
-        sums[0] = 0.f;
+    struct Rows5 {
+        RawRow<X, VW, E, TPR> x, dy;
+        RawRow<B, VW, E, TPR> b, g, dz;
+    } now, next;
+    auto load = [&](Rows5& r, int64_t row) {
+        r.x.load((const X*)p.x + row * p.x_sr, p.width, lane);
+        r.b.load((const B*)p.block + row * p.block_sr, p.width, lane);
+        r.g.load(p.gate ? (const B*)p.gate + row * p.gate_sr : nullptr, p.width, lane);
+        r.dy.load(p.grad_y ? (const X*)p.grad_y + row * p.grad_y_sr : nullptr, p.width, lane);
+        r.dz.load(p.grad_z ? (const B*)p.grad_z + row * p.grad_z_sr : nullptr, p.width, lane);
+    };
+    const int64_t first = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR, step = (int64_t)gridDim.x * RPB;
+    if (first < p.rows) load(next, first);
+    for (int64_t row = first; row < p.rows; row += step) {
+        now = next;
+        if (row + step < p.rows) load(next, row + step);
+        float sums[2] = {0.f, 0.f}, y[E], sg[E], w[E], r[E];
 #pragma unroll
-        for (int i = 0; i < E; ++i) sums[0] += b[i] * b[i];
+        for (int i = 0; i < E; ++i) sums[0] += now.b[i] * now.b[i];
         row_sums<TPR>(sums, 1, shared);
-        const float rb = 1.f / sqrtf(sums[0] / p.width + p.eps);
+        const float rb = 1.f / sqrtf(sums[0] * share + p.eps);
+        now.b.again();
         load_row<float, VW, E, TPR>(p.post, p.width, lane, w);
-        float r[E];
         load_row<float, VW, E, TPR>(p.res, p.width, lane, r);
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-            b[i] *= rb;
-            g[i] = p.gate ? sigmoid(g[i]) : 1.f;
+            sg[i] = p.gate ? sigmoid(now.g[i]) : 1.f;
             w[i] *= r[i];
-            x[i] += w[i] * (g[i] * b[i]);
+            y[i] = now.x[i] + w[i] * (sg[i] * (now.b[i] * rb));
         }
         load_row<float, VW, E, TPR>(p.pre, p.width, lane, r);
-        sums[0] = sums[1] = 0.f;
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-            sums[0] += x[i] * x[i];
-            sums[1] += x[i] * (dz[i] * r[i]);
-        }
-        row_sums<TPR>(sums, 2, shared);
-        const float ry = 1.f / sqrtf(sums[0] / p.width + p.eps), mean = sums[1] * ry / p.width;
         sums[0] = 0.f;
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-            const float yn = x[i] * ry;
-            sum_p[i] += dz[i] * yn;
-            dy[i] += ry * (dz[i] * r[i] - yn * mean);
-            sum_m[i] += dy[i] * (g[i] * b[i]);
-            r[i] = dy[i] * w[i];  // f res post
-            sums[0] += r[i] * g[i] * b[i];
+            sums[0] += y[i] * y[i];
+            sums[1] += y[i] * (now.dz[i] * r[i]);
         }
-        store_row<X, VW, E, TPR>((X*)p.grad_x + row * p.width, p.width, lane, dy);
+        row_sums<TPR>(sums, 2, shared);
+        const float ry = 1.f / sqrtf(sums[0] * share + p.eps), mean = sums[1] * ry * share;
+        now.b.again(), now.dz.again();
+        sums[0] = 0.f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {  // y becomes f
+            const float yn = y[i] * ry, bn = now.b[i] * rb;
+            sum_p[i] += now.dz[i] * yn;
+            y[i] = now.dy[i] + ry * (now.dz[i] * r[i] - yn * mean);
+            sum_m[i] += y[i] * (sg[i] * bn);
+            sums[0] += y[i] * w[i] * sg[i] * bn;
+        }
+        store_row<X, VW, E, TPR>((X*)p.grad_x + row * p.width, p.width, lane, y);
         row_sums<TPR>(sums, 1, shared);
-        const float back = sums[0] / p.width;
-        if (p.gate) {
+        const float back = sums[0] * share;
+        now.b.again();
 #pragma unroll
-            for (int i = 0; i < E; ++i) x[i] = r[i] * b[i] * (g[i] * (1.f - g[i]));
-            store_row<B, VW, E, TPR>((B*)p.grad_gate + row * p.width, p.width, lane, x);
+        for (int i = 0; i < E; ++i) {
+            const float bn = now.b[i] * rb, e = y[i] * w[i];
+            y[i] = rb * (e * sg[i] - bn * back);
+            sg[i] = e * bn * (sg[i] * (1.f - sg[i]));
         }
-#pragma unroll
-        for (int i = 0; i < E; ++i) x[i] = rb * (r[i] * g[i] - b[i] * back);
-        store_row<B, VW, E, TPR>((B*)p.grad_block + row * p.width, p.width, lane, x);
+        store_row<B, VW, E, TPR>((B*)p.grad_block + row * p.width, p.width, lane, y);
+        if (p.gate) store_row<B, VW, E, TPR>((B*)p.grad_gate + row * p.width, p.width, lane, sg);
     }
     float* to = p.partial + (int64_t)blockIdx.x * p.width;
     const int64_t second = (int64_t)gridDim.x * p.width;
@@ -412,7 +457,7 @@ __global__ __launch_bounds__(1024) void column_sums(const float* partial, int pa
     }
 }
 
-constexpr int64_t BLOCK_PARTS = 1024;
+constexpr int64_t BLOCK_PARTS = 512;
 
 int block_rows(int64_t width) { return width <= 1024 ? 4 : 1; }  // rows a workgroup holds at once
 int64_t block_parts(const lobpolicy_block* b) {
@@ -422,11 +467,12 @@ int64_t block_parts(const lobpolicy_block* b) {
 
 template <class X, class B, int VW, int E, int TPR>
 int block_launch(const Block& p, bool backward, int64_t parts, hipStream_t stream) {
-    const int64_t groups = ceil_div(p.rows, 256 / TPR);
+    constexpr int threads = TPR > 256 ? TPR : 256;
+    const int64_t groups = ceil_div(p.rows, threads / TPR);
     if (backward)
-        block_backward_kernel<X, B, VW, E, TPR><<<dim3((unsigned)parts), 256, 0, stream>>>(p);
+        block_backward_kernel<X, B, VW, E, TPR><<<dim3((unsigned)parts), threads, 0, stream>>>(p);
     else
-        block_forward_kernel<X, B, VW, E, TPR><<<dim3((unsigned)(groups < (1 << 20) ? groups : (1 << 20))), 256, 0, stream>>>(p);
+        block_forward_kernel<X, B, VW, E, TPR><<<dim3((unsigned)(groups < (1 << 20) ? groups : (1 << 20))), threads, 0, stream>>>(p);
     return launched();
 }
 
@@ -436,7 +482,7 @@ int block_wide(const Block& p, bool backward, int64_t parts, hipStream_t stream)
     if (p.width <= 64 * LEAST) return block_launch<X, B, VW, LEAST, 64>(p, backward, parts, stream);
     if (p.width <= 1024) return block_launch<X, B, VW, 16, 64>(p, backward, parts, stream);
     if (p.width <= 2048) return block_launch<X, B, VW, 8, 256>(p, backward, parts, stream);
-    return block_launch<X, B, VW, 32, 256>(p, backward, parts, stream);
+    return block_launch<X, B, VW, 8, 1024>(p, backward, parts, stream);
 }
 
 template <class X, class B>

@@ -121,7 +121,6 @@ struct Shape {
     static constexpr int COLS = DC == 128 ? 2 : 1;  // tiles of 16 of the state's columns to a wave
     static constexpr int WAVES = DC / 16 / COLS, THREADS = 64 * WAVES;
     static constexpr int LEAST_WAVES = DA <= 64 && DC <= 64 ? 3 : 2;  // per SIMD: bounds the registers
-    static constexpr bool AHEAD = DA + DC < 256;  // whether the next chunk is on its way while one is computed
     static constexpr int PAD = Tile<T>::PAD, SA = DA + PAD, SC = DC + PAD, SP = CH + PAD;
 };
 
@@ -222,6 +221,7 @@ __device__ __forceinline__ void walk_part(const Scan& s, int64_t unit, int64_t p
     typedef Shape<T, CH, DA, DC> S;
     typedef Tile<T> M;
     typedef typename M::Frag Frag;
+    constexpr bool AHEAD = !OUT || DA + DC < 256;  // whether the next chunk is on its way while one is computed: not where the registers end
     constexpr int KA = DA / M::K, KC = CH / M::K, DT = DA / 16, PER = M::K / 16;
     T *const tile_a = room.a, *const tile_b = room.b, *const tile_c = room.c, *const tile_p = room.p;
     float *const power = room.power, *const enter = room.enter, *const leave = room.leave;
@@ -265,7 +265,7 @@ __device__ __forceinline__ void walk_part(const Scan& s, int64_t unit, int64_t p
         move_c.load(places);
         flag = load_flag(first);
     };
-    if (S::AHEAD && begin < end) load(begin);
+    if (AHEAD && begin < end) load(begin);
 
     const int64_t matrix = (int64_t)s.da * s.dc, which = s.parts == 1 ? unit : unit * s.parts + part;
     f32x4 state[S::COLS][DT];  // rows 16 t + 4 g + r, column `column` + 16 ct + l
@@ -302,7 +302,7 @@ __device__ __forceinline__ void walk_part(const Scan& s, int64_t unit, int64_t p
     for (int64_t first = begin; first < end; first += CH, parity ^= 1) {
         at.fresh();
         const int places = end - first < CH ? (int)(end - first) : CH;
-        if (!S::AHEAD) load(first);
+        if (!AHEAD) load(first);
         if (OUT) move_a.store(tile_a, S::SA, places);
         move_b.store(tile_b, S::SA, places);
         move_c.store(tile_c, S::SC, places);
@@ -311,7 +311,7 @@ __device__ __forceinline__ void walk_part(const Scan& s, int64_t unit, int64_t p
         // (without outputs only a cut can take away what is not finite)
         if (!OUT && cuts && ((move_b.bad() | move_c.bad()) & NOT_FINITE<T>)) spoiled[parity] = 1;
         __syncthreads();
-        if (S::AHEAD && first + CH < end) load(first + CH);
+        if (AHEAD && first + CH < end) load(first + CH);
         const int enters = reverse && first == 0 ? 0 : 1;  // decays between what comes into the chunk and its first place
         const int tiles = (places + 15) / 16;
         Frag values[S::COLS][KC];  // c, by columns

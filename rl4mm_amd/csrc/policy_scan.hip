@@ -229,10 +229,10 @@ __device__ __forceinline__ void walk_part(const Scan& s, int64_t unit, int64_t p
     const bool reverse = s.reverse;
     const int64_t n = (uint32_t)unit / (uint32_t)s.heads;
     const int h = (int)((uint32_t)unit % (uint32_t)s.heads);
-    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, column = wave * S::COLS * 16;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, column = wave * S::COLS * 16;
     Lane at = {lane % 16, lane / 16};
 
-    const int64_t length = length_of(s, n), begin = part * s.part_steps;
+    const int64_t length = __builtin_amdgcn_readfirstlane((int)length_of(s, n)), begin = part * s.part_steps;
     const int64_t end = begin + s.part_steps < length ? begin + s.part_steps : length;
     const int64_t first_token = reverse ? length - 1 - begin : begin;
     T* out = OUT ? (T*)s.out.data + n * s.out.sn + h * s.out.sh : nullptr;
@@ -366,7 +366,7 @@ __device__ __forceinline__ void walk_part(const Scan& s, int64_t unit, int64_t p
             if (spoils != 0.f) spoiled[parity] = 1;
             __syncthreads();
         }
-        bool by_token = spoiled[parity] != 0;
+        bool by_token = __builtin_amdgcn_readfirstlane(spoiled[parity]) != 0;
         if (threadIdx.x == 0) spoiled[parity ^ 1] = 0;
         auto token = [&](int p) { return (reverse ? length - 1 - (first + p) : first + p) * s.out.st; };
 

@@ -244,14 +244,6 @@ __device__ __forceinline__ void walk_part(const Scan& s, int64_t unit, int64_t p
     auto load_flag = [&](int64_t first) -> uint32_t { return reset[(has_flag(first) ? (reverse ? length - (first + lane) : first + lane) : 0) * reset_st]; };
 
     const float log_decay = s.log_decay[h];
-    auto decay_of = [&](int k) { return k == 0 ? 1.f : expf(log_decay * (float)k); };  // (k = 0: not 0 * infinity)
-    for (int k = threadIdx.x; k <= CH; k += S::THREADS) {
-        const float x = decay_of(k);
-        power[k] = x;
-        enter[k] = x * s.out_scale;
-        if (k < CH) leave[CH - 1 - k] = x * s.in_scale;
-    }
-    if (threadIdx.x < 2) spoiled[threadIdx.x] = 0;
     Moving<T, CH, DA, S::THREADS, VEC> move_a, move_b;
     Moving<T, CH, DC, S::THREADS, VEC> move_c;
     uint32_t flag = 0;
@@ -282,6 +274,14 @@ __device__ __forceinline__ void walk_part(const Scan& s, int64_t unit, int64_t p
         }
     }
 
+    auto decay_of = [&](int k) { return k == 0 ? 1.f : expf(log_decay * (float)k); };  // (k = 0: not 0 * infinity)
+    for (int k = threadIdx.x; k <= CH; k += S::THREADS) {
+        const float x = decay_of(k);
+        power[k] = x;
+        enter[k] = x * s.out_scale;
+        if (k < CH) leave[CH - 1 - k] = x * s.in_scale;
+    }
+    if (threadIdx.x < 2) spoiled[threadIdx.x] = 0;
     // (the state has arrived before the walk begins: inside, a wait for it would be one for the loads ahead too)
 #pragma unroll
     for (int ct = 0; ct < S::COLS; ++ct)
@@ -522,7 +522,7 @@ __device__ __forceinline__ void walk_part(const Scan& s, int64_t unit, int64_t p
         __syncthreads();
     }
 
-    if (OUT && part == s.parts - 1)  // rows behind the last token
+    if (OUT && part == s.parts - 1 && length < s.steps)  // rows behind the last token
         for (int64_t t = length + threadIdx.x / 32; t < s.steps; t += S::THREADS / 32)
             for (int j = threadIdx.x % 32; j < s.dc; j += 32) out[t * s.out.st + j] = (T)0.f;
     if (!OUT && threadIdx.x == 0) s.carry_out[which] = any_cut ? -1.f : decay_of(begin < end ? (int)(end - begin) - (reverse && begin == 0 ? 1 : 0) : 0);

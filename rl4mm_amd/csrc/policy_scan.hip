@@ -540,6 +540,289 @@ __device__ __forceinline__ void walk_part(const Scan& s, int64_t unit, int64_t p
     }
 }
 
+// ---- short segments: all three gradients at once -----------------------------------------------------------------------------
+//
+// Where the steps are one chunk, a workgroup reads q, k, v and do once and writes dq, dk, dv and the gradient of the initial state: with
+// A = l^(i-j) scale (q_i . k_j) and Z = l^(i-j) scale (do_i . v_j), lower triangles without what a reset cuts, S0 the initial state, R the gradient
+// of the final one,
+//     dq_i = sum_j Z_ij k_j + scale l^(i+1) S0 do_i          dk_j = sum_i Z_ij q_i + l^(L-1-j) R v_j
+//     dv_j = sum_i A_ij do_i + l^(L-1-j) R^T k_j             dS0 = l^L R + scale sum_i l^(i+1) q_i do_i^T
+// Both score matrices lie in LDS by rows i: dq reads them by rows, dk and dv by columns.  Each wave has 16 columns of every result.  Three walks
+// read 9 operands instead of 4 and make 3 score matrices instead of 2: 20 steps x 4096 environments x 4 heads of 32 (f32) took 263 us that way, 193 us this.
+// A chunk with an infinity or a NaN is left to the walks.
+
+template <class T, int CH, int DK, int DV>
+struct OnceRoom {
+    static constexpr int SK = DK + Tile<T>::PAD, SV = DV + Tile<T>::PAD, SP = CH + Tile<T>::PAD;
+    alignas(16) T q[CH * SK], k[CH * SK], v[CH * SV], d[CH * SV], a[CH * SP], z[CH * SP];
+    float power[CH + 1];
+    uint32_t spoiled;
+};
+
+// Fragments of a matrix of floats in memory, [rows][columns] without gaps (NULL: zeros), the summed index in the order of Tile::rows
+template <class T, bool VEC, int K>
+__device__ __forceinline__ typename Tile<T>::Frag matrix_rows(__amdgpu_buffer_rsrc_t buffer, Lane at, int rows, int columns, int row, int k) {
+    constexpr int E = K / 4;
+    float x[E];
+    const int i = row + at.l, j = k + E * at.g;
+    if constexpr (VEC) {
+#pragma unroll
+        for (int e = 0; e < E; e += 4) {
+            typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+            const u32x4 y = __builtin_amdgcn_raw_buffer_load_b128(buffer, i < rows ? (j + e < columns ? (i * columns + j + e) * 4 : 0x40000000) : 0x40000000, 0, 0);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const uint32_t word = y[u];
+                x[e + u] = __builtin_bit_cast(float, word);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            x[e] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(buffer, i < rows ? (j + e < columns ? (i * columns + j + e) * 4 : 0x40000000) : 0x40000000, 0, 0));
+    }
+    typename Tile<T>::Frag f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) f[e] = (T)x[e];
+    return f;
+}
+template <class T, int K>
+__device__ __forceinline__ typename Tile<T>::Frag matrix_columns(__amdgpu_buffer_rsrc_t buffer, Lane at, int rows, int columns, int k, int column) {
+    constexpr int E = K / 4;
+    typename Tile<T>::Frag f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int i = k + E * at.g + e, j = column + at.l;
+        f[e] = (T)__builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(buffer, i < rows ? (j < columns ? (i * columns + j) * 4 : 0x40000000) : 0x40000000, 0, 0));
+    }
+    return f;
+}
+
+template <class T, bool VEC>
+__device__ __forceinline__ void store_columns(T* to, int j, int width, f32x4 x) {  // 4 columns from j on of a row
+    Pack<T, 4> y;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) y.v[r] = (T)x[r];
+    if (VEC) {
+        if (j < width) *reinterpret_cast<Pack<T, 4>*>(to + j) = y;
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (j + r < width) to[j + r] = y.v[r];
+    }
+}
+
+template <class T, int CH, int DK, int DV, bool VEC>
+__global__ __launch_bounds__((DK > DV ? DK : DV) * 4) void gradients_once(Walks w) {
+    typedef Tile<T> M;
+    typedef typename M::Frag Frag;
+    typedef OnceRoom<T, CH, DK, DV> R;
+    constexpr int WAVES = (DK > DV ? DK : DV) / 16, THREADS = 64 * WAVES, PER = M::K / 16, KC = CH / M::K, KK = DK / M::K, KV = DV / M::K;
+    static_assert((Shape<T, CH, DK, DV>::THREADS > Shape<T, CH, DV, DK>::THREADS ? Shape<T, CH, DK, DV>::THREADS : Shape<T, CH, DV, DK>::THREADS) == THREADS, "");
+    union Shared {
+        R once;
+        Room<T, CH, DK, DV, true> one;
+        Room<T, CH, DV, DK, true> other;
+    };
+    __shared__ __align__(16) char room[sizeof(Shared)];
+    Shared& shared = *reinterpret_cast<Shared*>(room);
+    R& s = shared.once;
+
+    const Scan &of_v = w.walk[0], &of_k = w.walk[1], &of_q = w.walk[2];
+    const uint32_t each = gridDim.x / 8, more = gridDim.x % 8, die = blockIdx.x % 8, unit = die * each + (die < more ? die : more) + blockIdx.x / 8;
+    const int64_t n = unit / (uint32_t)of_v.heads;
+    const int h = (int)(unit % (uint32_t)of_v.heads), dk = of_v.da, dv = of_v.dc;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, column = 16 * wave;
+    Lane at = {lane % 16, lane / 16};
+    const int length = __builtin_amdgcn_readfirstlane((int)length_of(of_v, n)), tiles = ((length + 15) / 16 + PER - 1) / PER * PER;
+    const float scale = of_v.in_scale, log_decay = of_v.log_decay[h];
+
+    Moving<T, CH, DK, THREADS, VEC> move_q, move_k;
+    Moving<T, CH, DV, THREADS, VEC> move_v, move_d;
+    move_q.begin((const T*)of_v.b.data + n * of_v.b.sn + h * of_v.b.sh, of_v.b.st, 0, false, dk);
+    move_k.begin((const T*)of_v.a.data + n * of_v.a.sn + h * of_v.a.sh, of_v.a.st, 0, false, dk);
+    move_v.begin((const T*)of_k.a.data + n * of_k.a.sn + h * of_k.a.sh, of_k.a.st, 0, false, dv);
+    move_d.begin((const T*)of_v.c.data + n * of_v.c.sn + h * of_v.c.sh, of_v.c.st, 0, false, dv);
+    move_q.load(length), move_k.load(length), move_v.load(length), move_d.load(length);
+    const bool flagged = of_v.reset && lane < length && of_v.reset[n * of_v.reset_sn + (lane < length ? lane : 0) * of_v.reset_st];
+
+    // the two states, as the results need them
+    const int bytes = dk * dv * 4;
+    const bool with_s0 = of_q.state_in, with_r = of_v.state_in;
+    const __amdgpu_buffer_rsrc_t s0 = __builtin_amdgcn_make_buffer_rsrc((void*)(of_q.state_in + (int64_t)unit * dk * dv), 0, with_s0 ? bytes : 0, 0x27000);
+    const __amdgpu_buffer_rsrc_t rr = __builtin_amdgcn_make_buffer_rsrc((void*)(of_v.state_in + (int64_t)unit * dk * dv), 0, with_r ? bytes : 0, 0x27000);
+    Frag s0_rows[KV], r_rows[KV], r_columns[KK];
+#pragma unroll
+    for (int kk = 0; kk < KV; ++kk) {
+        s0_rows[kk] = matrix_rows<T, VEC, M::K>(s0, at, dk, dv, column, kk * M::K);
+        r_rows[kk] = matrix_rows<T, VEC, M::K>(rr, at, dk, dv, column, kk * M::K);
+    }
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) r_columns[kk] = matrix_columns<T, M::K>(rr, at, dk, dv, kk * M::K, column);
+
+    for (int k = threadIdx.x; k <= CH; k += THREADS) s.power[k] = k == 0 ? 1.f : expf(log_decay * (float)k);
+    if (threadIdx.x == 0) s.spoiled = 0;
+    move_q.store(s.q, R::SK, length), move_k.store(s.k, R::SK, length), move_v.store(s.v, R::SV, length), move_d.store(s.d, R::SV, length);
+    const uint64_t cuts = __ballot(flagged);
+    __syncthreads();
+    float w_diagonal[4], w_below[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int gap = at.l - 4 * at.g - r;
+        w_diagonal[r] = gap >= 0 ? s.power[gap >= 0 ? gap : 0] * scale : 0.f;
+        w_below[r] = s.power[16 + gap] * scale;
+    }
+    float spoils = 0.f;  // becomes NaN with the first number that is none, or infinite
+    const int count = tiles * (tiles + 1) / 2;
+    for (int k0 = wave; k0 < count; k0 += WAVES) {
+        const int it = k0 >= 6 ? 3 : k0 >= 3 ? 2 : k0 >= 1 ? 1 : 0, jt = k0 - it * (it + 1) / 2, i = 16 * it + at.l;
+        f32x4 x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) x[0] = M::product(M::rows(at, s.k, R::SK, 16 * jt, kk * M::K), M::rows(at, s.q, R::SK, 16 * it, kk * M::K), x[0]);
+#pragma unroll
+        for (int kk = 0; kk < KV; ++kk) x[1] = M::product(M::rows(at, s.v, R::SV, 16 * jt, kk * M::K), M::rows(at, s.d, R::SV, 16 * it, kk * M::K), x[1]);
+        const float far = it - jt > 1 ? s.power[16 * (it - jt - 1)] : 1.f;
+        const uint64_t before = cuts & (~0ull >> (63 - i));
+        const int from = before ? 63 - __builtin_clzll(before) : 0;  // the first place that i sees
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            T* tile = u ? s.z : s.a;
+            Pack<T, 4> p;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                spoils = fmaf(x[u][r], 0.f, spoils);
+                const float y = x[u][r] * (it == jt ? w_diagonal[r] : w_below[r] * far);
+                p.v[r] = (T)(16 * jt + 4 * at.g + r >= from ? y : 0.f);
+            }
+            *reinterpret_cast<Pack<T, 4>*>(tile + i * R::SP + 16 * jt + 4 * at.g) = p;
+            if (PER == 2 && it == jt && it % 2 == 0) {  // the tile above the diagonal that shares a fragment with it
+#pragma unroll
+                for (int r = 0; r < 4; ++r) p.v[r] = (T)0.f;
+                *reinterpret_cast<Pack<T, 4>*>(tile + i * R::SP + 16 * jt + 16 + 4 * at.g) = p;
+            }
+        }
+    }
+    if (spoils != 0.f) s.spoiled = 1;
+    __syncthreads();
+    const bool by_walks = __builtin_amdgcn_readfirstlane(s.spoiled) != 0;
+    if (by_walks) {  // (the walk with fewer waves last: the others have ended by then)
+        __syncthreads();
+        constexpr int first = Shape<T, CH, DK, DV>::THREADS, others = Shape<T, CH, DV, DK>::THREADS;
+        if (first >= others) {
+            walk_part<T, CH, DK, DV, true, VEC>(of_v, unit, 0, shared.one);
+            __syncthreads();
+            if (threadIdx.x >= others) return;
+        }
+        walk_part<T, CH, DV, DK, true, VEC>(of_k, unit, 0, shared.other);
+        __syncthreads();
+        walk_part<T, CH, DV, DK, true, VEC>(of_q, unit, 0, shared.other);
+        if (first < others) {
+            __syncthreads();
+            if (threadIdx.x >= first) return;
+            walk_part<T, CH, DK, DV, true, VEC>(of_v, unit, 0, shared.one);
+        }
+        return;
+    }
+
+    const int last_cut = cuts ? 63 - __builtin_clzll(cuts) : 0;
+    // what the state's gradient behind the last token is worth at token j
+    auto tail = [&](int j, f32x4 x) {
+        const float by = s.power[j < length ? length - 1 - j : 0];
+        const bool seen = j >= last_cut;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = seen ? x[r] * by : 0.f;
+        return x;
+    };
+    if (column < DK) {
+        T* to_q = (T*)of_q.out.data + n * of_q.out.sn + h * of_q.out.sh;
+        T* to_k = (T*)of_k.out.data + n * of_k.out.sn + h * of_k.out.sh;
+        Frag keys[KC], queries[KC];
+#pragma unroll
+        for (int kk = 0; kk < KC; ++kk) keys[kk] = M::columns(at, s.k, R::SK, kk * M::K, column), queries[kk] = M::columns(at, s.q, R::SK, kk * M::K, column);
+#pragma unroll 1
+        for (int it = 0; it < tiles; ++it) {
+            at.fresh();
+            const int i = 16 * it + at.l;
+            f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int kk = 0; kk < KV; ++kk) {
+                x = M::product(s0_rows[kk], M::rows(at, s.d, R::SV, 16 * it, kk * M::K), x);
+                y = M::product(r_rows[kk], M::rows(at, s.v, R::SV, 16 * it, kk * M::K), y);
+            }
+            const float by = s.power[i + 1] * scale;
+            const bool sees = (cuts & (~0ull >> (63 - i))) == 0;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[r] = sees ? x[r] * by : 0.f;
+            y = tail(i, y);
+#pragma unroll
+            for (int kk = 0; kk < KC; ++kk) {
+                if (kk * PER <= it) x = M::product(keys[kk], M::rows(at, s.z, R::SP, 16 * it, kk * M::K), x);
+                if (kk * PER + PER > it && kk * PER < tiles) y = M::product(queries[kk], M::columns(at, s.z, R::SP, kk * M::K, 16 * it), y);
+            }
+            if (i < length) {
+                store_columns<T, VEC>(to_q + i * of_q.out.st, column + 4 * at.g, dk, x);
+                store_columns<T, VEC>(to_k + i * of_k.out.st, column + 4 * at.g, dk, y);
+            }
+        }
+        for (int64_t t = length + lane / 16; t < of_v.steps; t += 4)
+            if (column + at.l < dk) to_q[t * of_q.out.st + column + at.l] = to_k[t * of_k.out.st + column + at.l] = (T)0.f;
+    }
+    if (column < DV) {
+        T* to = (T*)of_v.out.data + n * of_v.out.sn + h * of_v.out.sh;
+        Frag values[KC];
+#pragma unroll
+        for (int kk = 0; kk < KC; ++kk) values[kk] = M::columns(at, s.d, R::SV, kk * M::K, column);
+#pragma unroll 1
+        for (int jt = 0; jt < tiles; ++jt) {
+            at.fresh();
+            const int j = 16 * jt + at.l;
+            f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk) x = M::product(r_columns[kk], M::rows(at, s.k, R::SK, 16 * jt, kk * M::K), x);
+            x = tail(j, x);
+#pragma unroll
+            for (int kk = 0; kk < KC; ++kk)
+                if (kk * PER + PER > jt && kk * PER < tiles) x = M::product(values[kk], M::columns(at, s.a, R::SP, kk * M::K, 16 * jt), x);
+            if (j < length) store_columns<T, VEC>(to + j * of_v.out.st, column + 4 * at.g, dv, x);
+        }
+        for (int64_t t = length + lane / 16; t < of_v.steps; t += 4)
+            if (column + at.l < dv) to[t * of_v.out.st + column + at.l] = (T)0.f;
+        if (of_v.state_out) {
+            const int first_cut = cuts ? __builtin_ctzll(cuts) : 64;
+            const Column to_state(of_v.state_out + (int64_t)unit * dk * dv, of_v, dv, 1, column + at.l);
+            const Column from(of_v.state_in + (int64_t)unit * dk * dv, of_v, dv, 1, column + at.l);
+            const float whole = s.power[length];
+            Frag right[KC][M::SPLITS];
+#pragma unroll
+            for (int kk = 0; kk < KC; ++kk) {
+                float by[M::K / 4];
+#pragma unroll
+                for (int e = 0; e < M::K / 4; ++e) {
+                    const int i = kk * M::K + M::place(at, e);
+                    by[e] = i < first_cut && i < length ? s.power[i + 1] * scale : 0.f;
+                }
+                M::weighted(values[kk], by, right[kk]);
+            }
+#pragma unroll 1
+            for (int t = 0; t < DK / 16; ++t) {
+                f32x4 x = {0.f, 0.f, 0.f, 0.f};
+                if (with_r && !cuts) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) x[r] = from.load(16 * t + 4 * at.g + r) * whole;
+                }
+#pragma unroll
+                for (int kk = 0; kk < KC; ++kk) {
+                    const Frag left = M::columns(at, s.q, R::SK, kk * M::K, 16 * t);
+#pragma unroll
+                    for (int i = 0; i < M::SPLITS; ++i) x = M::product(left, right[kk][i], x);
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) to_state.store(16 * t + 4 * at.g + r, x[r]);
+            }
+        }
+    }
+}
+
 // BOTH: the second and third walk have da and dc the other way round
 template <class T, int CH, int DA, int DC, bool BOTH, bool OUT, bool VEC>
 __global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS > Shape<T, CH, DC, DA>::THREADS && BOTH ? Shape<T, CH, DA, DC>::THREADS : BOTH ? Shape<T, CH, DC, DA>::THREADS : Shape<T, CH, DA, DC>::THREADS), (Shape<T, CH, DA, DC>::LEAST_WAVES)) void scan_chunks(Walks w) {
@@ -573,6 +856,13 @@ int scan_launch(const Walks& w, hipStream_t stream) {
     return launched();
 }
 
+template <class T, int CH, int DK, int DV, bool VEC>
+int once_launch(const Walks& w, hipStream_t stream) {
+    const Scan& s = w.walk[0];
+    gradients_once<T, CH, DK, DV, VEC><<<dim3((unsigned)(s.envs * s.heads)), (DK > DV ? DK : DV) * 4, 0, stream>>>(w);
+    return launched();
+}
+
 template <class T, int CH, int DA, int DC>
 int scan_aligned(const Walks& w, bool swapped, hipStream_t stream) {
     constexpr int W = 16 / sizeof(T);
@@ -582,6 +872,8 @@ int scan_aligned(const Walks& w, bool swapped, hipStream_t stream) {
         wide = wide && s.da % W == 0 && s.dc % W == 0 && aligned(s.out.data, 16) && s.out.st % 4 == 0 && s.out.sn % 4 == 0 && s.out.sh % 4 == 0;
         for (const Rows* r : {&s.a, &s.b, &s.c}) wide = wide && aligned(r->data, 16) && r->st % W == 0 && r->sn % W == 0 && r->sh % W == 0;
     }
+    if constexpr (DA <= 64 && DC <= 64)
+        if (swapped && w.walk[0].steps <= CH) return wide ? once_launch<T, CH, DA, DC, true>(w, stream) : once_launch<T, CH, DA, DC, false>(w, stream);
     if constexpr (DA != DC)
         if (swapped) return wide ? scan_launch<T, CH, DA, DC, true, true>(w, stream) : scan_launch<T, CH, DA, DC, true, false>(w, stream);
     return wide ? scan_launch<T, CH, DA, DC, false, true>(w, stream) : scan_launch<T, CH, DA, DC, false, false>(w, stream);

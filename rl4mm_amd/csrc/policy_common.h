@@ -36,6 +36,40 @@ struct alignas(sizeof(T) * W < 16 ? sizeof(T) * W : 16) Pack {
     T v[W];
 };
 
+// the same from and to any address: the hardware's wide loads and stores need no alignment
+template <class T, int W>
+__device__ __forceinline__ Pack<T, W> load_anywhere(const T* p) {
+    Pack<T, W> x;
+    __builtin_memcpy(&x, p, sizeof x);
+    return x;
+}
+template <class T, int W>
+__device__ __forceinline__ void store_anywhere(T* p, const Pack<T, W>& x) {
+    __builtin_memcpy(p, &x, sizeof x);
+}
+
+// element i is x's element i + s, and 0 from behind its end: the end of a row whose length is no multiple of W, loaded as the row's last W elements
+template <class T, int W>
+__device__ __forceinline__ Pack<T, W> shifted(Pack<T, W> x, int s) {
+    static_assert(sizeof x == 8 || sizeof x == 16, "");
+    constexpr int bits = 8 * (int)sizeof(T);
+    if constexpr (sizeof x == 8) {
+        const uint64_t y = __builtin_bit_cast(uint64_t, x);
+        return __builtin_bit_cast(Pack<T, W>, s >= W ? 0 : y >> (bits * s & 63));
+    } else {
+        struct Two {
+            uint64_t lo, hi;
+        } y = __builtin_bit_cast(Two, x);
+        const int half = W / 2;
+        y.lo = s >= half ? y.hi : y.lo;
+        y.hi = s >= half ? 0 : y.hi;
+        const int by = bits * (s >= half ? s - half : s) & 63;
+        y.lo = s >= W ? 0 : y.lo >> by | y.hi << 1 << (63 - by);
+        y.hi >>= by;
+        return __builtin_bit_cast(Pack<T, W>, y);
+    }
+}
+
 template <class T, int W>
 __device__ __forceinline__ void load_pack(const T* p, float* out) {
     const Pack<T, W> x = *reinterpret_cast<const Pack<T, W>*>(p);

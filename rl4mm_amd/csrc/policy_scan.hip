@@ -136,35 +136,41 @@ constexpr uint32_t NOT_FINITE = sizeof(T) == 2 ? 0x80008000u : 0x80000000u;
 // A tile's share of a thread, on its way: CH places in the order of the walk, 16 bytes at a time.  `at` is the thread's first row in the chunk to be
 // loaded next, `step` the bytes from place to place (negative where the walk goes backwards).  Rows behind the last place are loaded from the
 // chunk's first row instead and become 0 when they are stored: a branch around a load would make the next wait one for every load.
-template <class T, int CH, int D, int THREADS, bool VEC>
+// MODE 2: the rows begin at multiples of 16 bytes and are whole packs.  1: they begin anywhere and are one pack long or longer, and the last pack is
+// loaded as the row's last elements and shifted when it is stored.  0: anything, an element at a time.
+template <class T, int CH, int D, int THREADS, int MODE>
 struct Moving {
     static constexpr int VW = 16 / (int)sizeof(T), ROW = D / VW, ROWS = THREADS / ROW, N = CH > ROWS ? CH / ROWS : 1;
     static_assert(THREADS % ROW == 0 && (CH % ROWS == 0 || ROWS % CH == 0), "");
     static __device__ __forceinline__ int first_row() { return threadIdx.x / ROW; }
     static __device__ __forceinline__ int column() { return threadIdx.x % ROW * VW; }
     static __device__ __forceinline__ bool takes_part() { return ROWS <= CH || first_row() < CH; }
-    uint4 x[N];
+    Pack<T, VW> x[N];
     const char *origin, *at;  // the chunk's first row, and the thread's
     int64_t step;
     int width;
 
+    __device__ __forceinline__ int start() const {  // the column that is loaded for column()
+        if (MODE == 1) return column() < width - VW ? column() : width - VW;
+        return column() < width ? column() : 0;
+    }
     __device__ __forceinline__ void begin(const void* base, int64_t st, int64_t first_token, bool reverse, int elements) {
         step = (reverse ? -st : st) * (int64_t)sizeof(T);
         width = elements;
         origin = (const char*)base + first_token * st * (int64_t)sizeof(T);
-        at = origin + first_row() * step + (column() < width ? column() : 0) * (int)sizeof(T);
+        at = origin + first_row() * step + start() * (int)sizeof(T);
     }
     __device__ __forceinline__ void load(int places) {  // and on to the next chunk
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const char* from = first_row() + n * ROWS < places ? at + n * ROWS * step : origin;
-            if (VEC)
-                x[n] = *reinterpret_cast<const uint4*>(from);
+            const T* from = reinterpret_cast<const T*>(first_row() + n * ROWS < places ? at + n * ROWS * step : origin);
+            if (MODE == 2)
+                x[n] = *reinterpret_cast<const Pack<T, VW>*>(from);
+            else if (MODE == 1)
+                x[n] = load_anywhere<T, VW>(from);
             else {
-                Pack<T, VW> one;
 #pragma unroll
-                for (int e = 0; e < VW; ++e) one.v[e] = column() + e < width ? reinterpret_cast<const T*>(from)[e] : (T)0.f;
-                x[n] = __builtin_bit_cast(uint4, one);
+                for (int e = 0; e < VW; ++e) x[n].v[e] = column() + e < width ? from[e] : (T)0.f;
             }
         }
         origin += CH * step;
@@ -173,20 +179,39 @@ struct Moving {
     __device__ __forceinline__ void store(T* tile, int stride, int places) {
         if (places < CH || width < D) {
 #pragma unroll
-            for (int n = 0; n < N; ++n)
-                if (first_row() + n * ROWS >= places || column() >= width) x[n] = make_uint4(0, 0, 0, 0);
+            for (int n = 0; n < N; ++n) {
+                if (MODE == 1) x[n] = shifted(x[n], column() - start());
+                if (first_row() + n * ROWS >= places || column() >= width) x[n] = __builtin_bit_cast(Pack<T, VW>, make_uint4(0, 0, 0, 0));
+            }
         }
         if (!takes_part()) return;
 #pragma unroll
-        for (int n = 0; n < N; ++n) *reinterpret_cast<uint4*>(tile + (first_row() + n * ROWS) * stride + column()) = x[n];
+        for (int n = 0; n < N; ++n) *reinterpret_cast<Pack<T, VW>*>(tile + (first_row() + n * ROWS) * stride + column()) = x[n];
     }
     __device__ __forceinline__ uint32_t bad() const {  // of what was stored last
         uint32_t any = 0;
 #pragma unroll
-        for (int n = 0; n < N; ++n) any |= not_finite<T>(x[n]);
+        for (int n = 0; n < N; ++n) any |= not_finite<T>(__builtin_bit_cast(uint4, x[n]));
         return takes_part() ? any : 0;
     }
 };
+
+// 4 columns from j on of an output's row
+template <class T, int MODE>
+__device__ __forceinline__ void store_columns(T* to, int j, int width, f32x4 x) {
+    Pack<T, 4> y;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) y.v[r] = (T)x[r];
+    if (MODE == 2) {
+        if (j < width) *reinterpret_cast<Pack<T, 4>*>(to + j) = y;
+    } else if (MODE == 1 && j + 4 <= width)
+        store_anywhere(to + j, y);
+    else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (j + r < width) to[j + r] = y.v[r];
+    }
+}
 
 // A column of a state's matrix, by buffer instructions: a load from behind the buffer's end gives 0, a store there does nothing
 struct Column {
@@ -216,7 +241,7 @@ struct Room {
 };
 
 // One part of one walk.  OUT: its outputs; without it the state behind the part alone, from a state of 0 in front of it
-template <class T, int CH, int DA, int DC, bool OUT, bool VEC>
+template <class T, int CH, int DA, int DC, bool OUT, int MODE>
 __device__ __forceinline__ void walk_part(const Scan& s, int64_t unit, int64_t part, Room<T, CH, DA, DC, OUT>& room) {
     typedef Shape<T, CH, DA, DC> S;
     typedef Tile<T> M;
@@ -244,8 +269,8 @@ __device__ __forceinline__ void walk_part(const Scan& s, int64_t unit, int64_t p
     auto load_flag = [&](int64_t first) -> uint32_t { return reset[(has_flag(first) ? (reverse ? length - (first + lane) : first + lane) : 0) * reset_st]; };
 
     const float log_decay = s.log_decay[h];
-    Moving<T, CH, DA, S::THREADS, VEC> move_a, move_b;
-    Moving<T, CH, DC, S::THREADS, VEC> move_c;
+    Moving<T, CH, DA, S::THREADS, MODE> move_a, move_b;
+    Moving<T, CH, DC, S::THREADS, MODE> move_c;
     uint32_t flag = 0;
     if (OUT) move_a.begin((const T*)s.a.data + n * s.a.sn + h * s.a.sh, s.a.st, first_token, reverse, s.da);
     move_b.begin((const T*)s.b.data + n * s.b.sn + h * s.b.sh, s.b.st, first_token, reverse, s.da);
@@ -376,7 +401,7 @@ __device__ __forceinline__ void walk_part(const Scan& s, int64_t unit, int64_t p
             for (int ct = 0; ct < S::COLS; ++ct)
 #pragma unroll
                 for (int kk = 0; kk < KA; ++kk) left[ct][kk] = M::of_state(&state[ct][kk * PER]);
-            T* to = out + token(at.l) + column + 4 * at.g;
+            T* to = out + token(at.l);
             const int64_t on = (reverse ? -16 : 16) * s.out.st;
             float spoils = 0.f;
 #pragma unroll 1
@@ -428,19 +453,7 @@ __device__ __forceinline__ void walk_part(const Scan& s, int64_t unit, int64_t p
                     }
                     if (16 * (pair + u) + at.l < places) {
 #pragma unroll
-                        for (int ct = 0; ct < S::COLS; ++ct) {
-                            const int j = column + 16 * ct + 4 * at.g;
-                            Pack<T, 4> y;
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) y.v[r] = (T)x[u][ct][r];
-                            if (VEC) {
-                                if (j < s.dc) *reinterpret_cast<Pack<T, 4>*>(to + 16 * ct) = y;
-                            } else {
-#pragma unroll
-                                for (int r = 0; r < 4; ++r)
-                                    if (j + r < s.dc) to[16 * ct + r] = y.v[r];
-                            }
-                        }
+                        for (int ct = 0; ct < S::COLS; ++ct) store_columns<T, MODE>(to, column + 16 * ct + 4 * at.g, s.dc, x[u][ct]);
                     }
                     to += on;
                 }
@@ -598,21 +611,7 @@ __device__ __forceinline__ typename Tile<T>::Frag matrix_columns(__amdgpu_buffer
     return f;
 }
 
-template <class T, bool VEC>
-__device__ __forceinline__ void store_columns(T* to, int j, int width, f32x4 x) {  // 4 columns from j on of a row
-    Pack<T, 4> y;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) y.v[r] = (T)x[r];
-    if (VEC) {
-        if (j < width) *reinterpret_cast<Pack<T, 4>*>(to + j) = y;
-    } else {
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (j + r < width) to[j + r] = y.v[r];
-    }
-}
-
-template <class T, int CH, int DK, int DV, bool VEC>
+template <class T, int CH, int DK, int DV, int MODE>
 __global__ __launch_bounds__((DK > DV ? DK : DV) * 4) void gradients_once(Walks w) {
     typedef Tile<T> M;
     typedef typename M::Frag Frag;
@@ -637,8 +636,8 @@ __global__ __launch_bounds__((DK > DV ? DK : DV) * 4) void gradients_once(Walks 
     const int length = __builtin_amdgcn_readfirstlane((int)length_of(of_v, n)), tiles = ((length + 15) / 16 + PER - 1) / PER * PER;
     const float scale = of_v.in_scale, log_decay = of_v.log_decay[h];
 
-    Moving<T, CH, DK, THREADS, VEC> move_q, move_k;
-    Moving<T, CH, DV, THREADS, VEC> move_v, move_d;
+    Moving<T, CH, DK, THREADS, MODE> move_q, move_k;
+    Moving<T, CH, DV, THREADS, MODE> move_v, move_d;
     move_q.begin((const T*)of_v.b.data + n * of_v.b.sn + h * of_v.b.sh, of_v.b.st, 0, false, dk);
     move_k.begin((const T*)of_v.a.data + n * of_v.a.sn + h * of_v.a.sh, of_v.a.st, 0, false, dk);
     move_v.begin((const T*)of_k.a.data + n * of_k.a.sn + h * of_k.a.sh, of_k.a.st, 0, false, dv);
@@ -654,8 +653,8 @@ __global__ __launch_bounds__((DK > DV ? DK : DV) * 4) void gradients_once(Walks 
     Frag s0_rows[KV], r_rows[KV], r_columns[KK];
 #pragma unroll
     for (int kk = 0; kk < KV; ++kk) {
-        s0_rows[kk] = matrix_rows<T, VEC, M::K>(s0, at, dk, dv, column, kk * M::K);
-        r_rows[kk] = matrix_rows<T, VEC, M::K>(rr, at, dk, dv, column, kk * M::K);
+        s0_rows[kk] = matrix_rows<T, MODE == 2, M::K>(s0, at, dk, dv, column, kk * M::K);
+        r_rows[kk] = matrix_rows<T, MODE == 2, M::K>(rr, at, dk, dv, column, kk * M::K);
     }
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) r_columns[kk] = matrix_columns<T, M::K>(rr, at, dk, dv, kk * M::K, column);
@@ -709,17 +708,17 @@ __global__ __launch_bounds__((DK > DV ? DK : DV) * 4) void gradients_once(Walks 
         __syncthreads();
         constexpr int first = Shape<T, CH, DK, DV>::THREADS, others = Shape<T, CH, DV, DK>::THREADS;
         if (first >= others) {
-            walk_part<T, CH, DK, DV, true, VEC>(of_v, unit, 0, shared.one);
+            walk_part<T, CH, DK, DV, true, MODE>(of_v, unit, 0, shared.one);
             __syncthreads();
             if (threadIdx.x >= others) return;
         }
-        walk_part<T, CH, DV, DK, true, VEC>(of_k, unit, 0, shared.other);
+        walk_part<T, CH, DV, DK, true, MODE>(of_k, unit, 0, shared.other);
         __syncthreads();
-        walk_part<T, CH, DV, DK, true, VEC>(of_q, unit, 0, shared.other);
+        walk_part<T, CH, DV, DK, true, MODE>(of_q, unit, 0, shared.other);
         if (first < others) {
             __syncthreads();
             if (threadIdx.x >= first) return;
-            walk_part<T, CH, DK, DV, true, VEC>(of_v, unit, 0, shared.one);
+            walk_part<T, CH, DK, DV, true, MODE>(of_v, unit, 0, shared.one);
         }
         return;
     }
@@ -760,8 +759,8 @@ __global__ __launch_bounds__((DK > DV ? DK : DV) * 4) void gradients_once(Walks 
                 if (kk * PER + PER > it && kk * PER < tiles) y = M::product(queries[kk], M::columns(at, s.z, R::SP, kk * M::K, 16 * it), y);
             }
             if (i < length) {
-                store_columns<T, VEC>(to_q + i * of_q.out.st, column + 4 * at.g, dk, x);
-                store_columns<T, VEC>(to_k + i * of_k.out.st, column + 4 * at.g, dk, y);
+                store_columns<T, MODE>(to_q + i * of_q.out.st, column + 4 * at.g, dk, x);
+                store_columns<T, MODE>(to_k + i * of_k.out.st, column + 4 * at.g, dk, y);
             }
         }
         for (int64_t t = length + lane / 16; t < of_v.steps; t += 4)
@@ -783,7 +782,7 @@ __global__ __launch_bounds__((DK > DV ? DK : DV) * 4) void gradients_once(Walks 
 #pragma unroll
             for (int kk = 0; kk < KC; ++kk)
                 if (kk * PER + PER > jt && kk * PER < tiles) x = M::product(values[kk], M::columns(at, s.a, R::SP, kk * M::K, 16 * jt), x);
-            if (j < length) store_columns<T, VEC>(to + j * of_v.out.st, column + 4 * at.g, dv, x);
+            if (j < length) store_columns<T, MODE>(to + j * of_v.out.st, column + 4 * at.g, dv, x);
         }
         for (int64_t t = length + lane / 16; t < of_v.steps; t += 4)
             if (column + at.l < dv) to[t * of_v.out.st + column + at.l] = (T)0.f;
@@ -824,7 +823,7 @@ __global__ __launch_bounds__((DK > DV ? DK : DV) * 4) void gradients_once(Walks 
 }
 
 // BOTH: the second and third walk have da and dc the other way round
-template <class T, int CH, int DA, int DC, bool BOTH, bool OUT, bool VEC>
+template <class T, int CH, int DA, int DC, bool BOTH, bool OUT, int MODE>
 __global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS > Shape<T, CH, DC, DA>::THREADS && BOTH ? Shape<T, CH, DA, DC>::THREADS : BOTH ? Shape<T, CH, DC, DA>::THREADS : Shape<T, CH, DA, DC>::THREADS), (Shape<T, CH, DA, DC>::LEAST_WAVES)) void scan_chunks(Walks w) {
     union Shared {
         Room<T, CH, DA, DC, OUT> one;
@@ -838,45 +837,52 @@ __global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS > Shape<T, CH, DC, D
     const uint32_t which = index % (uint32_t)w.count, place = index / (uint32_t)w.count;
     const Scan& s = w.walk[which];
     if (!BOTH || which == 0) {
-        if (threadIdx.x < Shape<T, CH, DA, DC>::THREADS) walk_part<T, CH, DA, DC, OUT, VEC>(s, place % units, place / units, shared.one);
+        if (threadIdx.x < Shape<T, CH, DA, DC>::THREADS) walk_part<T, CH, DA, DC, OUT, MODE>(s, place % units, place / units, shared.one);
     } else if (BOTH) {
-        if (threadIdx.x < Shape<T, CH, DC, DA>::THREADS) walk_part<T, CH, BOTH ? DC : DA, BOTH ? DA : DC, OUT, VEC>(s, place % units, place / units, shared.other);
+        if (threadIdx.x < Shape<T, CH, DC, DA>::THREADS) walk_part<T, CH, BOTH ? DC : DA, BOTH ? DA : DC, OUT, MODE>(s, place % units, place / units, shared.other);
     }
 }
 
-template <class T, int CH, int DA, int DC, bool BOTH, bool VEC>
+template <class T, int CH, int DA, int DC, bool BOTH, int MODE>
 int scan_launch(const Walks& w, hipStream_t stream) {
     const Scan& s = w.walk[0];
     const dim3 grid((unsigned)(s.envs * s.heads * s.parts * w.count));
     constexpr int one = Shape<T, CH, DA, DC>::THREADS, other = BOTH ? Shape<T, CH, DC, DA>::THREADS : one, threads = one > other ? one : other;
     if (s.out.data)
-        scan_chunks<T, CH, DA, DC, BOTH, true, VEC><<<grid, threads, 0, stream>>>(w);
+        scan_chunks<T, CH, DA, DC, BOTH, true, MODE><<<grid, threads, 0, stream>>>(w);
     else if constexpr (!BOTH)
-        scan_chunks<T, CH, DA, DC, false, false, VEC><<<grid, threads, 0, stream>>>(w);
+        scan_chunks<T, CH, DA, DC, false, false, MODE><<<grid, threads, 0, stream>>>(w);
     return launched();
 }
 
-template <class T, int CH, int DK, int DV, bool VEC>
+template <class T, int CH, int DK, int DV, int MODE>
 int once_launch(const Walks& w, hipStream_t stream) {
     const Scan& s = w.walk[0];
-    gradients_once<T, CH, DK, DV, VEC><<<dim3((unsigned)(s.envs * s.heads)), (DK > DV ? DK : DV) * 4, 0, stream>>>(w);
+    gradients_once<T, CH, DK, DV, MODE><<<dim3((unsigned)(s.envs * s.heads)), (DK > DV ? DK : DV) * 4, 0, stream>>>(w);
     return launched();
+}
+
+template <class T, int CH, int DA, int DC, int MODE>
+int scan_mode(const Walks& w, bool swapped, hipStream_t stream) {
+    if constexpr (DA <= 64 && DC <= 64)
+        if (swapped && w.walk[0].steps <= CH) return once_launch<T, CH, DA, DC, MODE>(w, stream);
+    if constexpr (DA != DC)
+        if (swapped) return scan_launch<T, CH, DA, DC, true, MODE>(w, stream);
+    return scan_launch<T, CH, DA, DC, false, MODE>(w, stream);
 }
 
 template <class T, int CH, int DA, int DC>
 int scan_aligned(const Walks& w, bool swapped, hipStream_t stream) {
     constexpr int W = 16 / sizeof(T);
-    bool wide = true;
+    bool wide = true, packs = true;
     for (int i = 0; i < w.count; ++i) {
         const Scan& s = w.walk[i];
+        packs = packs && s.da >= W && s.dc >= W;
         wide = wide && s.da % W == 0 && s.dc % W == 0 && aligned(s.out.data, 16) && s.out.st % 4 == 0 && s.out.sn % 4 == 0 && s.out.sh % 4 == 0;
         for (const Rows* r : {&s.a, &s.b, &s.c}) wide = wide && aligned(r->data, 16) && r->st % W == 0 && r->sn % W == 0 && r->sh % W == 0;
     }
-    if constexpr (DA <= 64 && DC <= 64)
-        if (swapped && w.walk[0].steps <= CH) return wide ? once_launch<T, CH, DA, DC, true>(w, stream) : once_launch<T, CH, DA, DC, false>(w, stream);
-    if constexpr (DA != DC)
-        if (swapped) return wide ? scan_launch<T, CH, DA, DC, true, true>(w, stream) : scan_launch<T, CH, DA, DC, true, false>(w, stream);
-    return wide ? scan_launch<T, CH, DA, DC, false, true>(w, stream) : scan_launch<T, CH, DA, DC, false, false>(w, stream);
+    if (wide) return scan_mode<T, CH, DA, DC, 2>(w, swapped, stream);
+    return packs ? scan_mode<T, CH, DA, DC, 1>(w, swapped, stream) : scan_mode<T, CH, DA, DC, 0>(w, swapped, stream);
 }
 
 template <class T, int DA>

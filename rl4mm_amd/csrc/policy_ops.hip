@@ -248,25 +248,56 @@ __device__ __forceinline__ void row_sums(float* v, int count, float* shared) {
     }
 }
 
-template <class T, int VW, int E, int TPR>
-__device__ __forceinline__ void load_row(const T* row, int width, int lane, float* out) {
-#pragma unroll
-    for (int s = 0; s < E / VW; ++s) {
-        const int col = (s * TPR + lane) * VW;
-        if (row && col < width)
-            load_pack<T, VW>(row + col, out + s * VW);
+// A row's elements of one thread.  RAG: rows begin anywhere and are no whole number of packs; the last pack is loaded as the row's last VW elements and
+// shifted, without a branch (which would wait for what is on its way).  Where the row has no element, 0.
+template <class T, int VW, bool RAG>
+__device__ __forceinline__ Pack<T, VW> load_some(const T* row, int width, int col) {
+    if constexpr (RAG) {
+        const int from = col < width - VW ? col : width - VW;
+        return shifted(load_anywhere<T, VW>(row + from), col - from);
+    } else {
+        Pack<T, VW> x;
+        if (col < width)
+            x = *reinterpret_cast<const Pack<T, VW>*>(row + col);
         else
 #pragma unroll
-            for (int i = 0; i < VW; ++i) out[s * VW + i] = 0.f;
+            for (int i = 0; i < VW; ++i) x.v[i] = (T)0.f;
+        return x;
     }
 }
 
-template <class T, int VW, int E, int TPR>
+template <class T, int VW, int E, int TPR, bool RAG>
+__device__ __forceinline__ void load_row(const T* row, int width, int lane, float* out) {
+#pragma unroll
+    for (int s = 0; s < E / VW; ++s) {
+        Pack<T, VW> x;
+        if (row)
+            x = load_some<T, VW, RAG>(row, width, (s * TPR + lane) * VW);
+        else
+#pragma unroll
+            for (int i = 0; i < VW; ++i) x.v[i] = (T)0.f;
+#pragma unroll
+        for (int i = 0; i < VW; ++i) out[s * VW + i] = (float)x.v[i];
+    }
+}
+
+template <class T, int VW, int E, int TPR, bool RAG>
 __device__ __forceinline__ void store_row(T* row, int width, int lane, const float* in) {
 #pragma unroll
     for (int s = 0; s < E / VW; ++s) {
         const int col = (s * TPR + lane) * VW;
-        if (col < width) store_pack<T, VW>(row + col, in + s * VW);
+        Pack<T, VW> x;
+#pragma unroll
+        for (int i = 0; i < VW; ++i) x.v[i] = (T)in[s * VW + i];
+        if constexpr (RAG) {
+            if (col + VW <= width)
+                store_anywhere(row + col, x);
+            else
+#pragma unroll
+                for (int i = 0; i < VW; ++i)
+                    if (col + i < width) row[col + i] = x.v[i];
+        } else if (col < width)
+            *reinterpret_cast<Pack<T, VW>*>(row + col) = x;
     }
 }
 
@@ -274,15 +305,14 @@ __device__ __forceinline__ void store_row(T* row, int width, int lane, const flo
 __device__ __forceinline__ float sigmoid(float u) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * u)); }
 
 // A row as it lies in memory, in registers; numbers are converted where they are used, so that the next row fits beside this one
-template <class T, int VW, int E, int TPR>
+template <class T, int VW, int E, int TPR, bool RAG>
 struct RawRow {
     Pack<T, VW> x[E / VW];
     __device__ __forceinline__ void load(const T* row, int width, int lane) {
 #pragma unroll
         for (int s = 0; s < E / VW; ++s) {
-            const int col = (s * TPR + lane) * VW;
-            if (row && col < width)
-                x[s] = *reinterpret_cast<const Pack<T, VW>*>(row + col);
+            if (row)
+                x[s] = load_some<T, VW, RAG>(row, width, (s * TPR + lane) * VW);
             else
 #pragma unroll
                 for (int i = 0; i < VW; ++i) x[s].v[i] = (T)0.f;
@@ -301,7 +331,7 @@ struct RawRow {
     }
 };
 
-template <class X, class B, int VW, int E, int TPR>
+template <class X, class B, int VW, int E, int TPR, bool RAG>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void block_forward_kernel(Block p) {
     __shared__ float shared[TPR > 64 ? TPR / 32 : 1];
     constexpr int RPB = TPR > 256 ? 1 : 256 / TPR;
@@ -309,9 +339,9 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void block_forward_kernel(Bl
     const float share = 1.f / p.width;
     for (int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR; row < p.rows; row += (int64_t)gridDim.x * RPB) {
         float x[E], b[E], g[E], w[E];
-        load_row<X, VW, E, TPR>((const X*)p.x + row * p.x_sr, p.width, lane, x);
-        load_row<B, VW, E, TPR>((const B*)p.block + row * p.block_sr, p.width, lane, b);
-        load_row<B, VW, E, TPR>(p.gate ? (const B*)p.gate + row * p.gate_sr : nullptr, p.width, lane, g);
+        load_row<X, VW, E, TPR, RAG>((const X*)p.x + row * p.x_sr, p.width, lane, x);
+        load_row<B, VW, E, TPR, RAG>((const B*)p.block + row * p.block_sr, p.width, lane, b);
+        load_row<B, VW, E, TPR, RAG>(p.gate ? (const B*)p.gate + row * p.gate_sr : nullptr, p.width, lane, g);
         float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < E; ++i) sum += b[i] * b[i];
@@ -319,21 +349,21 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void block_forward_kernel(Bl
         const float rb = 1.f / sqrtf(sum * share + p.eps);
 #pragma unroll
         for (int i = 0; i < E; ++i) b[i] *= rb * (p.gate ? sigmoid(g[i]) : 1.f);
-        load_row<float, VW, E, TPR>(p.post, p.width, lane, w);
-        load_row<float, VW, E, TPR>(p.res, p.width, lane, g);
+        load_row<float, VW, E, TPR, RAG>(p.post, p.width, lane, w);
+        load_row<float, VW, E, TPR, RAG>(p.res, p.width, lane, g);
         sum = 0.f;
 #pragma unroll
         for (int i = 0; i < E; ++i) {
             x[i] += g[i] * (w[i] * b[i]);
             sum += x[i] * x[i];
         }
-        store_row<X, VW, E, TPR>((X*)p.y + row * p.width, p.width, lane, x);
+        store_row<X, VW, E, TPR, RAG>((X*)p.y + row * p.width, p.width, lane, x);
         row_sums<TPR>(&sum, 1, shared);
         const float ry = 1.f / sqrtf(sum * share + p.eps);
-        load_row<float, VW, E, TPR>(p.pre, p.width, lane, w);
+        load_row<float, VW, E, TPR, RAG>(p.pre, p.width, lane, w);
 #pragma unroll
         for (int i = 0; i < E; ++i) x[i] = x[i] * ry * w[i];
-        store_row<B, VW, E, TPR>((B*)p.z + row * p.width, p.width, lane, x);
+        store_row<B, VW, E, TPR, RAG>((B*)p.z + row * p.width, p.width, lane, x);
     }
 }
 
@@ -343,7 +373,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void block_forward_kernel(Bl
 //     dpre = sum dz yn;   m = sum f sg bn:  dpost = res m,  dres = post m
 // y is worked out again from x, b and the gate, which costs no memory.  A workgroup keeps its share of the two column sums in registers
 // over all its rows and writes it once; column_sums adds the workgroups' shares in their order.
-template <class X, class B, int VW, int E, int TPR>
+template <class X, class B, int VW, int E, int TPR, bool RAG>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void block_backward_kernel(Block p) {
     constexpr int RPB = TPR > 256 ? 1 : 256 / TPR;
     __shared__ float shared[TPR > 64 ? TPR / 32 : 1];
@@ -354,8 +384,8 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void block_backward_kernel(B
 #pragma unroll
     for (int i = 0; i < E; ++i) sum_m[i] = sum_p[i] = 0.f;
     struct Rows5 {
-        RawRow<X, VW, E, TPR> x, dy;
-        RawRow<B, VW, E, TPR> b, g, dz;
+        RawRow<X, VW, E, TPR, RAG> x, dy;
+        RawRow<B, VW, E, TPR, RAG> b, g, dz;
     } now, next;
     auto load = [&](Rows5& r, int64_t row) {
         r.x.load((const X*)p.x + row * p.x_sr, p.width, lane);
@@ -375,15 +405,15 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void block_backward_kernel(B
         row_sums<TPR>(sums, 1, shared);
         const float rb = 1.f / sqrtf(sums[0] * share + p.eps);
         now.b.again();
-        load_row<float, VW, E, TPR>(p.post, p.width, lane, w);
-        load_row<float, VW, E, TPR>(p.res, p.width, lane, r);
+        load_row<float, VW, E, TPR, RAG>(p.post, p.width, lane, w);
+        load_row<float, VW, E, TPR, RAG>(p.res, p.width, lane, r);
 #pragma unroll
         for (int i = 0; i < E; ++i) {
             sg[i] = p.gate ? sigmoid(now.g[i]) : 1.f;
             w[i] *= r[i];
             y[i] = now.x[i] + w[i] * (sg[i] * (now.b[i] * rb));
         }
-        load_row<float, VW, E, TPR>(p.pre, p.width, lane, r);
+        load_row<float, VW, E, TPR, RAG>(p.pre, p.width, lane, r);
         sums[0] = 0.f;
 #pragma unroll
         for (int i = 0; i < E; ++i) {
@@ -402,7 +432,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void block_backward_kernel(B
             sum_m[i] += y[i] * (sg[i] * bn);
             sums[0] += y[i] * w[i] * sg[i] * bn;
         }
-        store_row<X, VW, E, TPR>((X*)p.grad_x + row * p.width, p.width, lane, y);
+        store_row<X, VW, E, TPR, RAG>((X*)p.grad_x + row * p.width, p.width, lane, y);
         row_sums<TPR>(sums, 1, shared);
         const float back = sums[0] * share;
         now.b.again();
@@ -412,14 +442,14 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void block_backward_kernel(B
             y[i] = rb * (e * sg[i] - bn * back);
             sg[i] = e * bn * (sg[i] * (1.f - sg[i]));
         }
-        store_row<B, VW, E, TPR>((B*)p.grad_block + row * p.width, p.width, lane, y);
-        if (p.gate) store_row<B, VW, E, TPR>((B*)p.grad_gate + row * p.width, p.width, lane, sg);
+        store_row<B, VW, E, TPR, RAG>((B*)p.grad_block + row * p.width, p.width, lane, y);
+        if (p.gate) store_row<B, VW, E, TPR, RAG>((B*)p.grad_gate + row * p.width, p.width, lane, sg);
     }
     float* to = p.partial + (int64_t)blockIdx.x * p.width;
     const int64_t second = (int64_t)gridDim.x * p.width;
     if (TPR > 64) {
-        store_row<float, VW, E, TPR>(to, p.width, lane, sum_m);
-        store_row<float, VW, E, TPR>(to + second, p.width, lane, sum_p);
+        store_row<float, VW, E, TPR, RAG>(to, p.width, lane, sum_m);
+        store_row<float, VW, E, TPR, RAG>(to + second, p.width, lane, sum_p);
     } else {
         const int wave = threadIdx.x / 64;
         for (int which = 0; which < 2; ++which) {
@@ -465,24 +495,27 @@ int64_t block_parts(const lobpolicy_block* b) {
     return groups < BLOCK_PARTS ? groups : BLOCK_PARTS;
 }
 
-template <class X, class B, int VW, int E, int TPR>
+template <class X, class B, int VW, int E, int TPR, bool RAG>
 int block_launch(const Block& p, bool backward, int64_t parts, hipStream_t stream) {
     constexpr int threads = TPR > 256 ? TPR : 256;
     const int64_t groups = ceil_div(p.rows, threads / TPR);
     if (backward)
-        block_backward_kernel<X, B, VW, E, TPR><<<dim3((unsigned)parts), threads, 0, stream>>>(p);
+        block_backward_kernel<X, B, VW, E, TPR, RAG><<<dim3((unsigned)parts), threads, 0, stream>>>(p);
     else
-        block_forward_kernel<X, B, VW, E, TPR><<<dim3((unsigned)(groups < (1 << 20) ? groups : (1 << 20))), threads, 0, stream>>>(p);
+        block_forward_kernel<X, B, VW, E, TPR, RAG><<<dim3((unsigned)(groups < (1 << 20) ? groups : (1 << 20))), threads, 0, stream>>>(p);
     return launched();
 }
 
-template <class X, class B, int VW>
+template <class X, class B, int VW, bool RAG>
 int block_wide(const Block& p, bool backward, int64_t parts, hipStream_t stream) {
-    constexpr int LEAST = VW < 4 ? 4 : VW;
-    if (p.width <= 64 * LEAST) return block_launch<X, B, VW, LEAST, 64>(p, backward, parts, stream);
-    if (p.width <= 1024) return block_launch<X, B, VW, 16, 64>(p, backward, parts, stream);
-    if (p.width <= 2048) return block_launch<X, B, VW, 8, 256>(p, backward, parts, stream);
-    return block_launch<X, B, VW, 8, 1024>(p, backward, parts, stream);
+    if (p.width <= 64 * VW) return block_launch<X, B, VW, VW, 64, RAG>(p, backward, parts, stream);
+    if (p.width <= 512) return block_launch<X, B, VW, 8, 64, RAG>(p, backward, parts, stream);
+    if constexpr (RAG) {  // (the shifted packs of 16 elements to a lane are more than the registers hold)
+        if (p.width <= 1024) return block_launch<X, B, VW, 4, 256, RAG>(p, backward, parts, stream);
+    } else if (p.width <= 1024)
+        return block_launch<X, B, VW, 16, 64, RAG>(p, backward, parts, stream);
+    if (p.width <= 2048) return block_launch<X, B, VW, 8, 256, RAG>(p, backward, parts, stream);
+    return block_launch<X, B, VW, 8, 1024, RAG>(p, backward, parts, stream);
 }
 
 template <class X, class B>
@@ -494,9 +527,10 @@ int block_typed(const Block& p, bool backward, int64_t parts, hipStream_t stream
         ok = ok && aligned(p.block, bs) && aligned(p.gate, bs) && aligned(p.z, bs) && aligned(p.grad_z, bs) && aligned(p.grad_block, bs) && aligned(p.grad_gate, bs);
         return ok && aligned(p.post, fs) && aligned(p.res, fs) && aligned(p.pre, fs) && aligned(p.partial, fs);
     };
-    if (p.width > 256 && fits(8)) return block_wide<X, B, 8>(p, backward, parts, stream);
-    if (fits(4)) return block_wide<X, B, 4>(p, backward, parts, stream);
-    return block_wide<X, B, 1>(p, backward, parts, stream);
+    if (p.width > 256 && fits(8)) return block_wide<X, B, 8, false>(p, backward, parts, stream);
+    if (fits(4)) return block_wide<X, B, 4, false>(p, backward, parts, stream);
+    if (p.width >= 4) return block_wide<X, B, 4, true>(p, backward, parts, stream);
+    return block_launch<X, B, 1, 4, 64, false>(p, backward, parts, stream);
 }
 
 int block_any(const lobpolicy_block* b, const Block& p, bool backward, int64_t parts, void* stream) {

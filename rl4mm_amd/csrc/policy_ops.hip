@@ -150,7 +150,8 @@ struct Step {
     float scale;
 };
 
-template <class T, int VW, int LPR>
+// RAG: dv is no multiple of VW: a row's last pack is loaded as its last VW elements and shifted
+template <class T, int VW, int LPR, bool RAG>
 __global__ __launch_bounds__(256) void step_kernel(Step s) {
     constexpr int RG = 256 / LPR;
     __shared__ float part[RG][LPR * VW];
@@ -160,34 +161,46 @@ __global__ __launch_bounds__(256) void step_kernel(Step s) {
     T* out = (T*)s.out + n * s.out_sn + h * s.out_sh;
     if (s.skip && s.skip[n]) {
         if (mine && group == 0)
-            for (int i = 0; i < VW; ++i) out[col + i] = (T)0.f;
+            for (int i = 0; i < VW; ++i)
+                if (!RAG || col + i < s.dv) out[col + i] = (T)0.f;
         return;
     }
     const T* q = (const T*)s.q + n * s.q_sn + h * s.q_sh;
     const T* k = (const T*)s.k + n * s.k_sn + h * s.k_sh;
     const T* v = (const T*)s.v + n * s.v_sn + h * s.v_sh;
-    float* state = s.state + unit * s.dk * s.dv + col;
+    const int from = RAG && col > s.dv - VW ? s.dv - VW : col;
+    float* state = s.state + unit * s.dk * s.dv;
     const bool fresh = s.reset && s.reset[n * s.reset_sn];
     const float decay = expf(s.log_decay[h]);
     float value[VW], sum[VW];
 #pragma unroll
-    for (int i = 0; i < VW; ++i) value[i] = mine ? (float)v[col + i] : 0.f, sum[i] = 0.f;
+    for (int i = 0; i < VW; ++i) value[i] = mine && (!RAG || col + i < s.dv) ? (float)v[col + i] : 0.f, sum[i] = 0.f;
     if (mine) {
 #pragma unroll 4
         for (int row = group; row < s.dk; row += RG) {
-            float x[VW];
             const float key = (float)k[row], query = (float)q[row];
+            Pack<float, VW> x;
             if (fresh) {
 #pragma unroll
-                for (int i = 0; i < VW; ++i) x[i] = 0.f;
-            } else
-                load_pack<float, VW>(state + row * s.dv, x);
+                for (int i = 0; i < VW; ++i) x.v[i] = 0.f;
+            } else if constexpr (RAG)
+                x = shifted(load_anywhere<float, VW>(state + row * s.dv + from), col - from);
+            else
+                x = *reinterpret_cast<const Pack<float, VW>*>(state + row * s.dv + col);
 #pragma unroll
             for (int i = 0; i < VW; ++i) {
-                x[i] = x[i] * decay + key * value[i];
-                sum[i] += query * x[i];
+                x.v[i] = x.v[i] * decay + key * value[i];
+                sum[i] += query * x.v[i];
             }
-            store_pack<float, VW>(state + row * s.dv, x);
+            if (!RAG)
+                *reinterpret_cast<Pack<float, VW>*>(state + row * s.dv + col) = x;
+            else if (col + VW <= s.dv)
+                store_anywhere(state + row * s.dv + col, x);
+            else {
+#pragma unroll
+                for (int i = 0; i < VW; ++i)
+                    if (col + i < s.dv) state[row * s.dv + col + i] = x.v[i];
+            }
         }
     }
 #pragma unroll
@@ -203,15 +216,21 @@ __global__ __launch_bounds__(256) void step_kernel(Step s) {
 template <class T>
 int step_typed(const Step& s, int64_t units, hipStream_t stream) {
     const dim3 grid((unsigned)units);
-    const bool wide = s.dv % 4 == 0 && (uintptr_t)s.state % 16 == 0;
-    if (wide && s.dv <= 32)
-        step_kernel<T, 4, 8><<<grid, 256, 0, stream>>>(s);
-    else if (wide && s.dv <= 64)
-        step_kernel<T, 4, 16><<<grid, 256, 0, stream>>>(s);
-    else if (wide)
-        step_kernel<T, 4, 32><<<grid, 256, 0, stream>>>(s);
+    auto run = [&](auto lanes) {
+        constexpr int LPR = decltype(lanes)::value;
+        if (s.dv % 4 == 0 && aligned(s.state, 16))
+            step_kernel<T, 4, LPR, false><<<grid, 256, 0, stream>>>(s);
+        else
+            step_kernel<T, 4, LPR, true><<<grid, 256, 0, stream>>>(s);
+    };
+    if (s.dv < 4)
+        step_kernel<T, 1, 8, false><<<grid, 256, 0, stream>>>(s);
+    else if (s.dv <= 32)
+        run(std::integral_constant<int, 8>());
+    else if (s.dv <= 64)
+        run(std::integral_constant<int, 16>());
     else
-        step_kernel<T, 1, 128><<<grid, 256, 0, stream>>>(s);
+        run(std::integral_constant<int, 32>());
     return launched();
 }
 

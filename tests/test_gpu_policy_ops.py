@@ -267,7 +267,7 @@ def test_empty(ops):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
-@pytest.mark.parametrize("size", [(1, 1, 1, 1), (5, 2, 64, 64), (3, 3, 128, 128), (4, 1, 17, 5), (300, 2, 32, 32), (7, 2, 48, 80), (2, 2, 100, 31), (3, 1, 9, 100)], ids=str)
+@pytest.mark.parametrize("size", [(1, 1, 1, 1), (5, 2, 64, 64), (3, 3, 128, 128), (4, 1, 17, 5), (300, 2, 32, 32), (7, 2, 48, 80), (2, 2, 100, 31), (3, 1, 9, 100), (3, 2, 40, 3), (5, 1, 16, 4), (3, 2, 33, 127), (2, 1, 128, 33), (4, 2, 3, 7)], ids=str)
 def test_step(ops, size, dtype):
     N, H, dk, dv = size
     p, _, _ = problem(20, 3, N, H, dk, dv, dtype)

@@ -8,7 +8,8 @@ asynchronously on torch's current stream of the tensors' device, like the tensor
 
 float32 and bfloat16; states, norms and sums are float32 or wider.  There is no CPU path: CPU tensors raise, as does a missing
 library.  Every call can be captured into a graph (nothing waits for the device, nothing is allocated but results and workspaces, through
-torch's allocator).  A call that cannot be right raises ValueError or TypeError before anything is launched."""
+torch's allocator); a forward and a backward pass belong into the same capture, with no eager graph of the same leaves alive beside it, as torch
+asks of every operation.  A call that cannot be right raises ValueError or TypeError before anything is launched."""
 from __future__ import annotations
 
 import ctypes as C
@@ -336,7 +337,7 @@ def gated_residual_norm(x, block, gate, post_weight, residual_scale, pre_weight,
         for t, name in zip(weights, ("post_weight", "residual_scale", "pre_weight")):
             _tensor(t, name, (torch.float32,), x.device, (width,))
     eps = float(eps)
-    _need(math.isfinite(eps) and eps > 0.0, "eps is a positive number")
+    _need(math.isfinite(eps) and eps >= 2.0**-126, "eps is a positive number that 32 bits hold")
     shape, wanted = x.shape, torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, block, gate, *weights))
     rows = [_rows(t, width) if t is not None else None for t in (x, block, gate)]
     if x.numel() == 0:  # (nothing to compute, and the gradients are zeros: torch's own operations say so)

@@ -74,7 +74,7 @@ def test_attention_and_gradients(ops, size, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
-@pytest.mark.parametrize("size", [(20, 9, 2, 32, 32), (64, 7, 1, 48, 80), (150, 6, 2, 64, 64), (257, 5, 1, 128, 128), (90, 5, 2, 7, 13)], ids=str)
+@pytest.mark.parametrize("size", [(20, 9, 2, 32, 32), (64, 7, 1, 48, 80), (150, 6, 2, 64, 64), (257, 5, 1, 128, 128), (90, 5, 2, 7, 13), (30, 5, 2, 20, 50), (31, 5, 1, 50, 20), (32, 5, 1, 64, 64), (50, 4, 1, 5, 3), (28, 4, 1, 33, 64)], ids=str)
 def test_resets_and_lengths(ops, size, dtype):
     for resets, ragged in ((0.05, False), (0.0, True), (0.02, True), (0.6, True)):
         p, dout, dlast = problem(int(100 * resets) + 3 * ragged, *size, dtype, resets, ragged)
@@ -102,7 +102,7 @@ def test_lengths_at_the_borders(ops, dtype):
 
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("junk", [math.nan, math.inf, -math.inf])
-@pytest.mark.parametrize("size", [(200, 4, 2, 64, 64), (200, 4, 1, 32, 128), (40, 4, 1, 30, 21)], ids=str)
+@pytest.mark.parametrize("size", [(200, 4, 2, 64, 64), (200, 4, 1, 32, 128), (40, 4, 1, 30, 21), (30, 4, 2, 24, 60), (30, 4, 1, 60, 24), (30, 4, 1, 64, 64)], ids=str)
 def test_masked_places_hold_anything(ops, size, junk, dtype):
     """Behind an environment's last token, before a reset, in the state that a reset drops: whatever is there reaches nothing else."""
     T = size[0]
@@ -565,3 +565,73 @@ def test_two_streams_at_once(ops):
     torch.cuda.synchronize()
     for g, w in zip(got, want):
         assert all(torch.equal(a, b) for a, b in zip(g, w))
+
+
+def test_two_threads_at_once(ops):
+    import threading
+
+    sides = [make_everything(41), make_everything(43)]
+    want = [everything(ops, *s) for s in sides]
+    torch.cuda.synchronize()
+    got, wrong = [None, None], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(3):
+                    got[i] = everything(ops, *sides[i])
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    torch.cuda.synchronize()
+    assert not wrong
+    for g, w in zip(got, want):
+        assert all(torch.equal(a, b) for a, b in zip(g, w))
+
+
+# ---- beyond 32 bits of elements and offsets ----------------------------------------------------------------------------------------
+
+
+def test_attention_beyond_32_bits(ops):
+    """The last environments of a batch of more than 2^31 elements are what they are alone: each environment's arithmetic is its own."""
+    N = 131_100
+    x = torch.randn(64, N, 4, 64, device="cuda", dtype=BF16)
+    assert x.numel() > 2**31
+    g, reset = decays(4), torch.zeros(64, N, dtype=torch.bool, device="cuda")
+    reset[17, -2:] = True
+    leaf = x.requires_grad_(True)
+    out, last = ops.decay_attention(leaf, leaf.detach(), leaf.detach(), g, reset=reset)
+    (dx,) = torch.autograd.grad(out, leaf, x.detach())
+    alone = x.detach()[:, -2:].contiguous().requires_grad_(True)
+    out2, last2 = ops.decay_attention(alone, alone.detach(), alone.detach(), g, reset=reset[:, -2:].contiguous())
+    (dx2,) = torch.autograd.grad(out2, alone, alone.detach())
+    assert torch.equal(out[:, -2:], out2) and torch.equal(last[-2:], last2) and torch.equal(dx[:, -2:], dx2)
+    state = last.detach()
+    now = x.detach()[5]
+    tail = state[-2:].clone()
+    one = ops.decay_attention_step(now, now, now, g, state)
+    two = ops.decay_attention_step(now[-2:], now[-2:], now[-2:], g, tail)
+    assert torch.equal(one[-2:], two) and torch.equal(state[-2:], tail)
+
+
+def test_block_and_clip_beyond_32_bits(ops):
+    x = torch.randn(8_388_700, 256, device="cuda", dtype=BF16)
+    assert x.numel() > 2**31
+    w = [1 + 0.1 * normal(i, 256) for i in range(3)]
+    leaf = x.requires_grad_(True)
+    y, z = ops.gated_residual_norm(leaf, x.detach(), x.detach(), *w)
+    (dx,) = torch.autograd.grad([y, z], leaf, [x.detach(), x.detach()])
+    alone = x.detach()[-3:].clone().requires_grad_(True)
+    y2, z2 = ops.gated_residual_norm(alone, alone.detach(), alone.detach(), *w)
+    (dx2,) = torch.autograd.grad([y2, z2], alone, [alone.detach(), alone.detach()])
+    assert torch.equal(y[-3:], y2) and torch.equal(z[-3:], z2) and torch.equal(dx[-3:], dx2)
+    grad = x.detach()
+    before = grad[-2:].clone()
+    norm = ops.clip_grad_norm(grad, 1.0)
+    assert abs(float(norm) / grad.numel() ** 0.5 - 1.0) < 0.01
+    by = torch.tensor(1.0 / (float(norm) + 1e-6))
+    assert torch.allclose(grad[-2:].float(), before.float() * by.cuda(), rtol=2.0**-7, atol=0.0)

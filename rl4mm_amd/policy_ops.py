@@ -27,23 +27,37 @@ _NONE = capi.Operand(None, 0, 0, 0)
 _raw_stream = torch._C._cuda_getCurrentRawStream  # torch.cuda.current_stream(index).cuda_stream without the object around it
 
 
+_current_device = torch._C._cuda_getDevice
+
+
 class _on:
-    """The raw current stream of a device, with that device current inside the block."""
+    """The raw current stream of a device that is not the current one, with that device current inside the block."""
 
     __slots__ = ("index", "before")
 
-    def __init__(self, device):
-        self.index = device.index
+    def __init__(self, index):
+        self.index = index
 
     def __enter__(self):
         self.before = torch.cuda.current_device()
-        if self.before != self.index:
-            torch.cuda.set_device(self.index)
+        torch.cuda.set_device(self.index)
         return _raw_stream(self.index)
 
     def __exit__(self, *exc):
-        if self.before != self.index:
-            torch.cuda.set_device(self.before)
+        torch.cuda.set_device(self.before)
+
+
+def _call(device, name, *args):
+    """An entry point of the library, on the current stream of `device`, which is made the current device for it."""
+    lib = _lib._policy_binding or _lib.policy_binding()
+    index = device.index
+    if index == _current_device():
+        code = lib.fn[name](*args, _raw_stream(index))
+    else:
+        with _on(index) as stream:
+            code = lib.fn[name](*args, stream)
+    if code < 0:
+        lib.check(code, name)
 
 
 def _new(t):
@@ -156,9 +170,8 @@ def _attention_forward(q, k, v, log_decay, state, reset, lengths, scale):
     lib = _lib.policy_binding()
     a = _describe(q, k, v, log_decay, reset, lengths, scale)
     a.out, a.state_in, a.state_out = _operand(out), _ptr(state), last.data_ptr()
-    with _on(q.device) as stream:
-        held = _workspace(a, lib, q.device)
-        lib.check(lib.fn["attention_forward"](C.byref(a), stream), "attention_forward")
+    held = _workspace(a, lib, q.device)
+    _call(q.device, "attention_forward", C.byref(a))
     return out, last, held
 
 
@@ -185,10 +198,9 @@ class _DecayAttention(torch.autograd.Function):
         a = _describe(q, k, v, log_decay, reset, lengths, ctx.scale)
         a.out, a.state_in, a.grad_state_out = _operand(dout), _ptr(state), _ptr(dlast)
         a.grad_q, a.grad_k, a.grad_v, a.grad_state_in = _operand(dq), _operand(dk), _operand(dv), _ptr(dstate)
-        with _on(q.device) as stream:
-            held = _workspace(a, lib, q.device)  # noqa: F841
-            a.forward_workspace = _ptr(forward)
-            lib.check(lib.fn["attention_backward"](C.byref(a), stream), "attention_backward")
+        held = _workspace(a, lib, q.device)  # noqa: F841
+        a.forward_workspace = _ptr(forward)
+        _call(q.device, "attention_backward", C.byref(a))
         need = ctx.needs_input_grad
         return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, dstate, None, None, None
 
@@ -237,11 +249,9 @@ def decay_attention_step(q, k, v, log_decay, state, *, reset=None, skip=None, sc
         return out
     q, k, v = _lined(q), _lined(k), _lined(v)
     skip = None if skip is None else skip.contiguous()
-    lib = _lib.policy_binding()
     a = _describe(q, k, v, log_decay, reset, None, scale)
     a.out, a.state_out, a.skip = _operand(out), state.data_ptr(), _ptr(skip)
-    with _on(q.device) as stream:
-        lib.check(lib.fn["attention_step"](C.byref(a), stream), "attention_step")
+    _call(q.device, "attention_step", C.byref(a))
     _changed([state])
     return out
 
@@ -266,11 +276,9 @@ def _describe_block(x, block, gate, post, res, pre, eps):
 
 def _block_forward(x, block, gate, post, res, pre, eps):
     y, z = _new(x), _new(block)
-    lib = _lib.policy_binding()
     b = _describe_block(x, block, gate, post, res, pre, eps)
     b.y, b.z = y.data_ptr(), z.data_ptr()
-    with _on(x.device) as stream:
-        lib.check(lib.fn["block_forward"](C.byref(b), stream), "block_forward")
+    _call(x.device, "block_forward", C.byref(b))
     return y, z
 
 
@@ -298,11 +306,10 @@ class _GatedResidualNorm(torch.autograd.Function):
         b.grad_y_stride, b.grad_z_stride = 0 if dy is None else dy.stride(0), 0 if dz is None else dz.stride(0)
         b.grad_x, b.grad_block, b.grad_gate = dx.data_ptr(), dblock.data_ptr(), _ptr(dgate)
         b.grad_post, b.grad_res, b.grad_pre = dpost.data_ptr(), dres.data_ptr(), dpre.data_ptr()
-        with _on(x.device) as stream:
-            need = lib.check(lib.fn["block_workspace"](C.byref(b)), "block_workspace")
-            held = torch.empty(need, dtype=torch.uint8, device=x.device)
-            b.workspace, b.workspace_bytes = held.data_ptr(), need
-            lib.check(lib.fn["block_backward"](C.byref(b), stream), "block_backward")
+        need = lib.check(lib.fn["block_workspace"](C.byref(b)), "block_workspace")
+        held = torch.empty(need, dtype=torch.uint8, device=x.device)
+        b.workspace, b.workspace_bytes = held.data_ptr(), need
+        _call(x.device, "block_backward", C.byref(b))
         return tuple(g if wanted else None for g, wanted in zip((dx, dblock, dgate, dpost, dres, dpre), ctx.needs_input_grad)) + (None,)
 
 
@@ -387,15 +394,17 @@ def clip_grad_norm(grads, max_norm, norm_type=2.0):
         if count:
             spans.append((g.data_ptr(), count * g.itemsize, i))
     spans.sort()
-    for (p, size, i), (q, _, j) in zip(spans, spans[1:]):
-        _need(p + size <= q, f"gradients {min(i, j)} and {max(i, j)} share memory: each element is counted and scaled once")
+    end, last = 0, -1
+    for p, size, i in spans:
+        if p < end:
+            raise ValueError(f"gradients {min(i, last)} and {max(i, last)} share memory: each element is counted and scaled once")
+        end, last = p + size, i
     n = len(grads)
     tensors = (C.c_void_p * n)(*[g.data_ptr() for g in grads])
     counts, dtypes = (C.c_int64 * n)(*[g.numel() for g in grads]), (C.c_int32 * n)(*[_DTYPES[g.dtype] for g in grads])
     lib = _lib.policy_binding()
-    with _on(device) as stream:
-        need = lib.check(lib.fn["clip_workspace"](counts, dtypes, n), "clip_workspace")
-        norm, held = torch.empty((), dtype=torch.float32, device=device), torch.empty(max(need, 8), dtype=torch.uint8, device=device)
-        lib.check(lib.fn["clip"](tensors, counts, dtypes, n, 2 if norm_type == 2.0 else 0, max_norm, norm.data_ptr(), held.data_ptr(), need, stream), "clip")
+    need = lib.check(lib.fn["clip_workspace"](counts, dtypes, n), "clip_workspace")
+    norm, held = torch.empty((), dtype=torch.float32, device=device), torch.empty(max(need, 8), dtype=torch.uint8, device=device)
+    _call(device, "clip", tensors, counts, dtypes, n, 2 if norm_type == 2.0 else 0, max_norm, norm.data_ptr(), held.data_ptr(), need)
     _changed(grads)
     return norm

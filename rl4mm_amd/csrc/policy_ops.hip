@@ -27,13 +27,20 @@ int scan_typed(const Walks& w, bool swapped, hipStream_t stream) {
 }
 
 // Few environments and heads, many steps: the steps are split into parts.  A first walk finds what each part adds to the state, join_parts
-// turns that into the state in front of each part, a second walk starts from it.
+// turns that into the state in front of each part, a second walk starts from it.  That reads k and v twice, so it pays where the chip is
+// otherwise far from full, and then only until it is full.  Whole against split, forwards, in us:
+//     widths of 32 to 32 (bf16): 4096 steps, 32 units 202 : 29, 256 units 202 : 106, 384 units 235 : 192, 512 units 238 : 224, with the gradients 586 : 669
+//     64 to 64 (bf16): 4096 steps, 32 units 227 : 44, 128 units 227 : 112, 256 units 229 : 252;  128 to 128: 128 units 404 : 249, 256 units 428 : 456
+//     64 to 64 (f32): 128 units 365 : 232, 256 units 369 : 409
+// 512 and 1024 workgroups in all take 112 and 115 us of 128 units of 64 to 64, 89 and 62 us of 128 units of 32 to 32.  Below 512 steps the two
+// further launches take what the parts save (256 steps of 64 to 64, 32 units: 20 : 24, at 512 steps 34 : 25).
 struct Parts {
     int64_t steps;
     int count;
     Parts(const lobpolicy_attention* a) {
-        const int64_t units = a->envs * a->heads, wanted = a->dk > 64 || a->dv > 64 ? 512 : 1024;
-        int64_t n = a->steps < 512 || units >= 512 ? 1 : ceil_div(wanted, units);
+        const bool narrow = a->dk <= 32 && a->dv <= 32;
+        const int64_t units = a->envs * a->heads, wanted = narrow ? 1024 : 512;
+        int64_t n = a->steps < 512 || units >= (narrow ? 384 : 256) ? 1 : ceil_div(wanted, units);
         n = n < ceil_div(a->steps, 128) ? n : ceil_div(a->steps, 128);
         steps = ceil_div(ceil_div(a->steps, n), 64) * 64;
         count = (int)ceil_div(a->steps, steps);

@@ -521,31 +521,40 @@ int64_t block_parts(const lobpolicy_block* b) {
     return groups < BLOCK_PARTS ? groups : BLOCK_PARTS;
 }
 
-template <class X, class B, int VW, int E, int TPR, bool RAG>
-int block_launch(const Block& p, bool backward, int64_t parts, hipStream_t stream) {
+template <class X, class B, int VW, int E, int TPR, bool RAG, bool BACKWARD>
+int block_launch(const Block& p, int64_t parts, hipStream_t stream) {
     constexpr int threads = TPR > 256 ? TPR : 256;
-    const int64_t groups = ceil_div(p.rows, threads / TPR);
-    if (backward)
+    if constexpr (BACKWARD)
         block_backward_kernel<X, B, VW, E, TPR, RAG><<<dim3((unsigned)parts), threads, 0, stream>>>(p);
-    else
+    else {
+        const int64_t groups = ceil_div(p.rows, threads / TPR);
         block_forward_kernel<X, B, VW, E, TPR, RAG><<<dim3((unsigned)(groups < (1 << 20) ? groups : (1 << 20))), threads, 0, stream>>>(p);
+    }
     return launched();
 }
 
-template <class X, class B, int VW, bool RAG>
-int block_wide(const Block& p, bool backward, int64_t parts, hipStream_t stream) {
-    if (p.width <= 64 * VW) return block_launch<X, B, VW, VW, 64, RAG>(p, backward, parts, stream);
-    if (p.width <= 512) return block_launch<X, B, VW, 8, 64, RAG>(p, backward, parts, stream);
+// A row to a wave as long as its registers hold it, then to as many threads as it needs: idle threads cost as much as busy ones.  Both gradients
+// and results of 64 M elements in us, forwards + backwards (bf16): 1024 wide a wave to a row 130 + 264, 256 threads to a row 172 + 523 (sums through
+// LDS, every column sum in four times the threads); 4096 wide 512 threads 127 + 319, 1024 half of which are idle 251 + 673; 8192 wide, forwards
+// 1024 threads 155 (512: 185), backwards 512 threads 294 (1024, whose 128 registers do not hold a row and the next: 485).
+template <class X, class B, int VW, bool RAG, bool BACKWARD>
+int block_wide(const Block& p, int64_t parts, hipStream_t stream) {
+    if (p.width <= 64 * VW) return block_launch<X, B, VW, VW, 64, RAG, BACKWARD>(p, parts, stream);
+    if (p.width <= 512) return block_launch<X, B, VW, 8, 64, RAG, BACKWARD>(p, parts, stream);
     if constexpr (RAG) {  // (the shifted packs of 16 elements to a lane are more than the registers hold)
-        if (p.width <= 1024) return block_launch<X, B, VW, 4, 256, RAG>(p, backward, parts, stream);
+        if (p.width <= 1024) return block_launch<X, B, VW, 4, 256, RAG, BACKWARD>(p, parts, stream);
     } else if (p.width <= 1024)
-        return block_launch<X, B, VW, 16, 64, RAG>(p, backward, parts, stream);
-    if (p.width <= 2048) return block_launch<X, B, VW, 8, 256, RAG>(p, backward, parts, stream);
-    return block_launch<X, B, VW, 8, 1024, RAG>(p, backward, parts, stream);
+        return block_launch<X, B, VW, 16, 64, RAG, BACKWARD>(p, parts, stream);
+    if (p.width <= 2048) return block_launch<X, B, VW, 8, 256, RAG, BACKWARD>(p, parts, stream);
+    if (p.width <= 4096) return block_launch<X, B, VW, 8, 512, RAG, BACKWARD>(p, parts, stream);
+    if constexpr (!RAG && BACKWARD)
+        return block_launch<X, B, VW, 16, 512, RAG, BACKWARD>(p, parts, stream);
+    else
+        return block_launch<X, B, VW, 8, 1024, RAG, BACKWARD>(p, parts, stream);
 }
 
-template <class X, class B>
-int block_typed(const Block& p, bool backward, int64_t parts, hipStream_t stream) {
+template <class X, class B, bool BACKWARD>
+int block_typed(const Block& p, int64_t parts, hipStream_t stream) {
     auto fits = [&](int w) {
         const int64_t xs = w * sizeof(X) < 16 ? w * sizeof(X) : 16, bs = w * sizeof(B) < 16 ? w * sizeof(B) : 16, fs = w * 4 < 16 ? w * 4 : 16;
         bool ok = p.width % w == 0 && p.x_sr % w == 0 && p.block_sr % w == 0 && p.gate_sr % w == 0 && p.grad_y_sr % w == 0 && p.grad_z_sr % w == 0;
@@ -553,16 +562,20 @@ int block_typed(const Block& p, bool backward, int64_t parts, hipStream_t stream
         ok = ok && aligned(p.block, bs) && aligned(p.gate, bs) && aligned(p.z, bs) && aligned(p.grad_z, bs) && aligned(p.grad_block, bs) && aligned(p.grad_gate, bs);
         return ok && aligned(p.post, fs) && aligned(p.res, fs) && aligned(p.pre, fs) && aligned(p.partial, fs);
     };
-    if (p.width > 256 && fits(8)) return block_wide<X, B, 8, false>(p, backward, parts, stream);
-    if (fits(4)) return block_wide<X, B, 4, false>(p, backward, parts, stream);
-    if (p.width >= 4) return block_wide<X, B, 4, true>(p, backward, parts, stream);
-    return block_launch<X, B, 1, 4, 64, false>(p, backward, parts, stream);
+    // packs of 8 where a wave is full of them, else of 4; rows of no whole packs of 4 in shifted ones; 1024 wide, 65536 rows, forwards + backwards:
+    // packs of 8 130 + 264 us, of 4 143 + 826 (bf16), 163 + 349 and 170 + 777 (x f32), 203 + 510 and 186 + 498 (f32 only, where both are two loads)
+    if (p.width > 256 && fits(8)) return block_wide<X, B, 8, false, BACKWARD>(p, parts, stream);
+    if (fits(4)) return block_wide<X, B, 4, false, BACKWARD>(p, parts, stream);
+    if (p.width >= 4) return block_wide<X, B, 4, true, BACKWARD>(p, parts, stream);
+    return block_launch<X, B, 1, 4, 64, false, BACKWARD>(p, parts, stream);
 }
 
-int block_any(const lobpolicy_block* b, const Block& p, bool backward, int64_t parts, void* stream) {
+template <bool BACKWARD>
+int block_any(const lobpolicy_block* b, const Block& p, int64_t parts, void* stream) {
     hipStream_t s = (hipStream_t)stream;
-    if (b->stream_dtype == LOBPOLICY_F32) return b->dtype == LOBPOLICY_F32 ? block_typed<float, float>(p, backward, parts, s) : block_typed<float, bf16>(p, backward, parts, s);
-    return b->dtype == LOBPOLICY_F32 ? block_typed<bf16, float>(p, backward, parts, s) : block_typed<bf16, bf16>(p, backward, parts, s);
+    if (b->stream_dtype == LOBPOLICY_F32)
+        return b->dtype == LOBPOLICY_F32 ? block_typed<float, float, BACKWARD>(p, parts, s) : block_typed<float, bf16, BACKWARD>(p, parts, s);
+    return b->dtype == LOBPOLICY_F32 ? block_typed<bf16, float, BACKWARD>(p, parts, s) : block_typed<bf16, bf16, BACKWARD>(p, parts, s);
 }
 
 int check_block(const lobpolicy_block* b) {
@@ -906,7 +919,7 @@ int lobpolicy_block_forward(const lobpolicy_block* b, void* stream) {
     REQUIRE(b->y && b->z, "a result is missing");
     Block p = block_of(b);
     p.y = b->y, p.z = b->z;
-    return block_any(b, p, false, 0, stream);
+    return block_any<false>(b, p, 0, stream);
 }
 
 int lobpolicy_block_backward(const lobpolicy_block* b, void* stream) {
@@ -918,7 +931,7 @@ int lobpolicy_block_backward(const lobpolicy_block* b, void* stream) {
     p.grad_x = b->grad_x, p.grad_block = b->grad_block, p.grad_gate = b->grad_gate;
     p.partial = (float*)b->workspace;
     const int64_t parts = block_parts(b);
-    if (int e = block_any(b, p, true, parts, stream)) return e;
+    if (int e = block_any<true>(b, p, parts, stream)) return e;
     column_sums<<<dim3((unsigned)ceil_div(b->width, 32), 2), 1024, 0, (hipStream_t)stream>>>(p.partial, (int)parts, p.width, b->post, b->res, b->grad_post, b->grad_res, b->grad_pre);
     return launched();
 }

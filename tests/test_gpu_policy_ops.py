@@ -362,6 +362,14 @@ def test_block(ops, width, types):
         check_block(ops, args, dy, dz)
 
 
+@pytest.mark.parametrize("types", [(F32, F32), (BF16, BF16), (F32, BF16), (BF16, F32)], ids=["f32", "bf16", "f32+bf16", "bf16+f32"])
+@pytest.mark.parametrize("width", [2049, 2056, 4088, 4094, 4096, 4097, 4104, 8191])
+def test_block_wide_rows(ops, width, types):
+    """each number of threads that shares a long row, full and a little more than full"""
+    args, dy, dz = block_problem(width, 3, width, *types)
+    check_block(ops, args, dy, dz)
+
+
 def test_block_many_rows_and_order(ops):
     """More rows than workgroups: the weights' gradients, and twice the same bits"""
     for rows, width in ((5000, 32), (2500, 300), (1200, 1100)):

@@ -32,15 +32,16 @@ int scan_typed(const Walks& w, bool swapped, hipStream_t stream) {
 //     widths of 32 to 32 (bf16): 4096 steps, 32 units 202 : 29, 256 units 202 : 106, 384 units 235 : 192, 512 units 238 : 224, with the gradients 586 : 669
 //     64 to 64 (bf16): 4096 steps, 32 units 227 : 44, 128 units 227 : 112, 256 units 229 : 252;  128 to 128: 128 units 404 : 249, 256 units 428 : 456
 //     64 to 64 (f32): 128 units 365 : 232, 256 units 369 : 409
-// 512 and 1024 workgroups in all take 112 and 115 us of 128 units of 64 to 64, 89 and 62 us of 128 units of 32 to 32.  Below 512 steps the two
+// 512 and 1024 workgroups in all: 112 and 115 us (bf16, 128 units of 64 to 64), 89 and 62 us (32 to 32), 264 and 246 us (f32, 18000 steps of 32
+// units of 64 to 64), 88 and 98 us (bf16, 18000 steps of 8 units of 128 to 128).  Below 512 steps the two
 // further launches take what the parts save (256 steps of 64 to 64, 32 units: 20 : 24, at 512 steps 34 : 25).
 struct Parts {
     int64_t steps;
     int count;
     Parts(const lobpolicy_attention* a) {
-        const bool narrow = a->dk <= 32 && a->dv <= 32;
-        const int64_t units = a->envs * a->heads, wanted = narrow ? 1024 : 512;
-        int64_t n = a->steps < 512 || units >= (narrow ? 384 : 256) ? 1 : ceil_div(wanted, units);
+        const int widest = a->dk > a->dv ? a->dk : a->dv;
+        const int64_t units = a->envs * a->heads, wanted = widest <= (a->dtype == LOBPOLICY_F32 ? 64 : 32) ? 1024 : 512;
+        int64_t n = a->steps < 512 || units >= (widest <= 32 ? 384 : 256) ? 1 : ceil_div(wanted, units);
         n = n < ceil_div(a->steps, 128) ? n : ceil_div(a->steps, 128);
         steps = ceil_div(ceil_div(a->steps, n), 64) * 64;
         count = (int)ceil_div(a->steps, steps);

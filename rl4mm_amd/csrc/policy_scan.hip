@@ -118,9 +118,10 @@ struct Tile<bf16> {  // a fragment: 32 of the summed index, places 8 (lane / 16)
 
 template <class T, int CH, int DA, int DC>
 struct Shape {
-    static constexpr int COLS = DC == 128 ? 2 : 1;  // tiles of 16 of the state's columns to a wave
+    // tiles of 16 of the state's columns to a wave: each operand that waves share is read from LDS once for both (4096 steps, 128 units of 128 to 128,
+    // bf16: 248 us, with the gradients 743; one tile to a wave 292 and 936; at 64 columns two tiles leave two waves to a workgroup)
+    static constexpr int COLS = DC == 128 ? 2 : 1;
     static constexpr int WAVES = DC / 16 / COLS, THREADS = 64 * WAVES;
-    static constexpr int LEAST_WAVES = DA <= 64 && DC <= 64 ? 3 : 2;  // per SIMD: bounds the registers
     static constexpr int PAD = Tile<T>::PAD, SA = DA + PAD, SC = DC + PAD, SP = CH + PAD;
 };
 
@@ -246,7 +247,8 @@ __device__ __forceinline__ void walk_part(const Scan& s, int64_t unit, int64_t p
     typedef Shape<T, CH, DA, DC> S;
     typedef Tile<T> M;
     typedef typename M::Frag Frag;
-    constexpr bool AHEAD = !OUT || DA + DC < 256;  // whether the next chunk is on its way while one is computed: not where the registers end
+    // whether the next chunk is on its way while one is computed: not where the registers end (128 to 128, the figures above: ahead 259 and 791 us)
+    constexpr bool AHEAD = !OUT || DA + DC < 256;
     constexpr int KA = DA / M::K, KC = CH / M::K, DT = DA / 16, PER = M::K / 16;
     T *const tile_a = room.a, *const tile_b = room.b, *const tile_c = room.c, *const tile_p = room.p;
     float *const power = room.power, *const enter = room.enter, *const leave = room.leave;
@@ -823,8 +825,11 @@ __global__ __launch_bounds__((DK > DV ? DK : DV) * 4) void gradients_once(Walks 
 }
 
 // BOTH: the second and third walk have da and dc the other way round
+template <class T, int CH, int DA, int DC, bool BOTH>
+constexpr int SCAN_THREADS = BOTH && Shape<T, CH, DC, DA>::THREADS > Shape<T, CH, DA, DC>::THREADS ? Shape<T, CH, DC, DA>::THREADS : Shape<T, CH, DA, DC>::THREADS;
+
 template <class T, int CH, int DA, int DC, bool BOTH, bool OUT, int MODE>
-__global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS > Shape<T, CH, DC, DA>::THREADS && BOTH ? Shape<T, CH, DA, DC>::THREADS : BOTH ? Shape<T, CH, DC, DA>::THREADS : Shape<T, CH, DA, DC>::THREADS), (Shape<T, CH, DA, DC>::LEAST_WAVES)) void scan_chunks(Walks w) {
+__global__ __launch_bounds__((SCAN_THREADS<T, CH, DA, DC, BOTH>), 2) void scan_chunks(Walks w) {
     union Shared {
         Room<T, CH, DA, DC, OUT> one;
         Room<T, CH, BOTH ? DC : DA, BOTH ? DA : DC, OUT> other;
@@ -843,14 +848,18 @@ __global__ __launch_bounds__((Shape<T, CH, DA, DC>::THREADS > Shape<T, CH, DC, D
     }
 }
 
+// whether what comes with this length is one chunk at most
+template <class T, int CH>
+constexpr bool ONE_CHUNK = sizeof(T) == 2 && CH == 32;
+
 template <class T, int CH, int DA, int DC, bool BOTH, int MODE>
 int scan_launch(const Walks& w, hipStream_t stream) {
     const Scan& s = w.walk[0];
     const dim3 grid((unsigned)(s.envs * s.heads * s.parts * w.count));
-    constexpr int one = Shape<T, CH, DA, DC>::THREADS, other = BOTH ? Shape<T, CH, DC, DA>::THREADS : one, threads = one > other ? one : other;
+    constexpr int threads = SCAN_THREADS<T, CH, DA, DC, BOTH>;
     if (s.out.data)
         scan_chunks<T, CH, DA, DC, BOTH, true, MODE><<<grid, threads, 0, stream>>>(w);
-    else if constexpr (!BOTH)
+    else if constexpr (!BOTH && !ONE_CHUNK<T, CH>)  // (a part's state: there are many steps)
         scan_chunks<T, CH, DA, DC, false, false, MODE><<<grid, threads, 0, stream>>>(w);
     return launched();
 }
@@ -864,9 +873,10 @@ int once_launch(const Walks& w, hipStream_t stream) {
 
 template <class T, int CH, int DA, int DC, int MODE>
 int scan_mode(const Walks& w, bool swapped, hipStream_t stream) {
-    if constexpr (DA <= 64 && DC <= 64)
+    constexpr bool ONCE = DA <= 64 && DC <= 64;
+    if constexpr (ONCE)
         if (swapped && w.walk[0].steps <= CH) return once_launch<T, CH, DA, DC, MODE>(w, stream);
-    if constexpr (DA != DC)
+    if constexpr (DA != DC && !(ONCE && ONE_CHUNK<T, CH>))
         if (swapped) return scan_launch<T, CH, DA, DC, true, MODE>(w, stream);
     return scan_launch<T, CH, DA, DC, false, MODE>(w, stream);
 }
@@ -885,13 +895,23 @@ int scan_aligned(const Walks& w, bool swapped, hipStream_t stream) {
     return packs ? scan_mode<T, CH, DA, DC, 1>(w, swapped, stream) : scan_mode<T, CH, DA, DC, 0>(w, swapped, stream);
 }
 
-template <class T, int DA>
-int scan_rows(const Walks& w, bool swapped, hipStream_t stream) {
-    constexpr int CH = sizeof(T) == 4 ? 32 : 64;
+template <class T, int CH, int DA>
+int scan_columns(const Walks& w, bool swapped, hipStream_t stream) {
     const int dc = w.walk[0].dc;
     if (dc <= 32) return scan_aligned<T, CH, DA, 32>(w, swapped, stream);
     if (dc <= 64) return scan_aligned<T, CH, DA, 64>(w, swapped, stream);
     return scan_aligned<T, CH, DA, 128>(w, swapped, stream);
+}
+
+// Chunks of 32 tokens, and of 64 where there are more of bf16: scores cost CH instructions' worth a token, the state's rounding, update and barriers
+// 1 / CH.  32 : 64, forwards and with the gradients, us:  f32, 512 steps, 512 units of 64 to 64: 80 : 96, 268 : 351, 20 steps, 16384 units of 32 to
+// 32: 74 : 162, 215 : 411;  bf16, 4096 steps, 128 units of 128 to 128: 259 : 248, 777 : 743, 20 steps, 16384 units of 128 to 128: 340 : 343,
+// 909 : 1104, 64 to 64: 141 : 149, 345 : 367.
+template <class T, int DA>
+int scan_rows(const Walks& w, bool swapped, hipStream_t stream) {
+    if constexpr (sizeof(T) == 2)
+        if (w.walk[0].steps > 32) return scan_columns<T, 64, DA>(w, swapped, stream);
+    return scan_columns<T, 32, DA>(w, swapped, stream);
 }
 
 template int scan_rows<LOBPOLICY_TYPE, LOBPOLICY_ROWS>(const Walks&, bool, hipStream_t);

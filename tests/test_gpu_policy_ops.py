@@ -74,6 +74,18 @@ def test_attention_and_gradients(ops, size, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("steps", [1, 17, 31, 32, 33, 63, 64, 65])
+@pytest.mark.parametrize("widths", [(128, 128), (128, 24), (30, 100), (64, 32), (12, 7)], ids=str)
+def test_segments_about_a_chunk(ops, widths, steps, dtype):
+    """Segments as long as a chunk, one token shorter and longer; then with numbers that are none behind the sequences' ends, which computes token by token"""
+    p, dout, dlast = problem(steps + widths[1], steps, 5, 2, *widths, dtype, 0.1, True)
+    check(run(ops, p, dout, dlast), p, dout, dlast)
+    behind = torch.arange(steps, device="cuda")[:, None] >= p["lengths"][None]
+    dirty = {**p, **{key: torch.where(behind[:, :, None, None], math.nan, p[key]) for key in ("q", "k", "v")}}
+    check(run(ops, dirty, dout, dlast), p, dout, dlast)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("size", [(20, 9, 2, 32, 32), (64, 7, 1, 48, 80), (150, 6, 2, 64, 64), (257, 5, 1, 128, 128), (90, 5, 2, 7, 13), (30, 5, 2, 20, 50), (31, 5, 1, 50, 20), (32, 5, 1, 64, 64), (50, 4, 1, 5, 3), (28, 4, 1, 33, 64)], ids=str)
 def test_resets_and_lengths(ops, size, dtype):
     for resets, ragged in ((0.05, False), (0.0, True), (0.02, True), (0.6, True)):

@@ -50,7 +50,9 @@ struct Parts {
     int64_t bytes(const lobpolicy_attention* a) const { return count == 1 ? 0 : matrices(a) * (a->dk * a->dv + 1) * (int64_t)sizeof(float); }
 };
 
-// grid (elements / 256, units): `states` [unit][part] from what each part adds to what is in front of it; the state behind the last to state_out
+// grid (elements / 256, units): `states` [unit][part] from what each part adds to what is in front of it; the state behind the last to state_out.
+// Each element is a chain of its own over the parts, bound by the latency of its loads: 10 us for 8 units of 64 x 64 in 128 parts (30 us with each part's
+// load behind the one before), 19 us for 128 units of 128 x 128 in 4 (67 MB there and back).
 __global__ __launch_bounds__(256) void join_parts(Scan s, float* states, const float* __restrict__ carries) {
     const int64_t unit = blockIdx.y, matrix = (int64_t)s.da * s.dc, e = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (e >= matrix) return;
@@ -144,7 +146,9 @@ Scan scan_of(const lobpolicy_attention* a) {
 // decay attention, one token of every environment
 //
 // Reads and writes the state once: 8 dk dv bytes per environment and head, next to which the operands are nothing.  One workgroup per
-// environment and head; a thread holds VW neighbouring columns of every RG-th row, so that a wave moves whole rows.
+// environment and head; a thread holds VW neighbouring columns of every RG-th row, so that a wave moves whole rows.  Bound by memory: 4096
+// environments of 8 heads of 64 x 64 take 196 us (1.09 GB, 5.6 TB/s), 64 of 4 take 5 us, a launch's time.  The sum over the rows is in 32 bits, in
+// a fixed order: a group's rows, then the groups.
 
 struct Step {
     const void *q, *k, *v;
@@ -158,10 +162,12 @@ struct Step {
     float scale;
 };
 
-// RAG: dv is no multiple of VW: a row's last pack is loaded as its last VW elements and shifted
-template <class T, int VW, int LPR, bool RAG>
-__global__ __launch_bounds__(256) void step_kernel(Step s) {
-    constexpr int RG = 256 / LPR;
+// Rows of whole packs of 4 from a multiple of 16 bytes on, or elements: 61 x 59 of 4096 environments and 4 heads takes 75 us (6.3 TB/s) an element at a
+// time, 93 us in packs that begin anywhere.  A thread loads AT_ONCE rows before it stores one: a load behind a store waits for it, as far as the
+// compiler knows (100 x 101: 282 us, a row at a time 346).
+template <class T, int VW, int LPR, int THREADS>
+__global__ __launch_bounds__(THREADS) void step_kernel(Step s) {
+    constexpr int RG = THREADS / LPR, AT_ONCE = VW == 1 ? 8 : 4;
     __shared__ float part[RG][LPR * VW];
     const int64_t unit = blockIdx.x, n = unit / s.heads;
     const int h = (int)(unit % s.heads), col = (threadIdx.x % LPR) * VW, group = threadIdx.x / LPR;
@@ -169,76 +175,77 @@ __global__ __launch_bounds__(256) void step_kernel(Step s) {
     T* out = (T*)s.out + n * s.out_sn + h * s.out_sh;
     if (s.skip && s.skip[n]) {
         if (mine && group == 0)
-            for (int i = 0; i < VW; ++i)
-                if (!RAG || col + i < s.dv) out[col + i] = (T)0.f;
+            for (int i = 0; i < VW; ++i) out[col + i] = (T)0.f;
         return;
     }
     const T* q = (const T*)s.q + n * s.q_sn + h * s.q_sh;
     const T* k = (const T*)s.k + n * s.k_sn + h * s.k_sh;
     const T* v = (const T*)s.v + n * s.v_sn + h * s.v_sh;
-    const int from = RAG && col > s.dv - VW ? s.dv - VW : col;
-    float* state = s.state + unit * s.dk * s.dv;
+    typedef Pack<float, VW> P;
+    float* state = s.state + unit * s.dk * s.dv + col;
     const bool fresh = s.reset && s.reset[n * s.reset_sn];
     const float decay = expf(s.log_decay[h]);
     float value[VW], sum[VW];
 #pragma unroll
-    for (int i = 0; i < VW; ++i) value[i] = mine && (!RAG || col + i < s.dv) ? (float)v[col + i] : 0.f, sum[i] = 0.f;
-    if (mine) {
-#pragma unroll 4
-        for (int row = group; row < s.dk; row += RG) {
-            const float key = (float)k[row], query = (float)q[row];
-            Pack<float, VW> x;
-            if (fresh) {
+    for (int i = 0; i < VW; ++i) value[i] = mine ? (float)v[col + i] : 0.f, sum[i] = 0.f;
+    if (mine)
+        for (int first = group; first < s.dk; first += AT_ONCE * RG) {  // (rows behind the last are loaded as the last, and not used)
+            P x[AT_ONCE];
+            float key[AT_ONCE], query[AT_ONCE];
 #pragma unroll
-                for (int i = 0; i < VW; ++i) x.v[i] = 0.f;
-            } else if constexpr (RAG)
-                x = shifted(load_anywhere<float, VW>(state + row * s.dv + from), col - from);
-            else
-                x = *reinterpret_cast<const Pack<float, VW>*>(state + row * s.dv + col);
-#pragma unroll
-            for (int i = 0; i < VW; ++i) {
-                x.v[i] = x.v[i] * decay + key * value[i];
-                sum[i] += query * x.v[i];
+            for (int u = 0; u < AT_ONCE; ++u) {
+                const int row = min(first + u * RG, s.dk - 1);
+                key[u] = (float)k[row], query[u] = (float)q[row];
+                if (fresh)
+                    x[u] = P{};
+                else
+                    x[u] = *reinterpret_cast<const P*>(state + row * s.dv);
             }
-            if (!RAG)
-                *reinterpret_cast<Pack<float, VW>*>(state + row * s.dv + col) = x;
-            else if (col + VW <= s.dv)
-                store_anywhere(state + row * s.dv + col, x);
-            else {
 #pragma unroll
-                for (int i = 0; i < VW; ++i)
-                    if (col + i < s.dv) state[row * s.dv + col + i] = x.v[i];
+            for (int u = 0; u < AT_ONCE; ++u) {
+                const int row = first + u * RG;
+                if (row >= s.dk) break;
+#pragma unroll
+                for (int i = 0; i < VW; ++i) {
+                    x[u].v[i] = x[u].v[i] * decay + key[u] * value[i];
+                    sum[i] += query[u] * x[u].v[i];
+                }
+                *reinterpret_cast<P*>(state + row * s.dv) = x[u];
             }
         }
-    }
 #pragma unroll
     for (int i = 0; i < VW; ++i) part[group][(threadIdx.x % LPR) * VW + i] = sum[i];
     __syncthreads();
-    for (int c = threadIdx.x; c < s.dv; c += 256) {
+    for (int c = threadIdx.x; c < s.dv; c += THREADS) {
         float total = 0.f;
         for (int g = 0; g < RG; ++g) total += part[g][c];
         out[c] = (T)(total * s.scale);
     }
 }
 
+// elements of a state that one wave works on, rather than four: 16384 states of 16 x 16 13 and 20 us, 32 x 32 23 and 27, 48 x 48 48 both, 64 x 64 83 and 81
+constexpr int STEP_SMALL = 1024;
+
+template <class T, int VW, int LPR>
+int step_launch(const Step& s, int64_t units, hipStream_t stream) {
+    if (s.dk * s.dv <= STEP_SMALL)
+        step_kernel<T, VW, LPR, 64><<<dim3((unsigned)units), 64, 0, stream>>>(s);
+    else
+        step_kernel<T, VW, LPR, 256><<<dim3((unsigned)units), 256, 0, stream>>>(s);
+    return launched();
+}
+
 template <class T>
 int step_typed(const Step& s, int64_t units, hipStream_t stream) {
-    const dim3 grid((unsigned)units);
-    auto run = [&](auto lanes) {
-        constexpr int LPR = decltype(lanes)::value;
-        if (s.dv % 4 == 0 && aligned(s.state, 16))
-            step_kernel<T, 4, LPR, false><<<grid, 256, 0, stream>>>(s);
-        else
-            step_kernel<T, 4, LPR, true><<<grid, 256, 0, stream>>>(s);
-    };
-    if (s.dv < 4)
-        step_kernel<T, 1, 8, false><<<grid, 256, 0, stream>>>(s);
-    else if (s.dv <= 32)
-        run(std::integral_constant<int, 8>());
-    else if (s.dv <= 64)
-        run(std::integral_constant<int, 16>());
-    else
-        run(std::integral_constant<int, 32>());
+    if (s.dv % 4 == 0 && aligned(s.state, 16)) {
+        if (s.dv <= 32) return step_launch<T, 4, 8>(s, units, stream);
+        if (s.dv <= 64) return step_launch<T, 4, 16>(s, units, stream);
+        return step_launch<T, 4, 32>(s, units, stream);
+    }
+    if (s.dv <= 8) return step_launch<T, 1, 8>(s, units, stream);
+    if (s.dv <= 32) return step_launch<T, 1, 32>(s, units, stream);
+    if (s.dv <= 64) return step_launch<T, 1, 64>(s, units, stream);
+    step_kernel<T, 1, 128, 256><<<dim3((unsigned)units), 256, 0, stream>>>(s);
     return launched();
 }
 
@@ -246,7 +253,8 @@ int step_typed(const Step& s, int64_t units, hipStream_t stream) {
 // the block's end
 //
 // Bound by memory: every operand is read once and every result written once.  A row lives in the registers of one wave (width up to 1024)
-// or of one workgroup, VW neighbouring elements per thread and step, E elements per thread in all; the sums are 32-bit.
+// or of one workgroup, VW neighbouring elements per thread and step, E elements per thread in all; the sums are 32-bit.  65536 rows of 1024 (bf16):
+// 156 us forwards (671 MB, 4.3 TB/s; 64 M elements), 216 us backwards (1.07 GB, 5 TB/s), 7 us the weights' gradients; 64 rows of 256: 4 us.
 
 struct Block {
     const void *x, *block, *gate, *grad_y, *grad_z;
@@ -399,7 +407,8 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void block_forward_kernel(Bl
 //     dx  = f;   dgate = f res bn post sg (1 - sg);   db = (e - bn mean(e bn)) / rms(b),  e = f res sg post
 //     dpre = sum dz yn;   m = sum f sg bn:  dpost = res m,  dres = post m
 // y is worked out again from x, b and the gate, which costs no memory.  A workgroup keeps its share of the two column sums in registers
-// over all its rows and writes it once; column_sums adds the workgroups' shares in their order.
+// over all its rows and writes it once; column_sums adds the workgroups' shares in their order.  The next row is on its way while one is computed,
+// kept as it lies in memory (two rows of 32-bit numbers would not fit beside the sums).
 template <class X, class B, int VW, int E, int TPR, bool RAG>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void block_backward_kernel(Block p) {
     constexpr int RPB = TPR > 256 ? 1 : 256 / TPR;
@@ -539,19 +548,24 @@ int block_launch(const Block& p, int64_t parts, hipStream_t stream) {
 // LDS, every column sum in four times the threads); 4096 wide 512 threads 127 + 319, 1024 half of which are idle 251 + 673; 8192 wide, forwards
 // 1024 threads 155 (512: 185), backwards 512 threads 294 (1024, whose 128 registers do not hold a row and the next: 485).
 template <class X, class B, int VW, bool RAG, bool BACKWARD>
-int block_wide(const Block& p, int64_t parts, hipStream_t stream) {
-    if (p.width <= 64 * VW) return block_launch<X, B, VW, VW, 64, RAG, BACKWARD>(p, parts, stream);
-    if (p.width <= 512) return block_launch<X, B, VW, 8, 64, RAG, BACKWARD>(p, parts, stream);
+int block_long(const Block& p, int64_t parts, hipStream_t stream) {  // more than 512
     if constexpr (RAG) {  // (the shifted packs of 16 elements to a lane are more than the registers hold)
         if (p.width <= 1024) return block_launch<X, B, VW, 4, 256, RAG, BACKWARD>(p, parts, stream);
     } else if (p.width <= 1024)
         return block_launch<X, B, VW, 16, 64, RAG, BACKWARD>(p, parts, stream);
     if (p.width <= 2048) return block_launch<X, B, VW, 8, 256, RAG, BACKWARD>(p, parts, stream);
     if (p.width <= 4096) return block_launch<X, B, VW, 8, 512, RAG, BACKWARD>(p, parts, stream);
-    if constexpr (!RAG && BACKWARD)
+    if constexpr (!RAG && BACKWARD && VW > 1)
         return block_launch<X, B, VW, 16, 512, RAG, BACKWARD>(p, parts, stream);
     else
         return block_launch<X, B, VW, 8, 1024, RAG, BACKWARD>(p, parts, stream);
+}
+
+template <class X, class B, int VW, bool BACKWARD>
+int block_short(const Block& p, int64_t parts, hipStream_t stream) {  // up to 512
+    if constexpr (VW < 8)
+        if (p.width <= 256) return block_launch<X, B, VW, 4, 64, false, BACKWARD>(p, parts, stream);
+    return block_launch<X, B, VW, 8, 64, false, BACKWARD>(p, parts, stream);
 }
 
 template <class X, class B, bool BACKWARD>
@@ -563,12 +577,21 @@ int block_typed(const Block& p, int64_t parts, hipStream_t stream) {
         ok = ok && aligned(p.block, bs) && aligned(p.gate, bs) && aligned(p.z, bs) && aligned(p.grad_z, bs) && aligned(p.grad_block, bs) && aligned(p.grad_gate, bs);
         return ok && aligned(p.post, fs) && aligned(p.res, fs) && aligned(p.pre, fs) && aligned(p.partial, fs);
     };
-    // packs of 8 where a wave is full of them, else of 4; rows of no whole packs of 4 in shifted ones; 1024 wide, 65536 rows, forwards + backwards:
-    // packs of 8 130 + 264 us, of 4 143 + 826 (bf16), 163 + 349 and 170 + 777 (x f32), 203 + 510 and 186 + 498 (f32 only, where both are two loads)
-    if (p.width > 256 && fits(8)) return block_wide<X, B, 8, false, BACKWARD>(p, parts, stream);
-    if (fits(4)) return block_wide<X, B, 4, false, BACKWARD>(p, parts, stream);
-    if (p.width >= 4) return block_wide<X, B, 4, true, BACKWARD>(p, parts, stream);
-    return block_launch<X, B, 1, 4, 64, false, BACKWARD>(p, parts, stream);
+    // packs of 8 where a wave is full of them, else of 4; 1024 wide, 65536 rows, forwards + backwards: of 8 130 + 264 us, of 4 143 + 826 (bf16), 163 + 349
+    // and 170 + 777 (x f32), 203 + 510 and 186 + 498 (f32 only, where both are two loads).  Rows of no whole packs an element at a time (65536 rows of 330:
+    // 62 + 177 us, in packs that begin anywhere 67 + 205; f32 46 + 212 and 81 + 273), but for long ones of 16-bit numbers, where those are fewer
+    // instructions (8192 rows of 4001: 203 + 244 and 86 + 257; f32 100 + 306 and 125 + 350).
+    const bool pack8 = p.width > 256 && fits(8), pack4 = fits(4);
+    if (p.width <= 512) {
+        if (pack8) return block_short<X, B, 8, BACKWARD>(p, parts, stream);
+        return pack4 ? block_short<X, B, 4, BACKWARD>(p, parts, stream) : block_short<X, B, 1, BACKWARD>(p, parts, stream);
+    }
+    if (pack8) return block_long<X, B, 8, false, BACKWARD>(p, parts, stream);
+    if (pack4) return block_long<X, B, 4, false, BACKWARD>(p, parts, stream);
+    if constexpr (sizeof(X) == 4 && sizeof(B) == 4)
+        return block_long<X, B, 1, false, BACKWARD>(p, parts, stream);
+    else
+        return block_long<X, B, 4, true, BACKWARD>(p, parts, stream);
 }
 
 template <bool BACKWARD>
@@ -600,8 +623,9 @@ Block block_of(const lobpolicy_block* b) {
 // ---------------------------------------------------------------------------------------------------------------------------
 // the global norm, and clipping
 //
-// Two passes, each bound by memory (150 M values of both types, 457 MB: 99 us for the first, 4.6 TB/s, and 141 us for the second): the squares are summed in 64 bits (which neither overflows nor loses what many small gradients add),
-// one number per workgroup, in a fixed order; the second pass begins by adding those numbers up, in every workgroup alike, and scales.
+// Two passes, each bound by memory (150 M values of both types, 457 MB: 101 us for the first, 4.5 TB/s, and 141 us for the second, 6.5 TB/s of reads
+// and writes, of which the caches hold some): the squares are summed in 64 bits (which neither overflows nor loses what many small gradients add), one
+// number per workgroup, in a fixed order; the second pass begins by adding those numbers up, in every workgroup alike, and scales.
 // The tensors' table travels as a kernel argument: nothing is copied to the device, and a captured graph holds it.
 
 constexpr int CLIP_TENSORS = 128;        // per launch: 3 KB of arguments

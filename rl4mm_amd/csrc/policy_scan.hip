@@ -889,6 +889,8 @@ int scan_mode(const Walks& w, bool swapped, hipStream_t stream) {
     return scan_launch<T, CH, DA, DC, false, MODE>(w, stream);
 }
 
+// Whole packs of 16 bytes where every row begins and ends at one, packs that begin anywhere and shift their last where a row is one or longer (512 steps, 512
+// units of 61 to 61, forwards and with the gradients: bf16 56 + 170 us, an element at a time 98 + 328; f32 90 + 311 and 111 + 409), else elements
 template <class T, int CH, int DA, int DC>
 int scan_aligned(const Walks& w, bool swapped, hipStream_t stream) {
     constexpr int W = 16 / sizeof(T);

@@ -222,9 +222,10 @@ def decay_attention(q, k, v, log_decay, *, initial_state=None, reset=None, lengt
     if lengths is not None:
         _tensor(lengths, "lengths", (torch.int32,), q.device, (q.shape[1],))
         lengths = lengths.contiguous()
-    if q.shape[0] == 0 or q.shape[1] == 0:
-        state = torch.zeros((*q.shape[1:], v.shape[3]), dtype=torch.float32, device=q.device)
-        return v.clone(), state if initial_state is None else initial_state.clone()
+    if q.shape[0] == 0 or q.shape[1] == 0:  # (nothing to compute, and the gradients of what is empty are zeros: torch's own operations say so)
+        state = torch.zeros((*q.shape[1:], v.shape[3]), dtype=torch.float32, device=q.device) if initial_state is None else initial_state
+        nothing = 0.0 * (q.sum() + k.sum() + v.sum())
+        return v + nothing + 0.0 * state.sum().to(v.dtype), state + nothing.float()
     state = None if initial_state is None else initial_state.contiguous()
     args = (_lined(q), _lined(k), _lined(v), log_decay, state, reset, lengths, scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (state is not None and state.requires_grad)):
@@ -377,7 +378,7 @@ def clip_grad_norm(grads, max_norm, norm_type=2.0):
     grads: a tensor, or an iterable of tensors (None among them is passed over: a parameter without a gradient); float32 and bfloat16, mixed as you like, on
     one GPU, each dense in some order of its dimensions, no two of them overlapping.  norm_type 2.0: the root of the sum of all squares, summed in 64 bits
     in a fixed order; float("inf"): the largest magnitude.  A gradient that is not a number makes the norm one, and with it every gradient; an infinite
-    norm makes the finite ones 0.  No gradients: the norm is a CPU zero, as there is no device to put it on."""
+    norm makes the finite ones 0 (and with an infinite max_norm all of them not numbers, as the quotient is none).  No gradients: the norm is a CPU zero, as there is no device to put it on."""
     grads = [grads] if isinstance(grads, torch.Tensor) else [g for g in grads if g is not None]
     max_norm, norm_type = float(max_norm), float(norm_type)
     _need(max_norm >= 0.0, f"max_norm = {max_norm}: 0 or more")

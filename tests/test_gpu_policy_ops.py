@@ -275,6 +275,20 @@ def test_empty(ops):
     assert ops.decay_attention_step(q[0], q[0], v[0].detach(), decays(2), s.detach()).shape == (0, 2, 4)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(0, 3, 2), (5, 0, 2)], ids=str)
+def test_empty_reaches_every_operand(ops, shape, dtype):
+    """Each result of a segment without tokens has a gradient for each operand, like any other's: zeros, and the state's own."""
+    leaves = [normal(k, *shape, d, dtype=dtype).requires_grad_(True) for k, d in enumerate((8, 8, 4))] + [normal(3, shape[1], 2, 8, 4).requires_grad_(True)]
+    out, last = ops.decay_attention(*leaves[:3], decays(2), initial_state=leaves[3])
+    assert out.dtype == dtype and out.shape == (*shape, 4) and torch.equal(last, leaves[3])
+    for result, own in ((out, 0.0), (last, 1.0)):
+        grads = torch.autograd.grad(result.sum(), leaves, retain_graph=True)
+        assert all(g.shape == x.shape and g.dtype == x.dtype for g, x in zip(grads, leaves)) and torch.equal(grads[3], torch.full_like(grads[3], own))
+    out, last = ops.decay_attention(*leaves[:3], decays(2))
+    assert out.shape == (*shape, 4) and not last.any() and last.shape == (shape[1], 2, 8, 4)
+
+
 # ---- one token of every environment ----------------------------------------------------------------------------------------------
 
 

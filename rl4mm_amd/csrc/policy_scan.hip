@@ -571,7 +571,7 @@ __device__ __forceinline__ void walk_part(const Scan& s, int64_t unit, int64_t p
 //     dq_i = sum_j Z_ij k_j + scale l^(i+1) S0 do_i          dk_j = sum_i Z_ij q_i + l^(L-1-j) R v_j
 //     dv_j = sum_i A_ij do_i + l^(L-1-j) R^T k_j             dS0 = l^L R + scale sum_i l^(i+1) q_i do_i^T
 // Both score matrices lie in LDS by rows i: dq reads them by rows, dk and dv by columns.  Each wave has 16 columns of every result.  Three walks
-// read 9 operands instead of 4 and make 3 score matrices instead of 2: 20 steps x 4096 environments x 4 heads of 32 (f32) took 263 us that way, 193 us this.
+// read 9 operands instead of 4 and make 3 score matrices instead of 2: 20 steps x 4096 environments x 4 heads of 32 (f32) took 263 us that way, 181 us this (27 KB of LDS: 2.5 waves to a SIMD).
 // A chunk with an infinity or a NaN is left to the walks.
 
 template <class T, int CH, int DK, int DV>
@@ -619,6 +619,14 @@ __device__ __forceinline__ typename Tile<T>::Frag matrix_columns(__amdgpu_buffer
         f[e] = (T)__builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(buffer, i < rows ? (j < columns ? (i * columns + j) * 4 : 0x40000000) : 0x40000000, 0, 0));
     }
     return f;
+}
+
+// A kernel's first argument, read from memory from here on: what only a later part of the kernel needs is not kept in registers up to there
+template <class A>
+__device__ __forceinline__ const A& argument_again() {
+    auto from = (const __attribute__((address_space(4))) A*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(from));
+    return *(const A*)from;
 }
 
 template <class T, int CH, int DK, int DV, int MODE>
@@ -715,6 +723,7 @@ __global__ __launch_bounds__((DK > DV ? DK : DV) * 4) void gradients_once(Walks 
     __syncthreads();
     const bool by_walks = __builtin_amdgcn_readfirstlane(s.spoiled) != 0;
     if (by_walks) {  // (the walk with fewer waves last: the others have ended by then)
+        const Scan &of_v = argument_again<Walks>().walk[0], &of_k = argument_again<Walks>().walk[1], &of_q = argument_again<Walks>().walk[2];
         __syncthreads();
         constexpr int first = Shape<T, CH, DK, DV>::THREADS, others = Shape<T, CH, DV, DK>::THREADS;
         if (first >= others) {
@@ -743,6 +752,7 @@ __global__ __launch_bounds__((DK > DV ? DK : DV) * 4) void gradients_once(Walks 
         return x;
     };
     if (column < DK) {
+        const Scan &of_k = argument_again<Walks>().walk[1], &of_q = argument_again<Walks>().walk[2];
         T* to_q = (T*)of_q.out.data + n * of_q.out.sn + h * of_q.out.sh;
         T* to_k = (T*)of_k.out.data + n * of_k.out.sn + h * of_k.out.sh;
         Frag keys[KC], queries[KC];
@@ -773,10 +783,11 @@ __global__ __launch_bounds__((DK > DV ? DK : DV) * 4) void gradients_once(Walks 
                 store_columns<T, MODE>(to_k + i * of_k.out.st, column + 4 * at.g, dk, y);
             }
         }
-        for (int64_t t = length + lane / 16; t < of_v.steps; t += 4)
+        for (int64_t t = length + lane / 16; t < of_q.steps; t += 4)
             if (column + at.l < dk) to_q[t * of_q.out.st + column + at.l] = to_k[t * of_k.out.st + column + at.l] = (T)0.f;
     }
     if (column < DV) {
+        const Scan& of_v = argument_again<Walks>().walk[0];
         T* to = (T*)of_v.out.data + n * of_v.out.sn + h * of_v.out.sh;
         Frag values[KC];
 #pragma unroll

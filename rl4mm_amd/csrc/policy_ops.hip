@@ -51,7 +51,7 @@ struct Parts {
 };
 
 // grid (elements / 256, units): `states` [unit][part] from what each part adds to what is in front of it; the state behind the last to state_out.
-// Each element is a chain of its own over the parts, bound by the latency of its loads: 10 us for 8 units of 64 x 64 in 128 parts (30 us with each part's
+// Each element is a chain of its own over the parts, bound by the latency of its loads: 10 us for 8 units of 64 x 64 in 94 parts (30 us with each part's
 // load behind the one before), 19 us for 128 units of 128 x 128 in 4 (67 MB there and back).
 __global__ __launch_bounds__(256) void join_parts(Scan s, float* states, const float* __restrict__ carries) {
     const int64_t unit = blockIdx.y, matrix = (int64_t)s.da * s.dc, e = (int64_t)blockIdx.x * 256 + threadIdx.x;

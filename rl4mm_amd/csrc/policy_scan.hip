@@ -10,7 +10,7 @@ namespace lobpolicy {
 //     out_i = out_scale ( l^(i+1) a_i S + sum_{j <= i} l^(i-j) in_scale (a_i . b_j) c_j ),    S <- l^CH S + sum_j l^(CH-1-j) in_scale b_j c_j^T
 // where a reset between j and i takes the term away.  Four products of tiles, on 16x16 matrix instructions; one workgroup walks the
 // chunks of one environment and head (or of a part of its steps), its waves share the state by columns:
-//   - scores, transposed (rows j, columns i), weighted, rounded to T and put to LDS, each tile by one wave
+//   - scores, transposed (rows j, columns i), weighted and put to LDS as T, each tile by one wave
 //   - out, transposed (rows c, columns i), each wave its own columns of the state: S as it lies in the accumulators is the left operand
 //     of a_i S (an accumulator holds rows 4 (lane / 16) .. + 3 of column lane % 16, which read the other way round is the operand's
 //     layout), so the state never leaves the registers
@@ -23,8 +23,10 @@ namespace lobpolicy {
 // 0; a chunk that holds an infinity or a NaN anywhere is computed token by token instead, from the same LDS tiles, because a matrix
 // product would spread it to tokens that do not see it.
 //
-// bf16: the scores and the state's copy that multiplies a are rounded to bf16 once (half a step, 2^-8, of single terms, like the output's own
-// rounding); the state itself is kept in 32 bits, its update's weighted c split into three bf16 that together hold 24 bits.
+// bf16: what multiplies a bf16 operand is split, so that a result is rounded once, as it is stored: scores and the state's copy that multiplies a into two
+// bf16 (the number, and what its rounding leaves: off by 2^-16 of a term), the weighted c of the state's update, which adds up over all steps, into
+// three (24 bits).  The second halves cost, whole calls: 4500 steps, 128 units of 128 to 128, with the gradients, 815 -> 890 us, a fifth of it the scores'; 128
+// steps, 2048 units of 64 to 64, forwards, 50 -> 57 us in chunks of 64, where they leave LDS for three workgroups instead of four, and 48 us in chunks of 32.
 //
 // Few chunks are bound by what a chunk's products wait for in turn, many by the issue of instructions: at 128 to 128 (bf16, 4500 steps, 128 units, three
 // walks of the backward pass in one launch, 485 us) the matrix units work 20 %, the vector units 32 %, LDS 26 % of the time.  Forwards, us:
@@ -46,6 +48,16 @@ struct Lane {
     int l, g;
     __device__ __forceinline__ void fresh() { asm volatile("" : "+v"(l), "+v"(g)); }
 };
+
+// Two numbers rounded to bf16, and what that leaves of them
+__device__ __forceinline__ bf16x2 rounded(float& x, float& y) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    const bf16x2 two = __builtin_convertvector((f32x2{x, y}), bf16x2);
+    const uint32_t both = __builtin_bit_cast(uint32_t, two);
+    x -= __builtin_bit_cast(float, both << 16);
+    y -= __builtin_bit_cast(float, both & 0xffff0000u);
+    return two;
+}
 
 template <class T>
 struct Tile;
@@ -70,7 +82,8 @@ struct Tile<float> {  // a fragment: 16 of the summed index, places 4 (lane / 16
         return f;
     }
     static __device__ __forceinline__ int place(Lane at, int e) { return 4 * at.g + e; }  // of a fragment's element e in `columns`
-    static __device__ __forceinline__ Frag of_state(const f32x4* s) { return s[0]; }
+    static constexpr int HALVES = 1;  // fragments that hold 32-bit numbers where they multiply operands of T
+    static __device__ __forceinline__ void of_state(const f32x4* s, Frag* f) { f[0] = s[0]; }
     static constexpr int SPLITS = 1;
     // c's columns times w, as SPLITS fragments whose sum is the product
     static __device__ __forceinline__ void weighted(Frag c, const float* w, Frag* f) {
@@ -101,11 +114,17 @@ struct Tile<bf16> {  // a fragment: 32 of the summed index, places 8 (lane / 16)
         return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     }
     static __device__ __forceinline__ int place(Lane at, int e) { return 8 * at.g + e; }
-    static __device__ __forceinline__ Frag of_state(const f32x4* s) {
-        Frag f;
+    static constexpr int HALVES = 2;  // a number and what its rounding leaves, rounded: 17 bits
+    static __device__ __forceinline__ void of_state(const f32x4* s, Frag* f) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) f[r] = (bf16)s[0][r], f[4 + r] = (bf16)s[1][r];
-        return f;
+        for (int e = 0; e < 8; e += 2) {
+            float x = s[e / 4][e % 4], y = s[e / 4][e % 4 + 1];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const bf16x2 two = rounded(x, y);
+                f[half][e] = two[0], f[half][e + 1] = two[1];
+            }
+        }
     }
     static constexpr int SPLITS = 3;
     static __device__ __forceinline__ void weighted(Frag c, const float* w, Frag* f) {
@@ -236,6 +255,28 @@ struct Column {
     __device__ __forceinline__ void store(int i, float x) const { __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, x), buffer, offset(i), 0, 0); }
 };
 
+// 4 neighbouring scores to LDS: to each half, `apart` elements from one to the next; their sum are the scores
+template <class T>
+__device__ __forceinline__ void put_scores(T* to, int apart, f32x4 x) {
+#pragma unroll
+    for (int half = 0; half < Tile<T>::HALVES; ++half) {
+        Pack<T, 4> p;
+        if constexpr (Tile<T>::HALVES == 2) {
+#pragma unroll
+            for (int r = 0; r < 4; r += 2) {
+                float a = x[r], b = x[r + 1];
+                const bf16x2 two = rounded(a, b);
+                p.v[r] = two[0], p.v[r + 1] = two[1];
+                x[r] = a, x[r + 1] = b;
+            }
+        } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) p.v[r] = (T)x[r];
+        }
+        *reinterpret_cast<Pack<T, 4>*>(to + half * apart) = p;
+    }
+}
+
 // What a workgroup keeps in LDS
 template <class T, int CH, int DA, int DC, bool OUT>
 struct Room {
@@ -243,7 +284,7 @@ struct Room {
     alignas(16) T a[OUT ? CH * S::SA : 8];
     alignas(16) T b[CH * S::SA];
     alignas(16) T c[CH * S::SC];
-    alignas(16) T p[OUT ? CH * S::SP : 8];
+    alignas(16) T p[OUT ? Tile<T>::HALVES * CH * S::SP : 8];
     alignas(16) float leave[CH];              // l^(CH - 1 - j) in_scale
     float power[CH + 1], enter[CH + 1];       // l^k, and times out_scale
     uint32_t spoiled[2];
@@ -257,7 +298,7 @@ __device__ __forceinline__ void walk_part(const Scan& s, int64_t unit, int64_t p
     typedef typename M::Frag Frag;
     // whether the next chunk is on its way while one is computed: not where the registers end (128 to 128, the figures above: ahead 259 and 791 us)
     constexpr bool AHEAD = !OUT || DA + DC < 256;
-    constexpr int KA = DA / M::K, KC = CH / M::K, DT = DA / 16, PER = M::K / 16;
+    constexpr int KA = DA / M::K, KC = CH / M::K, DT = DA / 16, PER = M::K / 16, HALVES = M::HALVES, APART = CH * S::SP;
     T *const tile_a = room.a, *const tile_b = room.b, *const tile_c = room.c, *const tile_p = room.p;
     float *const power = room.power, *const enter = room.enter, *const leave = room.leave;
     uint32_t* const spoiled = room.spoiled;
@@ -387,15 +428,10 @@ __device__ __forceinline__ void walk_part(const Scan& s, int64_t unit, int64_t p
 #pragma unroll
                         for (int r = 0; r < 4; ++r) x[u][r] = 16 * jt[u] + 4 * at.g + r >= from ? x[u][r] : 0.f;
                     }
-                    Pack<T, 4> p;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) p.v[r] = (T)x[u][r];
-                    *reinterpret_cast<Pack<T, 4>*>(tile_p + i * S::SP + 16 * jt[u] + 4 * at.g) = p;
-                    if (PER == 2 && diagonal && it[u] % 2 == 0) {  // the tile above the diagonal that shares a fragment with it
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) p.v[r] = (T)0.f;
-                        *reinterpret_cast<Pack<T, 4>*>(tile_p + i * S::SP + 16 * jt[u] + 16 + 4 * at.g) = p;
-                    }
+                    T* to = tile_p + i * S::SP + 16 * jt[u] + 4 * at.g;
+                    put_scores(to, APART, x[u]);
+                    // the tile above the diagonal that shares a fragment with it
+                    if (PER == 2 && diagonal && it[u] % 2 == 0) put_scores(to + 16, APART, f32x4{0.f, 0.f, 0.f, 0.f});
                 }
             }
             if (spoils != 0.f) spoiled[parity] = 1;
@@ -406,11 +442,11 @@ __device__ __forceinline__ void walk_part(const Scan& s, int64_t unit, int64_t p
         auto token = [&](int p) { return (reverse ? length - 1 - (first + p) : first + p) * s.out.st; };
 
         if (OUT && !by_token) {
-            Frag left[S::COLS][KA];
+            Frag left[S::COLS][KA][HALVES];
 #pragma unroll
             for (int ct = 0; ct < S::COLS; ++ct)
 #pragma unroll
-                for (int kk = 0; kk < KA; ++kk) left[ct][kk] = M::of_state(&state[ct][kk * PER]);
+                for (int kk = 0; kk < KA; ++kk) M::of_state(&state[ct][kk * PER], left[ct][kk]);
             T* to = out + token(at.l);
             const int64_t on = (reverse ? -16 : 16) * s.out.st;
             float spoils = 0.f;
@@ -428,7 +464,9 @@ __device__ __forceinline__ void walk_part(const Scan& s, int64_t unit, int64_t p
                     for (int u = 0; u < 2; ++u) {
                         const Frag right = M::rows_as_state(at, tile_a, S::SA, 16 * (pair + u), kk * M::K);
 #pragma unroll
-                        for (int ct = 0; ct < S::COLS; ++ct) x[u][ct] = M::product(left[ct][kk], right, x[u][ct]);
+                        for (int ct = 0; ct < S::COLS; ++ct)
+#pragma unroll
+                            for (int half = 0; half < HALVES; ++half) x[u][ct] = M::product(left[ct][kk][half], right, x[u][ct]);
                     }
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
@@ -449,9 +487,12 @@ __device__ __forceinline__ void walk_part(const Scan& s, int64_t unit, int64_t p
 #pragma unroll
                     for (int u = 0; u < 2; ++u)
                         if (kk * PER <= pair + (PER == 2 ? 0 : u)) {
-                            const Frag right = M::rows(at, tile_p, S::SP, 16 * (pair + u), kk * M::K);
 #pragma unroll
-                            for (int ct = 0; ct < S::COLS; ++ct) x[u][ct] = M::product(values[ct][kk], right, x[u][ct]);
+                            for (int half = 0; half < HALVES; ++half) {
+                                const Frag right = M::rows(at, tile_p + half * APART, S::SP, 16 * (pair + u), kk * M::K);
+#pragma unroll
+                                for (int ct = 0; ct < S::COLS; ++ct) x[u][ct] = M::product(values[ct][kk], right, x[u][ct]);
+                            }
                         }
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
@@ -576,15 +617,25 @@ __device__ __forceinline__ void walk_part(const Scan& s, int64_t unit, int64_t p
 
 template <class T, int CH, int DK, int DV>
 struct OnceRoom {
-    static constexpr int SK = DK + Tile<T>::PAD, SV = DV + Tile<T>::PAD, SP = CH + Tile<T>::PAD;
-    alignas(16) T q[CH * SK], k[CH * SK], v[CH * SV], d[CH * SV], a[CH * SP], z[CH * SP];
+    static constexpr int SK = DK + Tile<T>::PAD, SV = DV + Tile<T>::PAD, SP = CH + Tile<T>::PAD, APART = CH * SP;
+    alignas(16) T q[CH * SK], k[CH * SK], v[CH * SV], d[CH * SV], a[Tile<T>::HALVES * APART], z[Tile<T>::HALVES * APART];
     float power[CH + 1];
     uint32_t spoiled;
 };
 
+// E floats as fragments of T, whose sum they are; what is not finite is the first one's alone
+template <class T, int E>
+__device__ __forceinline__ void in_halves(const float* x, typename Tile<T>::Frag* f) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        f[0][e] = (T)x[e];
+        if constexpr (Tile<T>::HALVES == 2) f[1][e] = (T)(__builtin_isfinite((float)f[0][e]) ? x[e] - (float)f[0][e] : 0.f);
+    }
+}
+
 // Fragments of a matrix of floats in memory, [rows][columns] without gaps (NULL: zeros), the summed index in the order of Tile::rows
 template <class T, bool VEC, int K>
-__device__ __forceinline__ typename Tile<T>::Frag matrix_rows(__amdgpu_buffer_rsrc_t buffer, Lane at, int rows, int columns, int row, int k) {
+__device__ __forceinline__ void matrix_rows(typename Tile<T>::Frag* f, __amdgpu_buffer_rsrc_t buffer, Lane at, int rows, int columns, int row, int k) {
     constexpr int E = K / 4;
     float x[E];
     const int i = row + at.l, j = k + E * at.g;
@@ -604,21 +655,18 @@ __device__ __forceinline__ typename Tile<T>::Frag matrix_rows(__amdgpu_buffer_rs
         for (int e = 0; e < E; ++e)
             x[e] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(buffer, i < rows ? (j + e < columns ? (i * columns + j + e) * 4 : 0x40000000) : 0x40000000, 0, 0));
     }
-    typename Tile<T>::Frag f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) f[e] = (T)x[e];
-    return f;
+    in_halves<T, E>(x, f);
 }
 template <class T, int K>
-__device__ __forceinline__ typename Tile<T>::Frag matrix_columns(__amdgpu_buffer_rsrc_t buffer, Lane at, int rows, int columns, int k, int column) {
+__device__ __forceinline__ void matrix_columns(typename Tile<T>::Frag* f, __amdgpu_buffer_rsrc_t buffer, Lane at, int rows, int columns, int k, int column) {
     constexpr int E = K / 4;
-    typename Tile<T>::Frag f;
+    float x[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
         const int i = k + E * at.g + e, j = column + at.l;
-        f[e] = (T)__builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(buffer, i < rows ? (j < columns ? (i * columns + j) * 4 : 0x40000000) : 0x40000000, 0, 0));
+        x[e] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(buffer, i < rows ? (j < columns ? (i * columns + j) * 4 : 0x40000000) : 0x40000000, 0, 0));
     }
-    return f;
+    in_halves<T, E>(x, f);
 }
 
 // A kernel's first argument, read from memory from here on: what only a later part of the kernel needs is not kept in registers up to there
@@ -634,7 +682,7 @@ __global__ __launch_bounds__((DK > DV ? DK : DV) * 4) void gradients_once(Walks 
     typedef Tile<T> M;
     typedef typename M::Frag Frag;
     typedef OnceRoom<T, CH, DK, DV> R;
-    constexpr int WAVES = (DK > DV ? DK : DV) / 16, THREADS = 64 * WAVES, PER = M::K / 16, KC = CH / M::K, KK = DK / M::K, KV = DV / M::K;
+    constexpr int WAVES = (DK > DV ? DK : DV) / 16, THREADS = 64 * WAVES, PER = M::K / 16, KC = CH / M::K, KK = DK / M::K, KV = DV / M::K, HALVES = M::HALVES;
     static_assert((Shape<T, CH, DK, DV>::THREADS > Shape<T, CH, DV, DK>::THREADS ? Shape<T, CH, DK, DV>::THREADS : Shape<T, CH, DV, DK>::THREADS) == THREADS, "");
     union Shared {
         R once;
@@ -668,14 +716,14 @@ __global__ __launch_bounds__((DK > DV ? DK : DV) * 4) void gradients_once(Walks 
     const bool with_s0 = of_q.state_in, with_r = of_v.state_in;
     const __amdgpu_buffer_rsrc_t s0 = __builtin_amdgcn_make_buffer_rsrc((void*)(of_q.state_in + (int64_t)unit * dk * dv), 0, with_s0 ? bytes : 0, 0x27000);
     const __amdgpu_buffer_rsrc_t rr = __builtin_amdgcn_make_buffer_rsrc((void*)(of_v.state_in + (int64_t)unit * dk * dv), 0, with_r ? bytes : 0, 0x27000);
-    Frag s0_rows[KV], r_rows[KV], r_columns[KK];
+    Frag s0_rows[KV][HALVES], r_rows[KV][HALVES], r_columns[KK][HALVES];
 #pragma unroll
     for (int kk = 0; kk < KV; ++kk) {
-        s0_rows[kk] = matrix_rows<T, MODE == 2, M::K>(s0, at, dk, dv, column, kk * M::K);
-        r_rows[kk] = matrix_rows<T, MODE == 2, M::K>(rr, at, dk, dv, column, kk * M::K);
+        matrix_rows<T, MODE == 2, M::K>(s0_rows[kk], s0, at, dk, dv, column, kk * M::K);
+        matrix_rows<T, MODE == 2, M::K>(r_rows[kk], rr, at, dk, dv, column, kk * M::K);
     }
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk) r_columns[kk] = matrix_columns<T, M::K>(rr, at, dk, dv, kk * M::K, column);
+    for (int kk = 0; kk < KK; ++kk) matrix_columns<T, M::K>(r_columns[kk], rr, at, dk, dv, kk * M::K, column);
 
     for (int k = threadIdx.x; k <= CH; k += THREADS) s.power[k] = k == 0 ? 1.f : expf(log_decay * (float)k);
     if (threadIdx.x == 0) s.spoiled = 0;
@@ -703,20 +751,16 @@ __global__ __launch_bounds__((DK > DV ? DK : DV) * 4) void gradients_once(Walks 
         const int from = before ? 63 - __builtin_clzll(before) : 0;  // the first place that i sees
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            T* tile = u ? s.z : s.a;
-            Pack<T, 4> p;
+            T* to = (u ? s.z : s.a) + i * R::SP + 16 * jt + 4 * at.g;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 spoils = fmaf(x[u][r], 0.f, spoils);
                 const float y = x[u][r] * (it == jt ? w_diagonal[r] : w_below[r] * far);
-                p.v[r] = (T)(16 * jt + 4 * at.g + r >= from ? y : 0.f);
+                x[u][r] = 16 * jt + 4 * at.g + r >= from ? y : 0.f;
             }
-            *reinterpret_cast<Pack<T, 4>*>(tile + i * R::SP + 16 * jt + 4 * at.g) = p;
-            if (PER == 2 && it == jt && it % 2 == 0) {  // the tile above the diagonal that shares a fragment with it
-#pragma unroll
-                for (int r = 0; r < 4; ++r) p.v[r] = (T)0.f;
-                *reinterpret_cast<Pack<T, 4>*>(tile + i * R::SP + 16 * jt + 16 + 4 * at.g) = p;
-            }
+            put_scores(to, R::APART, x[u]);
+            // the tile above the diagonal that shares a fragment with it
+            if (PER == 2 && it == jt && it % 2 == 0) put_scores(to + 16, R::APART, f32x4{0.f, 0.f, 0.f, 0.f});
         }
     }
     if (spoils != 0.f) s.spoiled = 1;
@@ -765,8 +809,12 @@ __global__ __launch_bounds__((DK > DV ? DK : DV) * 4) void gradients_once(Walks 
             f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int kk = 0; kk < KV; ++kk) {
-                x = M::product(s0_rows[kk], M::rows(at, s.d, R::SV, 16 * it, kk * M::K), x);
-                y = M::product(r_rows[kk], M::rows(at, s.v, R::SV, 16 * it, kk * M::K), y);
+                const Frag gradients = M::rows(at, s.d, R::SV, 16 * it, kk * M::K), values = M::rows(at, s.v, R::SV, 16 * it, kk * M::K);
+#pragma unroll
+                for (int half = 0; half < HALVES; ++half) {
+                    x = M::product(s0_rows[kk][half], gradients, x);
+                    y = M::product(r_rows[kk][half], values, y);
+                }
             }
             const float by = s.power[i + 1] * scale;
             const bool sees = (cuts & (~0ull >> (63 - i))) == 0;
@@ -775,8 +823,11 @@ __global__ __launch_bounds__((DK > DV ? DK : DV) * 4) void gradients_once(Walks 
             y = tail(i, y);
 #pragma unroll
             for (int kk = 0; kk < KC; ++kk) {
-                if (kk * PER <= it) x = M::product(keys[kk], M::rows(at, s.z, R::SP, 16 * it, kk * M::K), x);
-                if (kk * PER + PER > it && kk * PER < tiles) y = M::product(queries[kk], M::columns(at, s.z, R::SP, kk * M::K, 16 * it), y);
+#pragma unroll
+                for (int half = 0; half < HALVES; ++half) {
+                    if (kk * PER <= it) x = M::product(keys[kk], M::rows(at, s.z + half * R::APART, R::SP, 16 * it, kk * M::K), x);
+                    if (kk * PER + PER > it && kk * PER < tiles) y = M::product(queries[kk], M::columns(at, s.z + half * R::APART, R::SP, kk * M::K, 16 * it), y);
+                }
             }
             if (i < length) {
                 store_columns<T, MODE>(to_q + i * of_q.out.st, column + 4 * at.g, dk, x);
@@ -798,11 +849,18 @@ __global__ __launch_bounds__((DK > DV ? DK : DV) * 4) void gradients_once(Walks 
             const int j = 16 * jt + at.l;
             f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int kk = 0; kk < KK; ++kk) x = M::product(r_columns[kk], M::rows(at, s.k, R::SK, 16 * jt, kk * M::K), x);
+            for (int kk = 0; kk < KK; ++kk) {
+                const Frag keys = M::rows(at, s.k, R::SK, 16 * jt, kk * M::K);
+#pragma unroll
+                for (int half = 0; half < HALVES; ++half) x = M::product(r_columns[kk][half], keys, x);
+            }
             x = tail(j, x);
 #pragma unroll
             for (int kk = 0; kk < KC; ++kk)
-                if (kk * PER + PER > jt && kk * PER < tiles) x = M::product(values[kk], M::columns(at, s.a, R::SP, kk * M::K, 16 * jt), x);
+                if (kk * PER + PER > jt && kk * PER < tiles) {
+#pragma unroll
+                    for (int half = 0; half < HALVES; ++half) x = M::product(values[kk], M::columns(at, s.a + half * R::APART, R::SP, kk * M::K, 16 * jt), x);
+                }
             if (j < length) store_columns<T, MODE>(to + j * of_v.out.st, column + 4 * at.g, dv, x);
         }
         for (int64_t t = length + lane / 16; t < of_v.steps; t += 4)
@@ -867,9 +925,14 @@ __global__ __launch_bounds__((SCAN_THREADS<T, CH, DA, DC, BOTH>), 2) void scan_c
     }
 }
 
-// whether what comes with this length is one chunk at most
-template <class T, int CH>
-constexpr bool ONE_CHUNK = sizeof(T) == 2 && CH == 32;
+// Chunks of 32 tokens, of 64 where both widths of a bf16 state are above 64: scores cost CH instructions' worth a token and take CH * CH of LDS, the state's
+// rounding, update and barriers 1 / CH.  32 : 64, forwards or with the gradients (marked +), us:
+//     f32    512 steps, 512 units of 64 to 64: 80 : 96, +268 : 351;  20 steps, 16384 units of 32 to 32: 74 : 162, +215 : 411
+//     bf16   32 to 32: 4096 steps, 512 units +670 : 859, 128 steps, 8192 units +314 : 402;  64 to 64: 128 steps, 2048 units 49 : 57, 4096 steps, 512 units
+//            321 : 317, 1024 steps +282 : 295;  128 to 32: 1024 steps, 512 units 122 : 118, +388 : 450;  128 to 128: 4500 steps, 128 units +967 : 892,
+//            1024 steps, 512 units +705 : 671, 128 steps, 2048 units +500 : 485
+template <class T, int DA, int DC>
+constexpr bool LONG_CHUNKS = sizeof(T) == 2 && DA > 64 && DC > 64;
 
 template <class T, int CH, int DA, int DC, bool BOTH, int MODE>
 int scan_launch(const Walks& w, hipStream_t stream) {
@@ -878,7 +941,7 @@ int scan_launch(const Walks& w, hipStream_t stream) {
     constexpr int threads = SCAN_THREADS<T, CH, DA, DC, BOTH>;
     if (s.out.data)
         scan_chunks<T, CH, DA, DC, BOTH, true, MODE><<<grid, threads, 0, stream>>>(w);
-    else if constexpr (!BOTH && !ONE_CHUNK<T, CH>)  // (a part's state: there are many steps)
+    else if constexpr (!BOTH && (CH > 32 || !LONG_CHUNKS<T, DA, DC>))  // (a part's state: there are many steps)
         scan_chunks<T, CH, DA, DC, false, false, MODE><<<grid, threads, 0, stream>>>(w);
     return launched();
 }
@@ -892,10 +955,9 @@ int once_launch(const Walks& w, hipStream_t stream) {
 
 template <class T, int CH, int DA, int DC, int MODE>
 int scan_mode(const Walks& w, bool swapped, hipStream_t stream) {
-    constexpr bool ONCE = DA <= 64 && DC <= 64;
-    if constexpr (ONCE)
+    if constexpr (DA <= 64 && DC <= 64)
         if (swapped && w.walk[0].steps <= CH) return once_launch<T, CH, DA, DC, MODE>(w, stream);
-    if constexpr (DA != DC && !(ONCE && ONE_CHUNK<T, CH>))
+    if constexpr (DA != DC)
         if (swapped) return scan_launch<T, CH, DA, DC, true, MODE>(w, stream);
     return scan_launch<T, CH, DA, DC, false, MODE>(w, stream);
 }
@@ -916,23 +978,19 @@ int scan_aligned(const Walks& w, bool swapped, hipStream_t stream) {
     return packs ? scan_mode<T, CH, DA, DC, 1>(w, swapped, stream) : scan_mode<T, CH, DA, DC, 0>(w, swapped, stream);
 }
 
-template <class T, int CH, int DA>
+template <class T, int DA, int DC>
 int scan_columns(const Walks& w, bool swapped, hipStream_t stream) {
-    const int dc = w.walk[0].dc;
-    if (dc <= 32) return scan_aligned<T, CH, DA, 32>(w, swapped, stream);
-    if (dc <= 64) return scan_aligned<T, CH, DA, 64>(w, swapped, stream);
-    return scan_aligned<T, CH, DA, 128>(w, swapped, stream);
+    if constexpr (LONG_CHUNKS<T, DA, DC>)
+        if (w.walk[0].steps > 32) return scan_aligned<T, 64, DA, DC>(w, swapped, stream);
+    return scan_aligned<T, 32, DA, DC>(w, swapped, stream);
 }
 
-// Chunks of 32 tokens, and of 64 where there are more of bf16: scores cost CH instructions' worth a token, the state's rounding, update and barriers
-// 1 / CH.  32 : 64, forwards and with the gradients, us:  f32, 512 steps, 512 units of 64 to 64: 80 : 96, 268 : 351, 20 steps, 16384 units of 32 to
-// 32: 74 : 162, 215 : 411;  bf16, 4096 steps, 128 units of 128 to 128: 259 : 248, 777 : 743, 20 steps, 16384 units of 128 to 128: 340 : 343,
-// 909 : 1104, 64 to 64: 141 : 149, 345 : 367.
 template <class T, int DA>
 int scan_rows(const Walks& w, bool swapped, hipStream_t stream) {
-    if constexpr (sizeof(T) == 2)
-        if (w.walk[0].steps > 32) return scan_columns<T, 64, DA>(w, swapped, stream);
-    return scan_columns<T, 32, DA>(w, swapped, stream);
+    const int dc = w.walk[0].dc;
+    if (dc <= 32) return scan_columns<T, DA, 32>(w, swapped, stream);
+    if (dc <= 64) return scan_columns<T, DA, 64>(w, swapped, stream);
+    return scan_columns<T, DA, 128>(w, swapped, stream);
 }
 
 template int scan_rows<LOBPOLICY_TYPE, LOBPOLICY_ROWS>(const Walks&, bool, hipStream_t);

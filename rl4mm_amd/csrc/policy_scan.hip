@@ -152,15 +152,6 @@ struct Shape {
     static constexpr int PAD = Tile<T>::PAD, SA = DA + PAD, SC = DC + PAD, SP = CH + PAD;
 };
 
-// whether one of the 16 bytes' numbers has all exponent bits set
-template <class T>
-__device__ __forceinline__ uint32_t not_finite(uint4 x) {
-    constexpr uint32_t mask = sizeof(T) == 2 ? 0x7f807f80u : 0x7f800000u, one = sizeof(T) == 2 ? 0x00800080u : 0x00800000u;
-    return ((x.x & mask) + one) | ((x.y & mask) + one) | ((x.z & mask) + one) | ((x.w & mask) + one);
-}
-template <class T>
-constexpr uint32_t NOT_FINITE = sizeof(T) == 2 ? 0x80008000u : 0x80000000u;
-
 // A tile's share of a thread, on its way: CH places in the order of the walk, 16 bytes at a time.  `at` is the thread's first row in the chunk to be
 // loaded next, `step` the bytes from place to place (negative where the walk goes backwards).  Rows behind the last place are loaded from the
 // chunk's first row instead and become 0 when they are stored: a branch around a load would make the next wait one for every load.
@@ -215,12 +206,6 @@ struct Moving {
         if (!takes_part()) return;
 #pragma unroll
         for (int n = 0; n < N; ++n) *reinterpret_cast<Pack<T, VW>*>(tile + (first_row() + n * ROWS) * stride + column()) = x[n];
-    }
-    __device__ __forceinline__ uint32_t bad() const {  // of what was stored last
-        uint32_t any = 0;
-#pragma unroll
-        for (int n = 0; n < N; ++n) any |= not_finite<T>(__builtin_bit_cast(uint4, x[n]));
-        return takes_part() ? any : 0;
     }
 };
 
@@ -384,8 +369,6 @@ __device__ __forceinline__ void walk_part(const Scan& s, int64_t unit, int64_t p
         move_c.store(tile_c, S::SC, places);
         const uint64_t cuts = __ballot(has_flag(first) && flag != 0);
         any_cut |= cuts;
-        // (without outputs only a cut can take away what is not finite)
-        if (!OUT && cuts && ((move_b.bad() | move_c.bad()) & NOT_FINITE<T>)) spoiled[parity] = 1;
         __syncthreads();
         if (AHEAD && first + CH < end) load(first + CH);
         const int enters = reverse && first == 0 ? 0 : 1;  // decays between what comes into the chunk and its first place
@@ -437,8 +420,8 @@ __device__ __forceinline__ void walk_part(const Scan& s, int64_t unit, int64_t p
             if (spoils != 0.f) spoiled[parity] = 1;
             __syncthreads();
         }
-        bool by_token = __builtin_amdgcn_readfirstlane(spoiled[parity]) != 0;
-        if (threadIdx.x == 0) spoiled[parity ^ 1] = 0;
+        bool by_token = OUT && __builtin_amdgcn_readfirstlane(spoiled[parity]) != 0;
+        if (OUT && threadIdx.x == 0) spoiled[parity ^ 1] = 0;
         auto token = [&](int p) { return (reverse ? length - 1 - (first + p) : first + p) * s.out.st; };
 
         if (OUT && !by_token) {
@@ -479,7 +462,10 @@ __device__ __forceinline__ void walk_part(const Scan& s, int64_t unit, int64_t p
 #pragma unroll
                         for (int ct = 0; ct < S::COLS; ++ct)
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) x[u][ct][r] = sees ? x[u][ct][r] : 0.f;
+                            for (int r = 0; r < 4; ++r) {
+                                spoils = fmaf(x[u][ct][r], 0.f, spoils);  // (the last tile need not see the state)
+                                x[u][ct][r] = sees ? x[u][ct][r] : 0.f;
+                            }
                     }
                 }
 #pragma unroll
@@ -531,13 +517,11 @@ __device__ __forceinline__ void walk_part(const Scan& s, int64_t unit, int64_t p
                             const int i = 16 * t + 4 * at.g + r;
                             const float x = (cut ? 0.f : state[ct][t][r] * carry) + (float)tile_b[p * S::SA + i] * value;
                             state[ct][t][r] = i < s.da ? x : 0.f;
-                            if (OUT) sum += i < s.da ? (float)tile_a[p * S::SA + i] * x : 0.f;
+                            sum += i < s.da ? (float)tile_a[p * S::SA + i] * x : 0.f;
                         }
-                    if (OUT) {
-                        sum += __shfl_xor(sum, 16);
-                        sum += __shfl_xor(sum, 32);
-                        if (at.g == 0 && j < s.dc) out[token(p) + j] = (T)(sum * s.out_scale);
-                    }
+                    sum += __shfl_xor(sum, 16);
+                    sum += __shfl_xor(sum, 32);
+                    if (at.g == 0 && j < s.dc) out[token(p) + j] = (T)(sum * s.out_scale);
                 }
             }
         } else {
@@ -585,11 +569,51 @@ __device__ __forceinline__ void walk_part(const Scan& s, int64_t unit, int64_t p
         }
         __syncthreads();
     }
+    if (!OUT) {
+        // What is not finite has stayed in the state, or was cut off.  Whether it is infinite or no number at all is told by a walk of the wave's columns token
+        // by token: parts of an infinity, an infinity times decays whose product is 0 in 32 bits, and an infinity times the 0 of a cut are no numbers above
+        float spoils = 0.f;
+#pragma unroll
+        for (int ct = 0; ct < S::COLS; ++ct)
+#pragma unroll
+            for (int t = 0; t < DT; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) spoils = fmaf(state[ct][t][r], 0.f, spoils);
+        if (__ballot(spoils != 0.f)) {
+            const T *rows_b = (const T*)s.b.data + n * s.b.sn + h * s.b.sh, *rows_c = (const T*)s.c.data + n * s.c.sn + h * s.c.sh;
+#pragma unroll
+            for (int ct = 0; ct < S::COLS; ++ct)
+#pragma unroll
+                for (int t = 0; t < DT; ++t) state[ct][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+            for (int64_t place = begin; place < end; ++place) {
+                const int64_t token = reverse ? length - 1 - place : place;
+                const bool cut = s.reset && (!reverse || place > 0) && reset[(reverse ? length - place : place) * reset_st];
+                at.fresh();
+#pragma unroll
+                for (int ct = 0; ct < S::COLS; ++ct) {
+                    const int j = column + 16 * ct + at.l;
+                    const float value = j < s.dc ? (float)rows_c[token * s.c.st + j] * s.in_scale : 0.f;
+#pragma unroll
+                    for (int t = 0; t < DT; ++t)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const int i = 16 * t + 4 * at.g + r;
+                            if (i < s.da) state[ct][t][r] = (cut ? 0.f : state[ct][t][r] * power[1]) + (float)rows_b[token * s.b.st + i] * value;
+                        }
+                }
+            }
+        }
+    }
 
     if (OUT && part == s.parts - 1 && length < s.steps)  // rows behind the last token
         for (int64_t t = length + threadIdx.x / 32; t < s.steps; t += S::THREADS / 32)
             for (int j = threadIdx.x % 32; j < s.dc; j += 32) out[t * s.out.st + j] = (T)0.f;
-    if (!OUT && threadIdx.x == 0) s.carry_out[which] = any_cut ? -1.f : decay_of(begin < end ? (int)(end - begin) - (reverse && begin == 0 ? 1 : 0) : 0);
+    if (!OUT && threadIdx.x == 0) {
+        // the least number above 0 for a product of decays that is 0 in 32 bits: an infinite state stays infinite, and of a finite one less than 5e-7 is left
+        const float carry = decay_of(begin < end ? (int)(end - begin) - (reverse && begin == 0 ? 1 : 0) : 0);
+        s.carry_out[which] = any_cut ? -1.f : carry == 0.f && power[1] != 0.f ? 0x1p-149f : carry;
+    }
     if (s.state_out) {
         const bool leaves = reverse && s.parts == 1 && length > 0, cut = leaves && s.reset && reset[0];
         const float carry = leaves ? power[1] : 1.f;

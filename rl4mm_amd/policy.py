@@ -57,8 +57,11 @@ class SequencePolicy(torch.nn.Module):
         """The empty memory of ``envs`` environments: a state per block."""
         return [torch.zeros(envs, self.heads, self.head_dim, self.head_dim, dtype=torch.float32, device=self.log_decay.device) for _ in self.blocks]
 
-    def _walk(self, observations, attend):
-        x = self.embed((observations.float() - self.low) / self.span)
+    def _walk(self, observations, attend, behind=None):
+        scaled = (observations.float() - self.low) / self.span
+        if behind is not None:  # (times a gradient of 0, what is not finite or overflows on its way would be a gradient that is no number)
+            scaled = torch.where(behind[..., None], scaled.nan_to_num(0.0, 0.0, 0.0).clamp(-(2.0**16), 2.0**16), scaled)
+        x = self.embed(scaled)
         z = x * torch.rsqrt(x.square().mean(-1, keepdim=True) + self.eps) * self.first
         for i, block in enumerate(self.blocks):
             inner = self.heads * self.head_dim
@@ -75,15 +78,17 @@ class SequencePolicy(torch.nn.Module):
 
     def forward(self, observations, memory=None, reset=None, lengths=None):
         """observations [T, N, D] -> (actions float64 [T, N, A], values [T, N], the memory after the last step): differentiable.  reset [T, N]: where
-        episodes begin; lengths [N] int32: how many steps of each environment there are; memory: what came before (empty without one)."""
+        episodes begin; lengths [N] int32: how many steps of each environment there are; memory: what came before (empty without one).  Behind an
+        environment's last step the observations may hold anything; the actions and values there are finite and mean nothing: leave them out of the loss."""
         after = []
+        behind = None if lengths is None else torch.arange(observations.shape[0], device=observations.device)[:, None] >= lengths
 
         def attend(i, q, k, v):
             out, state = ops.decay_attention(q, k, v, self.log_decay, initial_state=None if memory is None else memory[i], reset=reset, lengths=lengths)
             after.append(state)
             return out
 
-        actions, values = self._walk(observations, attend)
+        actions, values = self._walk(observations, attend, behind)
         return actions, values, after
 
 

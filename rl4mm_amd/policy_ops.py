@@ -349,9 +349,8 @@ def gated_residual_norm(x, block, gate, post_weight, residual_scale, pre_weight,
     shape, wanted = x.shape, torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, block, gate, *weights))
     rows = [_rows(t, width) if t is not None else None for t in (x, block, gate)]
     if x.numel() == 0:  # (nothing to compute, and the gradients are zeros: torch's own operations say so)
-        y = rows[0] + 0.0 * sum(w.sum() for w in weights)
-        z = rows[1] + 0.0 * (rows[2] if gate is not None else rows[1])
-        return y.to(x.dtype).reshape(shape), z.to(block.dtype).reshape(shape)
+        nothing = 0.0 * sum(t.sum().float() for t in (*rows, *weights) if t is not None)
+        return tuple((t + nothing).to(t.dtype).reshape(shape) for t in rows[:2])
     args = (*rows, *(t.contiguous() for t in weights), eps)
     y, z = _GatedResidualNorm.apply(*args) if wanted else _block_forward(*args)
     return (y, z) if len(shape) == 2 else (y.view(shape), z.view(shape))

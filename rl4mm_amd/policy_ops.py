@@ -9,13 +9,15 @@ asynchronously on torch's current stream of the tensors' device, like the tensor
 float32 and bfloat16; states, norms and sums are float32 or wider.  There is no CPU path: CPU tensors raise, as does a missing
 library.  Every call can be captured into a graph (nothing waits for the device, nothing is allocated but results and workspaces, through
 torch's allocator); a forward and a backward pass belong into the same capture, with no eager graph of the same leaves alive beside it, as torch
-asks of every operation.  A call that cannot be right raises ValueError or TypeError before anything is launched."""
+asks of every operation.  torch.compile runs them between its graphs; forward-mode differentiation, torch.jit.trace and make_fx, which cannot see a
+launch, are refused.  A call that cannot be right raises ValueError or TypeError before anything is launched."""
 from __future__ import annotations
 
 import ctypes as C
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from . import _policy_capi as capi
@@ -58,6 +60,28 @@ def _call(device, name, *args):
             code = lib.fn[name](*args, stream)
     if code < 0:
         lib.check(code, name)
+
+
+_tracing, _modes = torch._C._is_tracing, torch._C._len_torch_dispatch_stack
+# the recorders that see operations before they are dispatched: the list itself, as looking it up takes longer than the rest of the check
+_early_modes = next(v for k, v in vars(torch._ops.mode_stack_state_for_pre_dispatch()).items() if k.endswith("infra_modes"))
+_NO_EARLY_MODES = [None] * len(_early_modes)
+
+
+def _seen(*tensors):
+    """Refuses what would pass the launches by without a word: tensors that carry a tangent, and recorders of torch's operations, whose record would lack them.
+    (torch.compile runs the operators as they are, between its graphs.)"""
+    if not _tracing() and not _modes() and _early_modes == _NO_EARLY_MODES and forward_ad._current_level < 0:
+        return
+    from torch._subclasses.fake_tensor import FakeTensor
+    from torch.fx.experimental.proxy_tensor import get_proxy_mode
+
+    _need(not _tracing(), "torch.jit.trace cannot record this operator: its launch would be missing from the trace")
+    _need(get_proxy_mode() is None, "make_fx cannot record this operator: its launch would be missing from the graph")
+    for t in tensors:
+        if t is not None:
+            _need(not isinstance(t, FakeTensor), "a fake tensor holds nothing to compute with", TypeError)
+            _need(forward_ad._current_level < 0 or forward_ad.unpack_dual(t).tangent is None, "forward-mode differentiation is not there: a tangent would be lost")
 
 
 def _new(t):
@@ -222,6 +246,7 @@ def decay_attention(q, k, v, log_decay, *, initial_state=None, reset=None, lengt
     if lengths is not None:
         _tensor(lengths, "lengths", (torch.int32,), q.device, (q.shape[1],))
         lengths = lengths.contiguous()
+    _seen(q, k, v, log_decay, initial_state)
     if q.shape[0] == 0 or q.shape[1] == 0:  # (nothing to compute, and the gradients of what is empty are zeros: torch's own operations say so)
         state = torch.zeros((*q.shape[1:], v.shape[3]), dtype=torch.float32, device=q.device) if initial_state is None else initial_state
         nothing = 0.0 * (q.sum() + k.sum() + v.sum())
@@ -245,6 +270,7 @@ def decay_attention_step(q, k, v, log_decay, state, *, reset=None, skip=None, sc
     _need(not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad)),
           "decay_attention_step has no gradient: call it under torch.no_grad(), or decay_attention for the gradients")  # fmt: skip
     reset, skip = _flags(reset, "reset", q.shape[:1], q.device), _flags(skip, "skip", q.shape[:1], q.device)
+    _seen(q, k, v, log_decay, state)
     out = _new(v)
     if q.shape[0] == 0:
         return out
@@ -346,6 +372,7 @@ def gated_residual_norm(x, block, gate, post_weight, residual_scale, pre_weight,
             _tensor(t, name, (torch.float32,), x.device, (width,))
     eps = float(eps)
     _need(math.isfinite(eps) and eps >= 2.0**-126, "eps is a positive number that 32 bits hold")
+    _seen(x, block, gate, *weights)
     shape, wanted = x.shape, torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, block, gate, *weights))
     rows = [_rows(t, width) if t is not None else None for t in (x, block, gate)]
     if x.numel() == 0:  # (nothing to compute, and the gradients are zeros: torch's own operations say so)
@@ -399,6 +426,7 @@ def clip_grad_norm(grads, max_norm, norm_type=2.0):
         if p < end:
             raise ValueError(f"gradients {min(i, last)} and {max(i, last)} share memory: each element is counted and scaled once")
         end, last = p + size, i
+    _seen(*grads)
     n = len(grads)
     tensors = (C.c_void_p * n)(*[g.data_ptr() for g in grads])
     counts, dtypes = (C.c_int64 * n)(*[g.numel() for g in grads]), (C.c_int32 * n)(*[_DTYPES[g.dtype] for g in grads])

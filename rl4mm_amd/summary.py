@@ -32,6 +32,14 @@ def policy_of(agent, action_dim: int, n_envs: int, n_steps: int):
     raise TypeError(f"no device policy for {type(agent).__name__}: step the env from the host (HistoricalOrderbookVectorEnv.vector_step)")
 
 
+def _note_end(venv, obs, reward, done) -> None:
+    """What the episodes ended with, on both of the env's paths: the finished envs sit out until they are reset, and their rows keep these values."""
+    t = venv._tensors()
+    t["obs"].copy_(obs), t["reward"].copy_(reward), t["done"].copy_(done)
+    venv._dones[:] = done.cpu().numpy().astype(bool)
+    venv._any_done = bool(venv._dones.any())
+
+
 def _policy_trajectories(policy, venv, T: int) -> Dict[str, np.ndarray]:
     """The episode of a SequencePolicy: its memory and actions on the device, one env step per action (T = 1 launches, whose trace row goes into the series)."""
     import torch
@@ -57,11 +65,10 @@ def _policy_trajectories(policy, venv, T: int) -> Dict[str, np.ndarray]:
                 cur.wait_stream(target)
             trace[k] = row[0]
             steps += active
+    finally:  # (also where the policy raises: the envs have stepped)
         torch.cuda.synchronize(dev)
-    finally:
         sim.set_trace_buffer(0, 0)
-    venv._dones[:] = done.cpu().numpy().astype(bool)
-    venv._any_done = bool(venv._dones.any())
+        _note_end(venv, obs, reward, done)
     return dict(steps=steps.cpu().numpy(), trace=trace.cpu().numpy(), observations=obs.cpu().numpy(), rewards=reward.cpu().numpy(), dones=done.cpu().numpy().astype(bool))
 
 
@@ -91,8 +98,7 @@ def generate_trajectories(agent, venv, n_steps: Optional[int] = None) -> Dict[st
         sim.sync()
     finally:
         sim.set_trace_buffer(0, 0)
-    venv._dones[:] = done.cpu().numpy().astype(bool)
-    venv._any_done = bool(venv._dones.any())
+    _note_end(venv, obs, reward, done)
     return dict(steps=steps.cpu().numpy(), trace=trace.cpu().numpy(), observations=obs.cpu().numpy(), rewards=reward.cpu().numpy(), dones=done.cpu().numpy().astype(bool))
 
 

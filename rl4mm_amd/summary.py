@@ -81,7 +81,8 @@ def generate_trajectories(agent, venv, n_steps: Optional[int] = None) -> Dict[st
 
     sim, n = venv.sim, venv.num_envs
     T = int(n_steps or round(venv.episode_length / venv.step_size))
-    if hasattr(agent, "memory") and hasattr(agent, "act"):  # (a SequencePolicy: its module needs torch)
+    # (a SequencePolicy, or what stands for one; a rule-based agent stays one, whatever else it can do)
+    if not isinstance(agent, (FixedActionAgent, Teradactyl, RandomAgent)) and callable(getattr(agent, "memory", None)) and callable(getattr(agent, "act", None)):
         return _policy_trajectories(agent, venv, T)
     venv.vector_reset()
     policy, params, acts = policy_of(agent, sim.action_dim, n, T)

@@ -7,6 +7,7 @@ from ._capi import LobsimError
 
 ABI_VERSION = 1  # LOBPOLICY_ABI_VERSION of the header this file mirrors
 MAX_HEAD, MAX_WIDTH = 128, 8192
+MAX_HEADS, MAX_UNITS, MAX_TENSORS = 1 << 16, 1 << 22, 1_000_000  # heads, environments x heads, tensors of one clip: what the entries check
 F32, BF16 = 0, 1
 
 

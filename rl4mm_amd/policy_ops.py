@@ -23,7 +23,7 @@ from . import _lib
 from . import _policy_capi as capi
 
 _DTYPES = {torch.float32: capi.F32, torch.bfloat16: capi.BF16}
-_NONE = capi.Operand(None, 0, 0, 0)
+_LARGEST = 2.0**128 - 2.0**104  # of the numbers of 32 bits
 
 
 _raw_stream = torch._C._cuda_getCurrentRawStream  # torch.cuda.current_stream(index).cuda_stream without the object around it
@@ -155,15 +155,16 @@ def _heads(q, k, v, log_decay, state, scale, dims):
         _tensor(k, "k", (q.dtype,), q.device, q.shape)
         _tensor(v, "v", (q.dtype,), q.device)
         _need(v.shape[:-1] == q.shape[:-1], f"v is [{', '.join(dims[:-1])}, dv] beside q {tuple(q.shape)}, got {tuple(v.shape)}")
-        heads, dk, dv = q.shape[-2], q.shape[-1], v.shape[-1]
+        shape, heads, dk, dv = q.shape, q.shape[-2], q.shape[-1], v.shape[-1]
         _need(heads >= 1 and 1 <= dk <= capi.MAX_HEAD and 1 <= dv <= capi.MAX_HEAD, f"{heads} heads of dk = {dk} and dv = {dv}: one head or more, dk and dv 1 to {capi.MAX_HEAD}")
         _tensor(log_decay, "log_decay", (torch.float32,), q.device, (heads,))
         _need(not log_decay.requires_grad, "log_decay takes no gradient: the decays are constants of the policy")
         if state is not None:
             _tensor(state, "the state", (torch.float32,), q.device, (q.shape[-3], heads, dk, dv))
         log_decay = log_decay.contiguous()
+    _need(heads <= capi.MAX_HEADS and shape[-3] * heads <= capi.MAX_UNITS, f"{shape[-3]} environments of {heads} heads: heads to {capi.MAX_HEADS}, environments x heads to {capi.MAX_UNITS}")
     scale = dk**-0.5 if scale is None else float(scale)
-    _need(math.isfinite(scale), "the scale is not finite")
+    _need(abs(scale) <= _LARGEST, f"the scale {scale} is not finite in 32 bits")
     return log_decay, scale
 
 
@@ -371,7 +372,7 @@ def gated_residual_norm(x, block, gate, post_weight, residual_scale, pre_weight,
         for t, name in zip(weights, ("post_weight", "residual_scale", "pre_weight")):
             _tensor(t, name, (torch.float32,), x.device, (width,))
     eps = float(eps)
-    _need(math.isfinite(eps) and eps >= 2.0**-126, "eps is a positive number that 32 bits hold")
+    _need(2.0**-126 <= eps <= _LARGEST, "eps is a positive number that 32 bits hold")
     _seen(x, block, gate, *weights)
     shape, wanted = x.shape, torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, block, gate, *weights))
     rows = [_rows(t, width) if t is not None else None for t in (x, block, gate)]
@@ -411,9 +412,10 @@ def clip_grad_norm(grads, max_norm, norm_type=2.0):
     _need(norm_type in (2.0, math.inf), f"norm_type = {norm_type}: 2 or inf")
     if not grads:
         return torch.zeros(())
+    _need(len(grads) <= capi.MAX_TENSORS, f"{len(grads)} gradients: {capi.MAX_TENSORS} at most")
     device, spans = getattr(grads[0], "device", None), []
     for i, g in enumerate(grads):
-        if not (type(g) is torch.Tensor and g.dtype in _DTYPES and g.device == device and g.is_cuda and not g.requires_grad and g.is_contiguous()):
+        if not (type(g) is torch.Tensor and g.dtype in _DTYPES and g.device == device and g.is_cuda and not g.requires_grad and g.layout is torch.strided and g.is_contiguous()):
             _tensor(g, f"gradient {i}", _DTYPES, device)
             _need(not g.requires_grad, f"gradient {i} requires a gradient itself: it is scaled outside autograd (detach it)")
             _need(_dense(g), f"gradient {i} is not dense in memory (shape {tuple(g.shape)}, strides {g.stride()}): it could not be scaled in place")

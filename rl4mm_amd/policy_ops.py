@@ -108,8 +108,8 @@ def _tensor(t, name, dtypes, device=None, shape=None):
 
 
 def _lined(t):
-    """`t`, its last dimension contiguous."""
-    return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
+    """`t`, its last dimension contiguous, and its memory what it says (the imaginary part of a conjugate is negated on the way, unless it has been copied)."""
+    return t.resolve_neg() if t.shape[-1] == 1 else t if t.stride(-1) == 1 else t.contiguous()
 
 
 def _operand(t):  # [T, N, H, D] or [N, H, D]

@@ -262,6 +262,7 @@ struct Block {
     const float *post, *res, *pre;
     void *y, *z, *grad_x, *grad_block, *grad_gate;
     float* partial;  // [2][gridDim.x][width]
+    int* parts;      // host: gridDim.x of the launch
     int64_t rows;
     int width;
     float eps;
@@ -546,18 +547,22 @@ __global__ __launch_bounds__(1024) void column_sums(const float* partial, int pa
 
 constexpr int64_t BLOCK_PARTS = 512;
 
-int block_rows(int64_t width) { return width <= 1024 ? 4 : 1; }  // rows a workgroup holds at once
-int64_t block_parts(const lobpolicy_block* b) {
-    const int64_t groups = ceil_div(b->rows, block_rows(b->width));
+// Workgroups of the backward pass.  A wave or a workgroup takes a row at a time, so at most 4 rows are in a workgroup at once, and one where the row needs more
+// than a wave: which kernel that is depends on the operands' alignment too, so the workspace is for the larger number.
+// 512 rows of 750 (bf16), whose 256 threads hold one row: 512 workgroups 8.3 + 6.9 us for their sums, 128 workgroups 16.3 + 3.8 us; 1000 rows 12.2 + 6.6, 17.6 + 4.1.
+int64_t backward_parts(int64_t rows, int64_t at_once) {
+    const int64_t groups = ceil_div(rows, at_once);
     return groups < BLOCK_PARTS ? groups : BLOCK_PARTS;
 }
+int64_t most_parts(const lobpolicy_block* b) { return backward_parts(b->rows, b->width <= 512 ? 4 : 1); }
 
 template <class X, class B, int VW, int E, int TPR, bool RAG, bool BACKWARD>
-int block_launch(const Block& p, int64_t parts, hipStream_t stream) {
+int block_launch(const Block& p, hipStream_t stream) {
     constexpr int threads = TPR > 256 ? TPR : 256;
-    if constexpr (BACKWARD)
-        block_backward_kernel<X, B, VW, E, TPR, RAG><<<dim3((unsigned)parts), threads, 0, stream>>>(p);
-    else {
+    if constexpr (BACKWARD) {
+        *p.parts = (int)backward_parts(p.rows, threads / TPR);
+        block_backward_kernel<X, B, VW, E, TPR, RAG><<<dim3((unsigned)*p.parts), threads, 0, stream>>>(p);
+    } else {
         const int64_t groups = ceil_div(p.rows, threads / TPR);
         block_forward_kernel<X, B, VW, E, TPR, RAG><<<dim3((unsigned)(groups < (1 << 20) ? groups : (1 << 20))), threads, 0, stream>>>(p);
     }
@@ -569,28 +574,28 @@ int block_launch(const Block& p, int64_t parts, hipStream_t stream) {
 // LDS, every column sum in four times the threads); 4096 wide 512 threads 127 + 319, 1024 half of which are idle 251 + 673; 8192 wide, forwards
 // 1024 threads 155 (512: 185), backwards 512 threads 294 (1024, whose 128 registers do not hold a row and the next: 485).
 template <class X, class B, int VW, bool RAG, bool BACKWARD>
-int block_long(const Block& p, int64_t parts, hipStream_t stream) {  // more than 512
+int block_long(const Block& p, hipStream_t stream) {  // more than 512
     if constexpr (RAG) {  // (the shifted packs of 16 elements to a lane are more than the registers hold)
-        if (p.width <= 1024) return block_launch<X, B, VW, 4, 256, RAG, BACKWARD>(p, parts, stream);
+        if (p.width <= 1024) return block_launch<X, B, VW, 4, 256, RAG, BACKWARD>(p, stream);
     } else if (p.width <= 1024)
-        return block_launch<X, B, VW, 16, 64, RAG, BACKWARD>(p, parts, stream);
-    if (p.width <= 2048) return block_launch<X, B, VW, 8, 256, RAG, BACKWARD>(p, parts, stream);
-    if (p.width <= 4096) return block_launch<X, B, VW, 8, 512, RAG, BACKWARD>(p, parts, stream);
+        return block_launch<X, B, VW, 16, 64, RAG, BACKWARD>(p, stream);
+    if (p.width <= 2048) return block_launch<X, B, VW, 8, 256, RAG, BACKWARD>(p, stream);
+    if (p.width <= 4096) return block_launch<X, B, VW, 8, 512, RAG, BACKWARD>(p, stream);
     if constexpr (!RAG && BACKWARD && VW > 1)
-        return block_launch<X, B, VW, 16, 512, RAG, BACKWARD>(p, parts, stream);
+        return block_launch<X, B, VW, 16, 512, RAG, BACKWARD>(p, stream);
     else
-        return block_launch<X, B, VW, 8, 1024, RAG, BACKWARD>(p, parts, stream);
+        return block_launch<X, B, VW, 8, 1024, RAG, BACKWARD>(p, stream);
 }
 
 template <class X, class B, int VW, bool BACKWARD>
-int block_short(const Block& p, int64_t parts, hipStream_t stream) {  // up to 512
+int block_short(const Block& p, hipStream_t stream) {  // up to 512
     if constexpr (VW < 8)
-        if (p.width <= 256) return block_launch<X, B, VW, 4, 64, false, BACKWARD>(p, parts, stream);
-    return block_launch<X, B, VW, 8, 64, false, BACKWARD>(p, parts, stream);
+        if (p.width <= 256) return block_launch<X, B, VW, 4, 64, false, BACKWARD>(p, stream);
+    return block_launch<X, B, VW, 8, 64, false, BACKWARD>(p, stream);
 }
 
 template <class X, class B, bool BACKWARD>
-int block_typed(const Block& p, int64_t parts, hipStream_t stream) {
+int block_typed(const Block& p, hipStream_t stream) {
     auto fits = [&](int w) {
         const int64_t xs = w * sizeof(X) < 16 ? w * sizeof(X) : 16, bs = w * sizeof(B) < 16 ? w * sizeof(B) : 16, fs = w * 4 < 16 ? w * 4 : 16;
         bool ok = p.width % w == 0 && p.x_sr % w == 0 && p.block_sr % w == 0 && p.gate_sr % w == 0 && p.grad_y_sr % w == 0 && p.grad_z_sr % w == 0;
@@ -604,23 +609,23 @@ int block_typed(const Block& p, int64_t parts, hipStream_t stream) {
     // instructions (8192 rows of 4001: 203 + 244 and 86 + 257; f32 100 + 306 and 125 + 350).
     const bool pack8 = p.width > 256 && fits(8), pack4 = fits(4);
     if (p.width <= 512) {
-        if (pack8) return block_short<X, B, 8, BACKWARD>(p, parts, stream);
-        return pack4 ? block_short<X, B, 4, BACKWARD>(p, parts, stream) : block_short<X, B, 1, BACKWARD>(p, parts, stream);
+        if (pack8) return block_short<X, B, 8, BACKWARD>(p, stream);
+        return pack4 ? block_short<X, B, 4, BACKWARD>(p, stream) : block_short<X, B, 1, BACKWARD>(p, stream);
     }
-    if (pack8) return block_long<X, B, 8, false, BACKWARD>(p, parts, stream);
-    if (pack4) return block_long<X, B, 4, false, BACKWARD>(p, parts, stream);
+    if (pack8) return block_long<X, B, 8, false, BACKWARD>(p, stream);
+    if (pack4) return block_long<X, B, 4, false, BACKWARD>(p, stream);
     if constexpr (sizeof(X) == 4 && sizeof(B) == 4)
-        return block_long<X, B, 1, false, BACKWARD>(p, parts, stream);
+        return block_long<X, B, 1, false, BACKWARD>(p, stream);
     else
-        return block_long<X, B, 4, true, BACKWARD>(p, parts, stream);
+        return block_long<X, B, 4, true, BACKWARD>(p, stream);
 }
 
 template <bool BACKWARD>
-int block_any(const lobpolicy_block* b, const Block& p, int64_t parts, void* stream) {
+int block_any(const lobpolicy_block* b, const Block& p, void* stream) {
     hipStream_t s = (hipStream_t)stream;
     if (b->stream_dtype == LOBPOLICY_F32)
-        return b->dtype == LOBPOLICY_F32 ? block_typed<float, float, BACKWARD>(p, parts, s) : block_typed<float, bf16, BACKWARD>(p, parts, s);
-    return b->dtype == LOBPOLICY_F32 ? block_typed<bf16, float, BACKWARD>(p, parts, s) : block_typed<bf16, bf16, BACKWARD>(p, parts, s);
+        return b->dtype == LOBPOLICY_F32 ? block_typed<float, float, BACKWARD>(p, s) : block_typed<float, bf16, BACKWARD>(p, s);
+    return b->dtype == LOBPOLICY_F32 ? block_typed<bf16, float, BACKWARD>(p, s) : block_typed<bf16, bf16, BACKWARD>(p, s);
 }
 
 int check_block(const lobpolicy_block* b) {
@@ -957,7 +962,7 @@ int lobpolicy_attention_step(const lobpolicy_attention* a, void* stream) {
 
 int64_t lobpolicy_block_workspace(const lobpolicy_block* b) {
     if (int e = check_block(b)) return e;
-    return 2 * block_parts(b) * b->width * (int64_t)sizeof(float);
+    return 2 * most_parts(b) * b->width * (int64_t)sizeof(float);
 }
 
 int lobpolicy_block_forward(const lobpolicy_block* b, void* stream) {
@@ -965,7 +970,7 @@ int lobpolicy_block_forward(const lobpolicy_block* b, void* stream) {
     REQUIRE(b->y && b->z, "a result is missing");
     Block p = block_of(b);
     p.y = b->y, p.z = b->z;
-    return block_any<false>(b, p, 0, stream);
+    return block_any<false>(b, p, stream);
 }
 
 int lobpolicy_block_backward(const lobpolicy_block* b, void* stream) {
@@ -976,9 +981,10 @@ int lobpolicy_block_backward(const lobpolicy_block* b, void* stream) {
     p.grad_y = b->grad_y, p.grad_z = b->grad_z, p.grad_y_sr = b->grad_y ? b->grad_y_stride : 0, p.grad_z_sr = b->grad_z ? b->grad_z_stride : 0;
     p.grad_x = b->grad_x, p.grad_block = b->grad_block, p.grad_gate = b->grad_gate;
     p.partial = (float*)b->workspace;
-    const int64_t parts = block_parts(b);
-    if (int e = block_any<true>(b, p, parts, stream)) return e;
-    column_sums<<<dim3((unsigned)ceil_div(b->width, 32), 2), 1024, 0, (hipStream_t)stream>>>(p.partial, (int)parts, p.width, b->post, b->res, b->grad_post, b->grad_res, b->grad_pre);
+    int parts = 0;
+    p.parts = &parts;
+    if (int e = block_any<true>(b, p, stream)) return e;
+    column_sums<<<dim3((unsigned)ceil_div(b->width, 32), 2), 1024, 0, (hipStream_t)stream>>>(p.partial, parts, p.width, b->post, b->res, b->grad_post, b->grad_res, b->grad_pre);
     return launched();
 }
 

@@ -776,9 +776,10 @@ __global__ __launch_bounds__(256) void clip_kernel(ClipTable t, const double* pa
     }
 }
 
-// Few values: one workgroup does both passes in one launch, each quarter of it a chunk at a time.  100 000 values in 4 tensors take 6.7 us, 130 000
-// take 9.0 us; two launches take 4.4 + 4.5 us and the gap between them, and a program that calls one after the other is through with a policy of
-// 70 000 values in 16.3 us a call instead of 19.9.
+// Few values: one workgroup does both passes in one launch, each quarter of it a chunk at a time.  What that saves is the second launch, which a program pays for that
+// calls it as it goes along; in a captured graph, where launches are cheap, the kernel alone counts, which from 8 chunks on is slower than the two.  One
+// launch : two, us a call, eager and in a graph: 1000 values 12.9 : 15.3 and 3.0 : 4.1; 65 536 11.2 : 14.2 and 4.9 : 5.0; six tensors of 69 636 in 13 chunks
+// 16.6 : 19.7 and 6.3 : 5.1; 131 072 11.4 : 14.1 and 7.0 : 5.0.  The rule is for the eager call, and by the sizes alone, so that both give the same bits.
 template <bool MAX>
 __global__ __launch_bounds__(1024) void clip_few_kernel(ClipTable t, double max_norm, float* norm_out) {
     __shared__ double shared[16];

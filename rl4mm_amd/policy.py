@@ -8,6 +8,8 @@ the same function:
             place, forgotten where an episode begins, left alone where an environment is done
   forward   recorded segments [T, N] at once, differentiable: what an update trains on
 
+Parameters and memories are float32; under ``torch.autocast("cuda", torch.bfloat16)`` the projections, and with them the operators, work in bfloat16.
+
 ``update`` takes a step of any torch optimizer with the gradients clipped by their global norm, and
 ``summary.generate_trajectories`` / ``get_episode_summary_dict`` evaluate the policy like the rule-based agents."""
 from __future__ import annotations

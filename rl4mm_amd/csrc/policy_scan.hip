@@ -630,7 +630,7 @@ __device__ __forceinline__ void walk_part(const Scan& s, int64_t unit, int64_t p
 
 // ---- short segments: all three gradients at once -----------------------------------------------------------------------------
 //
-// Where the steps are one chunk, a workgroup reads q, k, v and do once and writes dq, dk, dv and the gradient of the initial state: with
+// Where the steps are one chunk of 32, a workgroup reads q, k, v and do once and writes dq, dk, dv and the gradient of the initial state: with
 // A = l^(i-j) scale (q_i . k_j) and Z = l^(i-j) scale (do_i . v_j), lower triangles without what a reset cuts, S0 the initial state, R the gradient
 // of the final one,
 //     dq_i = sum_j Z_ij k_j + scale l^(i+1) S0 do_i          dk_j = sum_i Z_ij q_i + l^(L-1-j) R v_j
@@ -639,8 +639,9 @@ __device__ __forceinline__ void walk_part(const Scan& s, int64_t unit, int64_t p
 // read 9 operands instead of 4 and make 3 score matrices instead of 2: 20 steps x 4096 environments x 4 heads of 32 (f32) took 263 us that way, 181 us this (27 KB of LDS: 2.5 waves to a SIMD).
 // A chunk with an infinity or a NaN is left to the walks.
 
-template <class T, int CH, int DK, int DV>
+template <class T, int DK, int DV>
 struct OnceRoom {
+    static constexpr int CH = 32;
     static constexpr int SK = DK + Tile<T>::PAD, SV = DV + Tile<T>::PAD, SP = CH + Tile<T>::PAD, APART = CH * SP;
     alignas(16) T q[CH * SK], k[CH * SK], v[CH * SV], d[CH * SV], a[Tile<T>::HALVES * APART], z[Tile<T>::HALVES * APART];
     float power[CH + 1];
@@ -701,11 +702,12 @@ __device__ __forceinline__ const A& argument_again() {
     return *(const A*)from;
 }
 
-template <class T, int CH, int DK, int DV, int MODE>
+template <class T, int DK, int DV, int MODE>
 __global__ __launch_bounds__((DK > DV ? DK : DV) * 4) void gradients_once(Walks w) {
     typedef Tile<T> M;
     typedef typename M::Frag Frag;
-    typedef OnceRoom<T, CH, DK, DV> R;
+    typedef OnceRoom<T, DK, DV> R;
+    constexpr int CH = R::CH;
     constexpr int WAVES = (DK > DV ? DK : DV) / 16, THREADS = 64 * WAVES, PER = M::K / 16, KC = CH / M::K, KK = DK / M::K, KV = DV / M::K, HALVES = M::HALVES;
     static_assert((Shape<T, CH, DK, DV>::THREADS > Shape<T, CH, DV, DK>::THREADS ? Shape<T, CH, DK, DV>::THREADS : Shape<T, CH, DV, DK>::THREADS) == THREADS, "");
     union Shared {
@@ -764,13 +766,12 @@ __global__ __launch_bounds__((DK > DV ? DK : DV) * 4) void gradients_once(Walks 
     float spoils = 0.f;  // becomes NaN with the first number that is none, or infinite
     const int count = tiles * (tiles + 1) / 2;
     for (int k0 = wave; k0 < count; k0 += WAVES) {
-        const int it = k0 >= 6 ? 3 : k0 >= 3 ? 2 : k0 >= 1 ? 1 : 0, jt = k0 - it * (it + 1) / 2, i = 16 * it + at.l;
+        const int it = k0 >= 1 ? 1 : 0, jt = k0 == 2 ? 1 : 0, i = 16 * it + at.l;
         f32x4 x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) x[0] = M::product(M::rows(at, s.k, R::SK, 16 * jt, kk * M::K), M::rows(at, s.q, R::SK, 16 * it, kk * M::K), x[0]);
 #pragma unroll
         for (int kk = 0; kk < KV; ++kk) x[1] = M::product(M::rows(at, s.v, R::SV, 16 * jt, kk * M::K), M::rows(at, s.d, R::SV, 16 * it, kk * M::K), x[1]);
-        const float far = it - jt > 1 ? s.power[16 * (it - jt - 1)] : 1.f;
         const uint64_t before = cuts & (~0ull >> (63 - i));
         const int from = before ? 63 - __builtin_clzll(before) : 0;  // the first place that i sees
 #pragma unroll
@@ -779,7 +780,7 @@ __global__ __launch_bounds__((DK > DV ? DK : DV) * 4) void gradients_once(Walks 
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 spoils = fmaf(x[u][r], 0.f, spoils);
-                const float y = x[u][r] * (it == jt ? w_diagonal[r] : w_below[r] * far);
+                const float y = x[u][r] * (it == jt ? w_diagonal[r] : w_below[r]);
                 x[u][r] = 16 * jt + 4 * at.g + r >= from ? y : 0.f;
             }
             put_scores(to, R::APART, x[u]);
@@ -970,17 +971,17 @@ int scan_launch(const Walks& w, hipStream_t stream) {
     return launched();
 }
 
-template <class T, int CH, int DK, int DV, int MODE>
+template <class T, int DK, int DV, int MODE>
 int once_launch(const Walks& w, hipStream_t stream) {
     const Scan& s = w.walk[0];
-    gradients_once<T, CH, DK, DV, MODE><<<dim3((unsigned)(s.envs * s.heads)), (DK > DV ? DK : DV) * 4, 0, stream>>>(w);
+    gradients_once<T, DK, DV, MODE><<<dim3((unsigned)(s.envs * s.heads)), (DK > DV ? DK : DV) * 4, 0, stream>>>(w);
     return launched();
 }
 
 template <class T, int CH, int DA, int DC, int MODE>
 int scan_mode(const Walks& w, bool swapped, hipStream_t stream) {
     if constexpr (DA <= 64 && DC <= 64)
-        if (swapped && w.walk[0].steps <= CH) return once_launch<T, CH, DA, DC, MODE>(w, stream);
+        if (swapped && w.walk[0].steps <= CH) return once_launch<T, DA, DC, MODE>(w, stream);
     if constexpr (DA != DC)
         if (swapped) return scan_launch<T, CH, DA, DC, true, MODE>(w, stream);
     return scan_launch<T, CH, DA, DC, false, MODE>(w, stream);

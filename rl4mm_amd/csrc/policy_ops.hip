@@ -28,20 +28,25 @@ int scan_typed(const Walks& w, bool swapped, hipStream_t stream) {
 
 // Few environments and heads, many steps: the steps are split into parts.  A first walk finds what each part adds to the state, join_parts
 // turns that into the state in front of each part, a second walk starts from it.  That reads k and v twice, so it pays where the chip is
-// otherwise far from full, and then only until it is full.  Whole against split, forwards, in us:
-//     widths of 32 to 32 (bf16): 4096 steps, 32 units 202 : 29, 256 units 202 : 106, 384 units 235 : 192, 512 units 238 : 224, with the gradients 586 : 669
-//     64 to 64 (bf16): 4096 steps, 32 units 227 : 44, 128 units 227 : 112, 256 units 229 : 252;  128 to 128: 128 units 404 : 249, 256 units 428 : 456
-//     64 to 64 (f32): 128 units 365 : 232, 256 units 369 : 409
-// 512 and 1024 workgroups in all: 112 and 115 us (bf16, 128 units of 64 to 64), 89 and 62 us (32 to 32), 264 and 246 us (f32, 18000 steps of 32
-// units of 64 to 64), 88 and 98 us (bf16, 18000 steps of 8 units of 128 to 128).  Below 512 steps the two
-// further launches take what the parts save (256 steps of 64 to 64, 32 units: 20 : 24, at 512 steps 34 : 25).
+// otherwise far from full, and then only until it is full: as many parts as fit, not one more (100 units of 128 to 128 in 5 parts 239 us, in 6, of which
+// the last 88 workgroups run by themselves, 299).  Whole against split, us in a graph, forwards / with the gradients:
+//     32 to 32, bf16:   4096 steps, 32 units 234 : 30, 256 units 235 : 119, 384 units 265 : 186 / 580 : 589;  512 steps, 192 units 36 : 27 / 77 : 62
+//     64 to 64, bf16:   4096 steps, 75 units 275 : 85 / 550 : 247, 192 units 279 : 189 / 650 : 556, 220 units 278 : 218 / 656 : 603;  1024 steps, 192 units 77 : 64 / 182 : 172,
+//                       220 units 78 : 67 / 185 : 195;  512 steps, 100 units 41 : 34 / 89 : 80, 150 units 41 : 38 / 91 : 98
+//     64 to 64, f32:    4096 steps, 192 units 389 : 358 / 1156 : 1047, 220 units 392 : 411 / 1165 : 1194;  512 steps, 100 units 55 : 45 / 135 : 117, 150 units 56 : 57 / 140 : 157
+//     128 to 128, bf16: 4096 steps, 75 units 474 : 196 / 944 : 599, 150 units 484 : 359 / 1100 : 1107, 192 units 493 : 473 / 1500 : 1404;  1024 steps, 100 units 120 : 88 / 276 : 257,
+//                       192 units 127 : 145 / 394 : 433;  512 steps, 75 units 65 : 56 / 133 : 147, 100 units 65 : 61 / 154 : 178, 150 units 67 : 80 / 160 : 230
+//     128 to 128, f32:  4096 steps, 150 units 970 : 803 / 2566 : 2671, 192 units 983 : 1140 / 3498 : 3503
+// 512 and 1024 workgroups in all, the latter where they are small: 64 to 64, bf16, 4096 steps, 128 units 139 : 125 / 386 : 366; 32 to 32, 256 units 197 : 119; 128 to 128, 128
+// units 292 : 322.  Below 512 steps the two further launches take what the parts save (256 steps of 64 to 64, 32 units: 22.1 : 22.8 / 44.6 : 47.7; at 512 steps 39.5 : 24.5).
 struct Parts {
     int64_t steps;
     int count;
     Parts(const lobpolicy_attention* a) {
         const int widest = a->dk > a->dv ? a->dk : a->dv;
-        const int64_t units = a->envs * a->heads, wanted = widest <= (a->dtype == LOBPOLICY_F32 ? 64 : 32) ? 1024 : 512;
-        int64_t n = a->steps < 512 || units >= (widest <= 32 ? 384 : 256) ? 1 : ceil_div(wanted, units);
+        const int64_t units = a->envs * a->heads, wanted = widest <= 64 ? 1024 : 512;
+        const int64_t most = widest <= 32 ? 384 : (widest <= 64 ? 208 : 160) / (a->steps < 1024 ? 2 : 1);  // units
+        int64_t n = a->steps < 512 || units >= most ? 1 : wanted / units;
         n = n < ceil_div(a->steps, 128) ? n : ceil_div(a->steps, 128);
         steps = ceil_div(ceil_div(a->steps, n), 64) * 64;
         count = (int)ceil_div(a->steps, steps);

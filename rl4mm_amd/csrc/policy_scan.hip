@@ -951,11 +951,10 @@ __global__ __launch_bounds__((SCAN_THREADS<T, CH, DA, DC, BOTH>), 2) void scan_c
 }
 
 // Chunks of 32 tokens, of 64 where both widths of a bf16 state are above 64: scores cost CH instructions' worth a token and take CH * CH of LDS, the state's
-// rounding, update and barriers 1 / CH.  32 : 64, forwards or with the gradients (marked +), us:
-//     f32    512 steps, 512 units of 64 to 64: 80 : 96, +268 : 351;  20 steps, 16384 units of 32 to 32: 74 : 162, +215 : 411
-//     bf16   32 to 32: 4096 steps, 512 units +670 : 859, 128 steps, 8192 units +314 : 402;  64 to 64: 128 steps, 2048 units 49 : 57, 4096 steps, 512 units
-//            321 : 317, 1024 steps +282 : 295;  128 to 32: 1024 steps, 512 units 122 : 118, +388 : 450;  128 to 128: 4500 steps, 128 units +967 : 892,
-//            1024 steps, 512 units +705 : 671, 128 steps, 2048 units +500 : 485
+// rounding, update and barriers 1 / CH.  32 : 64, us in a graph, forwards or (+) with the gradients:
+//     f32    512 steps, 512 units of 64 to 64 94 : 110, +310 : 392, of 32 to 32 +163 : 223
+//     bf16   32 to 32: 4096 steps, 512 units +703 : 856, 128 steps, 8192 units +312 : 403;  64 to 64: 128 steps, 2048 units 49 : 55, 4096 steps, 512 units 349 : 343;
+//            128 to 32: 1024 steps, 512 units 129 : 129, +404 : 461;  128 to 128: 4500 steps, 128 units +964 : 930, 1024 steps, 512 units +713 : 677
 template <class T, int DA, int DC>
 constexpr bool LONG_CHUNKS = sizeof(T) == 2 && DA > 64 && DC > 64;
 
@@ -981,7 +980,7 @@ int once_launch(const Walks& w, hipStream_t stream) {
 template <class T, int CH, int DA, int DC, int MODE>
 int scan_mode(const Walks& w, bool swapped, hipStream_t stream) {
     if constexpr (DA <= 64 && DC <= 64)
-        if (swapped && w.walk[0].steps <= CH) return once_launch<T, DA, DC, MODE>(w, stream);
+        if (swapped && w.walk[0].steps <= 32) return once_launch<T, DA, DC, MODE>(w, stream);
     if constexpr (DA != DC)
         if (swapped) return scan_launch<T, CH, DA, DC, true, MODE>(w, stream);
     return scan_launch<T, CH, DA, DC, false, MODE>(w, stream);

@@ -38,7 +38,9 @@ typedef struct lobpolicy_operand {
 
 /* Decay attention.  Of every environment n and head h, with a state S [dk][dv] (float32):
  *     S = reset[t][n] ? 0 : S;   S = exp(log_decay[h]) S + k_t v_t^T;   out_t = scale q_t^T S          t = 0 .. min(lengths[n], steps) - 1
- * Rows t >= lengths[n] are not read; their rows of out, dq, dk and dv are set to 0. */
+ * Rows t >= lengths[n] are not used; their rows of out, dq, dk and dv are set to 0.  A bfloat16 result is rounded once, as it is stored: sums and the
+ * state are float32, scores and the state where they multiply a bfloat16 operand two bfloat16 each.  An infinite operand gives infinities and not-numbers as the
+ * formula has them, however the steps are split. */
 typedef struct lobpolicy_attention {
     int32_t dtype; /* of q, k, v, out and their gradients */
     int32_t heads, dk, dv;

@@ -29,16 +29,16 @@ int scan_typed(const Walks& w, bool swapped, hipStream_t stream) {
 // Few environments and heads, many steps: the steps are split into parts.  A first walk finds what each part adds to the state, join_parts
 // turns that into the state in front of each part, a second walk starts from it.  That reads k and v twice, so it pays where the chip is
 // otherwise far from full, and then only until it is full: as many parts as fit, not one more (100 units of 128 to 128 in 5 parts 239 us, in 6, of which
-// the last 88 workgroups run by themselves, 299).  Whole against split, us in a graph, forwards / with the gradients:
-//     32 to 32, bf16:   4096 steps, 32 units 234 : 30, 256 units 235 : 119, 384 units 265 : 186 / 580 : 589;  512 steps, 192 units 36 : 27 / 77 : 62
-//     64 to 64, bf16:   4096 steps, 75 units 275 : 85 / 550 : 247, 192 units 279 : 189 / 650 : 556, 220 units 278 : 218 / 656 : 603;  1024 steps, 192 units 77 : 64 / 182 : 172,
-//                       220 units 78 : 67 / 185 : 195;  512 steps, 100 units 41 : 34 / 89 : 80, 150 units 41 : 38 / 91 : 98
-//     64 to 64, f32:    4096 steps, 192 units 389 : 358 / 1156 : 1047, 220 units 392 : 411 / 1165 : 1194;  512 steps, 100 units 55 : 45 / 135 : 117, 150 units 56 : 57 / 140 : 157
-//     128 to 128, bf16: 4096 steps, 75 units 474 : 196 / 944 : 599, 150 units 484 : 359 / 1100 : 1107, 192 units 493 : 473 / 1500 : 1404;  1024 steps, 100 units 120 : 88 / 276 : 257,
-//                       192 units 127 : 145 / 394 : 433;  512 steps, 75 units 65 : 56 / 133 : 147, 100 units 65 : 61 / 154 : 178, 150 units 67 : 80 / 160 : 230
-//     128 to 128, f32:  4096 steps, 150 units 970 : 803 / 2566 : 2671, 192 units 983 : 1140 / 3498 : 3503
-// 512 and 1024 workgroups in all, the latter where they are small: 64 to 64, bf16, 4096 steps, 128 units 139 : 125 / 386 : 366; 32 to 32, 256 units 197 : 119; 128 to 128, 128
-// units 292 : 322.  Below 512 steps the two further launches take what the parts save (256 steps of 64 to 64, 32 units: 22.1 : 22.8 / 44.6 : 47.7; at 512 steps 39.5 : 24.5).
+// the last 88 workgroups run by themselves, 299).  Whole : split, us in a graph, forwards and with the gradients:
+//     32 to 32, bf16:   4096 steps, 32 units 233 : 30, 256 units 236 : 119, 384 units 267 : 227 and 597 : 621;  512 steps, 192 units 35 : 28 and 76 : 63
+//     64 to 64, bf16:   4096 steps, 75 units 275 : 82 and 553 : 238, 192 units 278 : 177 and 649 : 529, 220 units 279 : 215 and 653 : 592;  1024 steps, 192 units 77 : 59 and
+//                       181 : 170, 220 units 78 : 67 and 185 : 190;  512 steps, 100 units 41 : 33 and 89 : 79, 150 units 41 : 37 and 91 : 98
+//     64 to 64, f32:    4096 steps, 192 units 388 : 350 and 1153 : 1028, 220 units 397 : 405 and 1166 : 1179;  512 steps, 100 units 55 : 45 and 135 : 115, 150 units 56 : 57 and 138 : 155
+//     128 to 128, bf16: 4096 steps, 75 units 476 : 192 and 946 : 577, 150 units 486 : 347 and 1102 : 1069, 192 units 493 : 460 and 1497 : 1386;  1024 steps, 100 units 120 : 88 and
+//                       277 : 256, 192 units 127 : 142 and 396 : 434;  512 steps, 75 units 64 : 56 and 134 : 147, 100 units 65 : 60 and 153 : 173, 150 units 68 : 78 and 159 : 228
+//     128 to 128, f32:  4096 steps, 150 units 972 : 803 and 2558 : 2666, 192 units 984 : 1140 and 3457 : 3485
+// 512 : 1024 workgroups in all, the latter where they are small: 4096 steps, 128 units of 64 to 64 (bf16) 139 : 124 and 380 : 368, 256 units of 32 to 32 200 : 120, 128 units of
+// 128 to 128 292 : 310 and 837 : 915.  Below 512 steps the two further launches take what the parts save (256 steps of 64 to 64, 32 units: 22.2 : 23.0; 512 steps: 39.0 : 25.3).
 struct Parts {
     int64_t steps;
     int count;
@@ -152,7 +152,7 @@ Scan scan_of(const lobpolicy_attention* a) {
 //
 // Reads and writes the state once: 8 dk dv bytes per environment and head, next to which the operands are nothing.  One workgroup per
 // environment and head; a thread holds VW neighbouring columns of every RG-th row, so that a wave moves whole rows.  Bound by memory: 4096
-// environments of 8 heads of 64 x 64 take 187 us (1.09 GB, 5.8 TB/s), 64 of 4 take 4.5 us, a launch's time.  The sum over the rows is in 32 bits, in
+// environments of 8 heads of 64 x 64 take 189 us (1.09 GB, 5.8 TB/s), 64 of 4 take 4.3 us, a launch's time.  The sum over the rows is in 32 bits, in
 // a fixed order: a group's rows, then the groups.
 
 struct Step {
@@ -228,7 +228,7 @@ __global__ __launch_bounds__(THREADS) void step_kernel(Step s) {
     }
 }
 
-// elements of a state that one wave works on, rather than four: 16384 states of 16 x 16 13 and 20 us, 32 x 32 23 and 27, 48 x 48 48 both, 64 x 64 83 and 81
+// elements of a state that one wave works on, rather than four: 16384 states of 16 x 16 10.9 and 21.7 us, 32 x 32 23 and 32, 48 x 48 48 both, 64 x 64 87 and 83
 constexpr int STEP_SMALL = 1024;
 
 template <class T, int VW, int LPR>
@@ -259,7 +259,7 @@ int step_typed(const Step& s, int64_t units, hipStream_t stream) {
 //
 // Bound by memory: every operand is read once and every result written once.  A row lives in the registers of one wave (width up to 1024)
 // or of one workgroup, VW neighbouring elements per thread and step, E elements per thread in all; the sums are 32-bit.  65536 rows of 1024 (bf16):
-// 156 us forwards (671 MB, 4.3 TB/s; 64 M elements), 216 us backwards (1.07 GB, 5 TB/s), 7 us the weights' gradients; 64 rows of 256: 4 us.
+// 155 us forwards (671 MB, 4.3 TB/s; 64 M elements), 219 us backwards (1.07 GB, 4.9 TB/s), 7 us the weights' gradients; 64 rows of 256: 4 us.
 
 struct Block {
     const void *x, *block, *gate, *grad_y, *grad_z;
@@ -574,10 +574,10 @@ int block_launch(const Block& p, hipStream_t stream) {
     return launched();
 }
 
-// A row to a wave as long as its registers hold it, then to as many threads as it needs: idle threads cost as much as busy ones.  Both gradients
-// and results of 64 M elements in us, forwards + backwards (bf16): 1024 wide a wave to a row 130 + 264, 256 threads to a row 172 + 523 (sums through
-// LDS, every column sum in four times the threads); 4096 wide 512 threads 127 + 319, 1024 half of which are idle 251 + 673; 8192 wide, forwards
-// 1024 threads 155 (512: 185), backwards 512 threads 294 (1024, whose 128 registers do not hold a row and the next: 485).
+// A row to a wave as long as its registers hold it, then to as many threads as it needs: idle threads cost as much as busy ones.  64 M elements (bf16), us in a
+// graph, forwards and with the gradients: 1024 wide a wave to a row 151 and 365, 256 threads to a row 208 and 639 (sums through LDS, every column sum in four
+// times the threads); 4096 wide 512 threads 158 and 415, without them (1024 forwards, half of which are idle, 512 of 16 elements backwards) 295 and 605; 8192 wide,
+// forwards 1024 threads 190 (512: 230), with the gradients, which take 512, 436 (1024, whose 128 registers do not hold a row and the next: 640 - 230 + 190 = 600).
 template <class X, class B, int VW, bool RAG, bool BACKWARD>
 int block_long(const Block& p, hipStream_t stream) {  // more than 512
     if constexpr (RAG) {  // (the shifted packs of 16 elements to a lane are more than the registers hold)
@@ -608,10 +608,10 @@ int block_typed(const Block& p, hipStream_t stream) {
         ok = ok && aligned(p.block, bs) && aligned(p.gate, bs) && aligned(p.z, bs) && aligned(p.grad_z, bs) && aligned(p.grad_block, bs) && aligned(p.grad_gate, bs);
         return ok && aligned(p.post, fs) && aligned(p.res, fs) && aligned(p.pre, fs) && aligned(p.partial, fs);
     };
-    // packs of 8 where a wave is full of them, else of 4; 1024 wide, 65536 rows, forwards + backwards: of 8 130 + 264 us, of 4 143 + 826 (bf16), 163 + 349
-    // and 170 + 777 (x f32), 203 + 510 and 186 + 498 (f32 only, where both are two loads).  Rows of no whole packs an element at a time (65536 rows of 330:
-    // 62 + 177 us, in packs that begin anywhere 67 + 205; f32 46 + 212 and 81 + 273), but for long ones of 16-bit numbers, where those are fewer
-    // instructions (8192 rows of 4001: 203 + 244 and 86 + 257; f32 100 + 306 and 125 + 350).
+    // packs of 8 where a wave is full of them, else of 4; 1024 wide, 65536 rows, forwards and with the gradients, of 8 : of 4: 151 : 165 and 365 : 977 us (bf16), 191 : 194
+    // and 474 : 937 (x f32), 254 : 238 and 664 : 645 (f32 only, where both are two loads, and of 4 are 2 to 5 % faster up to 2048 wide, 3 to 20 % slower beyond).  Rows of
+    // no whole packs an element at a time up to 512 wide (65536 rows of 330: 62 + 177 us of kernels, in packs that begin anywhere 67 + 205; f32 46 + 212 and 81 + 273), and
+    // long ones of f32 (8192 rows of 4001: 145 and 398 us, in packs 186 and 586), but long ones of 16-bit numbers in packs (118 and 436, an element at a time 409 and 608).
     const bool pack8 = p.width > 256 && fits(8), pack4 = fits(4);
     if (p.width <= 512) {
         if (pack8) return block_short<X, B, 8, BACKWARD>(p, stream);
@@ -654,7 +654,7 @@ Block block_of(const lobpolicy_block* b) {
 // ---------------------------------------------------------------------------------------------------------------------------
 // the global norm, and clipping
 //
-// Two passes, each bound by memory (150 M values of both types, 457 MB: 101 us for the first, 4.5 TB/s, and 141 us for the second, 6.5 TB/s of reads
+// Two passes, each bound by memory (150 M values of both types, 457 MB: 100 us for the first, 4.6 TB/s, and 140 us for the second, 6.5 TB/s of reads
 // and writes, of which the caches hold some): the squares are summed in 64 bits (which neither overflows nor loses what many small gradients add), one
 // number per workgroup, in a fixed order; the second pass begins by adding those numbers up, in every workgroup alike, and scales.
 // The tensors' table travels as a kernel argument: nothing is copied to the device, and a captured graph holds it.

@@ -25,15 +25,16 @@ namespace lobpolicy {
 //
 // bf16: what multiplies a bf16 operand is split, so that a result is rounded once, as it is stored: scores and the state's copy that multiplies a into two
 // bf16 (the number, and what its rounding leaves: off by 2^-16 of a term), the weighted c of the state's update, which adds up over all steps, into
-// three (24 bits).  The second halves cost, whole calls: 4500 steps, 128 units of 128 to 128, with the gradients, 815 -> 890 us, a fifth of it the scores'; 128
-// steps, 2048 units of 64 to 64, forwards, 50 -> 57 us in chunks of 64, where they leave LDS for three workgroups instead of four, and 48 us in chunks of 32.
+// three (24 bits).  The second halves cost (kernels): 4500 steps, 128 units of 128 to 128, forwards 176 -> 199 us, the three walks of the backward pass 494 -> 561 us,
+// four fifths of it the state's; 128 steps, 2048 units of 64 to 64, forwards, 47 us in chunks of 64 without them, 46 us in chunks of 32 with them.
 //
-// Few chunks are bound by what a chunk's products wait for in turn, many by the issue of instructions: at 128 to 128 (bf16, 4500 steps, 128 units, three
-// walks of the backward pass in one launch, 485 us) the matrix units work 20 %, the vector units 32 %, LDS 26 % of the time.  Forwards, us:
-//     128 steps, 2048 units of 64 to 64, bf16      47    4.3 TB/s of operands, results and states
-//     20 steps, 16384 units of 32 to 32, f32       90    3.4 TB/s
-//     18000 steps, 8 units of 64 to 64, f32        82    24 the parts' states, 10 joined, 48 the outputs
-//     4500 steps, 128 units of 128 to 128, bf16   290    85, 19, 188
+// Few chunks are bound by what a chunk's products wait for in turn, many by the issue of instructions: at 128 to 128 (bf16, 4500 steps, 128 units, forwards and the
+// three walks) the matrix units work 21 %, the vector units 38 %, LDS 24 % of the time, at 1.5 waves to a SIMD; at 64 to 64 (bf16, 128 steps, 2048 units) 11, 53 and
+// 27 %.  Forwards, kernels, us:
+//     128 steps, 2048 units of 64 to 64, bf16      46    4.4 TB/s of operands, results and states
+//     20 steps, 16384 units of 32 to 32, f32       91    3.3 TB/s
+//     18000 steps, 8 units of 64 to 64, f32        81    22 the parts' states, 10 joined, 49 the outputs
+//     4500 steps, 128 units of 128 to 128, bf16   297    79, 19, 199
 // The token by token recurrence took 350 us of the first (the state's row in registers, a read and a write of LDS to each token) and 37 700 of the third.
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -146,7 +147,7 @@ struct Tile<bf16> {  // a fragment: 32 of the summed index, places 8 (lane / 16)
 template <class T, int CH, int DA, int DC>
 struct Shape {
     // tiles of 16 of the state's columns to a wave: each operand that waves share is read from LDS once for both (4096 steps, 128 units of 128 to 128,
-    // bf16: 248 us, with the gradients 743; one tile to a wave 292 and 936; at 64 columns two tiles leave two waves to a workgroup)
+    // bf16: 295 us, with the gradients 850; one tile to a wave 328 and 1060; at 64 columns two tiles leave two waves to a workgroup)
     static constexpr int COLS = DC == 128 ? 2 : 1;
     static constexpr int WAVES = DC / 16 / COLS, THREADS = 64 * WAVES;
     static constexpr int PAD = Tile<T>::PAD, SA = DA + PAD, SC = DC + PAD, SP = CH + PAD;
@@ -281,7 +282,7 @@ __device__ __forceinline__ void walk_part(const Scan& s, int64_t unit, int64_t p
     typedef Shape<T, CH, DA, DC> S;
     typedef Tile<T> M;
     typedef typename M::Frag Frag;
-    // whether the next chunk is on its way while one is computed: not where the registers end (128 to 128, the figures above: ahead 259 and 791 us)
+    // whether the next chunk is on its way while one is computed: not where the registers end (128 to 128, the case above: ahead 300 and 878 us)
     constexpr bool AHEAD = !OUT || DA + DC < 256;
     constexpr int KA = DA / M::K, KC = CH / M::K, DT = DA / 16, PER = M::K / 16, HALVES = M::HALVES, APART = CH * S::SP;
     T *const tile_a = room.a, *const tile_b = room.b, *const tile_c = room.c, *const tile_p = room.p;
@@ -636,7 +637,8 @@ __device__ __forceinline__ void walk_part(const Scan& s, int64_t unit, int64_t p
 //     dq_i = sum_j Z_ij k_j + scale l^(i+1) S0 do_i          dk_j = sum_i Z_ij q_i + l^(L-1-j) R v_j
 //     dv_j = sum_i A_ij do_i + l^(L-1-j) R^T k_j             dS0 = l^L R + scale sum_i l^(i+1) q_i do_i^T
 // Both score matrices lie in LDS by rows i: dq reads them by rows, dk and dv by columns.  Each wave has 16 columns of every result.  Three walks
-// read 9 operands instead of 4 and make 3 score matrices instead of 2: 20 steps x 4096 environments x 4 heads of 32 (f32) took 263 us that way, 181 us this (27 KB of LDS: 2.5 waves to a SIMD).
+// read 9 operands instead of 4 and make 3 score matrices instead of 2: 20 steps x 16384 units, with the forward pass, take
+// 314 us that way and 257 us this (32 to 32, f32: 27 KB of LDS, 2 waves to a SIMD), 195 and 169 us (32 to 32, bf16), 584 and 490 us (64 to 64, bf16).
 // A chunk with an infinity or a NaN is left to the walks.
 
 template <class T, int DK, int DV>
@@ -987,7 +989,7 @@ int scan_mode(const Walks& w, bool swapped, hipStream_t stream) {
 }
 
 // Whole packs of 16 bytes where every row begins and ends at one, packs that begin anywhere and shift their last where a row is one or longer (512 steps, 512
-// units of 61 to 61, forwards and with the gradients: bf16 56 + 170 us, an element at a time 98 + 328; f32 90 + 311 and 111 + 409), else elements
+// units of 61 to 61, forwards and with the gradients: bf16 62 and 195 us, an element at a time 95 and 332; f32 102 and 340, 124 and 433), else elements
 template <class T, int CH, int DA, int DC>
 int scan_aligned(const Walks& w, bool swapped, hipStream_t stream) {
     constexpr int W = 16 / sizeof(T);

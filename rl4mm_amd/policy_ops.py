@@ -6,7 +6,7 @@ asynchronously on torch's current stream of the tensors' device, like the tensor
   gated_residual_norm    a block's end: norm, gate, residual scale, and the norm before the next block; differentiable
   clip_grad_norm         the global gradient norm, and clipping by it
 
-float32 and bfloat16; states, norms and sums are float32 or wider.  There is no CPU path: CPU tensors raise, as does a missing
+float32 and bfloat16; states, norms and sums are float32 or wider, and a bfloat16 result is rounded once, as it is stored.  There is no CPU path: CPU tensors raise, as does a missing
 library.  Every call can be captured into a graph (nothing waits for the device, nothing is allocated but results and workspaces, through
 torch's allocator); a forward and a backward pass belong into the same capture, with no eager graph of the same leaves alive beside it, as torch
 asks of every operation.  torch.compile runs them between its graphs; forward-mode differentiation, torch.jit.trace and make_fx, which cannot see a
@@ -240,8 +240,9 @@ def decay_attention(q, k, v, log_decay, *, initial_state=None, reset=None, lengt
     q, k [T, N, H, dk], v [T, N, H, dv], float32 or bfloat16, time-major like the framework's traces; any strides, so they may be views of one
     projection's output.  log_decay [H] float32, a constant (no gradient).  reset [T, N] bool or uint8: token t is the first of a new episode, and
     nothing before it reaches it - not even a value that is not a number.  lengths [N] int32: environment n has that many tokens (clamped to 0 .. T);
-    what lies behind them is not read, its rows of ``out`` and of the gradients are 0, and the state is the one after its last token.  scale: dk ** -0.5
-    by default.  Gradients reach q, k, v and initial_state."""
+    what lies behind them is not used, its rows of ``out`` and of the gradients are 0, and the state is the one after its last token.  scale: dk ** -0.5
+    by default.  Gradients reach q, k, v and initial_state.  bfloat16: what lies between the operands and a result is held in 32 bits, or in two
+    bfloat16 that are off by 2^-16 of a term; decays are float32 exponentials, off by 2^-24 of them and of their exponent."""
     log_decay, scale = _heads(q, k, v, log_decay, initial_state, scale, ("T", "N", "H", "dk"))
     reset = _flags(reset, "reset", q.shape[:2], q.device)
     if lengths is not None:
@@ -348,7 +349,8 @@ def gated_residual_norm(x, block, gate, post_weight, residual_scale, pre_weight,
 
     x: the residual stream, float32 or bfloat16, y its type.  block: what the block put out; gate: its gate's logits (None: no gate); z has their type,
     float32 or bfloat16, and is taken from y before that is rounded.  The three weights: float32 [width].  width: 1 to 8192; rows of any stride.
-    Differentiable in all six; the weights' gradients are summed in a fixed order."""
+    Differentiable in all six; the weights' gradients are summed in a fixed order.  The gate's exponential and reciprocal are the hardware's: off by about
+    (1 + abs(gate)) 2^-23 of sigmoid(gate) and of its slope, however far open or shut the gate is."""
     weights = (post_weight, residual_scale, pre_weight)
     try:  # one look at all of it; what is wrong is found out below
         device, shape = x.device, x.shape

@@ -64,7 +64,7 @@ def _call(device, name, *args):
 
 _tracing, _modes = torch._C._is_tracing, torch._C._len_torch_dispatch_stack
 # the recorders that see operations before they are dispatched: the list itself, as looking it up takes longer than the rest of the check
-_early_modes = next(v for k, v in vars(torch._ops.mode_stack_state_for_pre_dispatch()).items() if k.endswith("infra_modes"))
+_early_modes = next((v for k, v in vars(torch._ops.mode_stack_state_for_pre_dispatch()).items() if k.endswith("infra_modes")), [])
 _NO_EARLY_MODES = [None] * len(_early_modes)
 
 

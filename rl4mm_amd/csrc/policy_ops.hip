@@ -32,20 +32,27 @@ int scan_typed(const Walks& w, bool swapped, hipStream_t stream) {
 // the last 88 workgroups run by themselves, 299).  Whole : split, us in a graph, forwards and with the gradients:
 //     32 to 32, bf16:   4096 steps, 32 units 233 : 30, 256 units 236 : 119, 384 units 267 : 227 and 597 : 621;  512 steps, 192 units 35 : 28 and 76 : 63
 //     64 to 64, bf16:   4096 steps, 75 units 275 : 82 and 553 : 238, 192 units 278 : 177 and 649 : 529, 220 units 279 : 215 and 653 : 592;  1024 steps, 192 units 77 : 59 and
-//                       181 : 170, 220 units 78 : 67 and 185 : 190;  512 steps, 100 units 41 : 33 and 89 : 79, 150 units 41 : 37 and 91 : 98
-//     64 to 64, f32:    4096 steps, 192 units 388 : 350 and 1153 : 1028, 220 units 397 : 405 and 1166 : 1179;  512 steps, 100 units 55 : 45 and 135 : 115, 150 units 56 : 57 and 138 : 155
-//     128 to 128, bf16: 4096 steps, 75 units 476 : 192 and 946 : 577, 150 units 486 : 347 and 1102 : 1069, 192 units 493 : 460 and 1497 : 1386;  1024 steps, 100 units 120 : 88 and
-//                       277 : 256, 192 units 127 : 142 and 396 : 434;  512 steps, 75 units 64 : 56 and 134 : 147, 100 units 65 : 60 and 153 : 173, 150 units 68 : 78 and 159 : 228
-//     128 to 128, f32:  4096 steps, 150 units 972 : 803 and 2558 : 2666, 192 units 984 : 1140 and 3457 : 3485
+//                       181 : 170, 220 units 78 : 67 and 185 : 190;  640 steps, 150 units 51 : 41 and 110 : 108, 190 units 51 : 46 and 121 : 129;  512 steps, 128 units 42 : 34 and 90 : 85,
+//                       150 units 41 : 37 and 91 : 98
+//     64 to 64, f32:    4096 steps, 192 units 388 : 350 and 1153 : 1028, 220 units 397 : 405 and 1166 : 1179;  512 steps, 128 units 56 : 48 and 138 : 130, 150 units 56 : 57 and 138 : 155
+//     107 to 53, bf16:  768 steps, 150 units 91 : 71 and 206 : 196, 190 units 93 : 93 and 233 : 248;  640 steps, 128 units 78 : 60 and 174 : 162, 150 units 79 : 71 and 175 : 192
+//     128 to 128, bf16: 4096 steps, 75 units 476 : 192 and 946 : 577, 150 units 486 : 347 and 1102 : 1069, 192 units 493 : 460 and 1497 : 1386;  1024 steps, 128 units 121 : 98 and
+//                       280 : 302, 150 units 122 : 119 and 286 : 369;  768 steps, 104 units 93 : 74 and 215 : 220, 128 units 94 : 81 and 218 : 253;  512 steps, 75 units 64 : 56 and 134 : 147,
+//                       100 units 65 : 60 and 153 : 173
+//     128 to 128, f32:  4096 steps, 150 units 972 : 803 and 2558 : 2666, 192 units 984 : 1140 and 3457 : 3485;  768 steps, 128 units 176 : 150 and 484 : 462, 150 units 181 : 187 and 493 : 565
 // 512 : 1024 workgroups in all, the latter where they are small: 4096 steps, 128 units of 64 to 64 (bf16) 139 : 124 and 380 : 368, 256 units of 32 to 32 200 : 120, 128 units of
 // 128 to 128 292 : 310 and 837 : 915.  Below 512 steps the two further launches take what the parts save (256 steps of 64 to 64, 32 units: 22.2 : 23.0; 512 steps: 39.0 : 25.3).
 struct Parts {
     int64_t steps;
     int count;
     Parts(const lobpolicy_attention* a) {
-        const int widest = a->dk > a->dv ? a->dk : a->dv;
+        const int widest = a->dk > a->dv ? a->dk : a->dv, narrowest = a->dk > a->dv ? a->dv : a->dk;
         const int64_t units = a->envs * a->heads, wanted = widest <= 64 ? 1024 : 512;
-        const int64_t most = widest <= 32 ? 384 : (widest <= 64 ? 208 : 160) / (a->steps < 1024 ? 2 : 1);  // units
+        int64_t most = 384;  // units
+        if (narrowest > 64)
+            most = a->steps < 1344 ? 48 + a->steps / 12 : 160;
+        else if (widest > 32)
+            most = (widest <= 64 ? 208 : 160) * (a->steps < 768 ? a->steps : 768) / 768;
         int64_t n = a->steps < 512 || units >= most ? 1 : wanted / units;
         n = n < ceil_div(a->steps, 128) ? n : ceil_div(a->steps, 128);
         steps = ceil_div(ceil_div(a->steps, n), 64) * 64;

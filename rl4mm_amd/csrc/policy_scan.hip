@@ -403,8 +403,8 @@ __device__ __forceinline__ void walk_part(const Scan& s, int64_t unit, int64_t p
                     const float far = it[u] - jt[u] > 1 ? power[16 * (it[u] - jt[u] - 1)] : 1.f;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        spoils = fmaf(x[u][r], 0.f, spoils);  // (the tiles on the diagonal see every row of a and b)
                         x[u][r] *= diagonal ? w_diagonal[r] : w_below[r] * far;
+                        spoils = fmaf(x[u][r], 0.f, spoils);  // (the tiles on the diagonal see every row of a and b; weighted, as halves of an infinity are none)
                     }
                     if (cuts) {
                         const uint64_t before = cuts & (~0ull >> (63 - i));
@@ -781,8 +781,8 @@ __global__ __launch_bounds__((DK > DV ? DK : DV) * 4) void gradients_once(Walks 
             T* to = (u ? s.z : s.a) + i * R::SP + 16 * jt + 4 * at.g;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                spoils = fmaf(x[u][r], 0.f, spoils);
                 const float y = x[u][r] * (it == jt ? w_diagonal[r] : w_below[r]);
+                spoils = fmaf(y, 0.f, spoils);
                 x[u][r] = 16 * jt + 4 * at.g + r >= from ? y : 0.f;
             }
             put_scores(to, R::APART, x[u]);

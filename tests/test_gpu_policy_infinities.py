@@ -63,3 +63,15 @@ def test_infinite_gradients(ops, steps, dtype):
     got = run(ops, p, dout, dlast)
     for key in ("dq", "dk", "dv", "dstate"):
         same_kind(got[key], want[key], tol[key], key)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("steps", [1, 5, 20, 32, 40, 100, 150, 700])
+@pytest.mark.parametrize("width", [32, 64, 128])
+def test_results_beyond_the_type(ops, width, steps, dtype):
+    """All operands 1 and a scale of 1e38: every result that has the scale once is more than 32 bits hold, and infinite; none is no number."""
+    q, k, v = (torch.ones(steps, 2, 1, width, dtype=dtype, device="cuda", requires_grad=True) for _ in range(3))
+    out, last = ops.decay_attention(q, k, v, torch.tensor([-0.01], device="cuda"), scale=1e38)
+    assert torch.isposinf(out).all() and torch.isfinite(last).all()
+    for g in torch.autograd.grad(out, (q, k, v), torch.ones_like(out)):
+        assert torch.isposinf(g).all()

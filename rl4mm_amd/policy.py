@@ -83,7 +83,9 @@ class SequencePolicy(torch.nn.Module):
         episodes begin; lengths [N] int32: how many steps of each environment there are; memory: what came before (empty without one).  Behind an
         environment's last step the observations may hold anything; the actions and values there are finite and mean nothing: leave them out of the loss."""
         after = []
-        behind = None if lengths is None else torch.arange(observations.shape[0], device=observations.device)[:, None] >= lengths
+        behind = None
+        if isinstance(lengths, torch.Tensor) and lengths.device == observations.device and lengths.shape == observations.shape[1:2]:  # (others the operator refuses)
+            behind = torch.arange(observations.shape[0], device=observations.device)[:, None] >= lengths
 
         def attend(i, q, k, v):
             out, state = ops.decay_attention(q, k, v, self.log_decay, initial_state=None if memory is None else memory[i], reset=reset, lengths=lengths)

@@ -85,3 +85,15 @@ def test_an_update_on_padded_segments():
     _, values, _ = policy(observations, lengths=lengths)
     norm = P.update(policy, torch.optim.SGD(policy.parameters(), lr=0.1), values[there].square().sum())
     assert torch.isfinite(norm) and all(torch.isfinite(p).all() for p in policy.parameters())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lengths, error", [(torch.zeros(N + 1, dtype=torch.int32), ValueError), (torch.zeros(N, dtype=torch.int32), ValueError), (torch.zeros(N), TypeError), ([1] * N, TypeError)],
+                         ids=["too many", "on the host", "type", "a list"])  # fmt: skip
+def test_lengths_that_are_none(lengths, error):
+    """refused by the operator, as without padding"""
+    policy = make("cuda")
+    if isinstance(lengths, torch.Tensor) and not (error is ValueError and len(lengths) == N):
+        lengths = lengths.cuda()
+    with pytest.raises(error):
+        policy(torch.randn(T, N, D, device="cuda"), lengths=lengths)
